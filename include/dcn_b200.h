@@ -49,6 +49,8 @@ enum { DCN_PATH_TCGEN05 = 1, DCN_PATH_SIMT_TILED = 2, DCN_PATH_SIMT_DIRECT = 3 }
 
 /* Epilogue applied to output channels [act_lo, act_hi) after bias. */
 enum { DCN_ACT_NONE = 0, DCN_ACT_SIGMOID = 1 };
+/* Activations of the matrix products (dcn_linear_*); GELU is the exact form z * Phi(z). */
+enum { DCN_ACT_RELU = 2, DCN_ACT_GELU = 3 };
 
 /*
  * One forward problem.  Tensor layouts are the reference's:
@@ -352,6 +354,70 @@ int dcn_msda_backward(const void *value, const int64_t *spatial_shapes, const in
                       int64_t batch, int64_t spatial_size, int64_t num_heads, int64_t channels,
                       int64_t num_levels, int64_t num_query, int64_t num_point, int32_t device,
                       void *stream);
+
+/*
+ * Matrix product with bias, activation and residual in its epilogue:
+ *     y[r, n] = act(sum_k x[r, k] * weight[n, k] + bias[n]) + residual[r, n]
+ * x is [rows, cin] with row stride ldx elements (>= cin), weight [cout, cin] with row stride ldw,
+ * residual [rows, cout] with row stride ldr, y [rows, cout] dense; all of element type `dtype`
+ * (DCN_DTYPE_*); bias and residual may be NULL; act is DCN_ACT_NONE, DCN_ACT_RELU or
+ * DCN_ACT_GELU.  Sums are held in fp32 and rounded once.  (The feed-forward and projection layers
+ * of mmcv/cnn/bricks/transformer.py and mmcv/ops/multi_scale_deform_attn.py:354-384, which call a
+ * library product and separate element-wise kernels.)
+ *
+ * saved (may be NULL): what the activation's derivative needs, for dcn_linear_backward.
+ *   RELU  uint32 words [rows][(cout + 31) / 32]; bit j % 32 of word j / 32 is set where the
+ *         pre-activation is not <= 0;
+ *   GELU  the pre-activation, [rows, cout] dense, element type `dtype`; NONE: not written.
+ *
+ * dcn_linear_backward, from gy = dL/dy [rows, cout] (row stride ldgy) and gz = gy * act'(z):
+ *     gx = (gz weight) * in_act'(in_saved) + gx_add      [rows, cin] dense
+ *     gw = gz^T x   [cout, cin] dense,     gb = sum_r gz [cout]
+ * gx, gw and gb may be NULL (not wanted); x may be NULL when gw is, weight when gx is.  in_act /
+ * in_saved apply the derivative of the activation that produced x (its own `saved` tensor), for a
+ * caller that runs two products back to back; DCN_ACT_NONE leaves it out.  gx_add [rows, cin]
+ * dense, or NULL.  The result does not depend on the order in which blocks run.
+ *
+ * The workspace is scratch, 256-byte aligned, of the size the two *_workspace_bytes functions
+ * report for the same arguments (alignment: the bitwise OR of the operands' addresses and of their
+ * row strides in bytes; only its low four bits count).  Asynchronous on `stream`, no allocation.
+ * rows may be 0: y is empty, gw and gb are zero.  One-time work per device (kernel attributes) is
+ * done by the first call on it, also inside a stream capture.
+ */
+int dcn_linear_workspace_bytes(int32_t dtype, int64_t rows, int64_t cin, int64_t cout, int64_t alignment,
+                               size_t *bytes);
+int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias,
+                       const void *residual, int64_t ldr, void *y, void *saved, int32_t dtype, int32_t act,
+                       int64_t rows, int64_t cin, int64_t cout, int32_t device, void *workspace,
+                       size_t workspace_bytes, void *stream);
+int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t cout,
+                                        int64_t alignment, int32_t want_gx, int32_t want_gw, size_t *bytes);
+int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
+                        int64_t ldw, const void *saved, const void *in_saved, const void *gx_add, void *gx,
+                        void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
+                        int64_t cin, int64_t cout, int32_t device, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/*
+ * Layer norm over the last dimension: n = (x - mean) / sqrt(var + eps), y = n * weight + bias,
+ * mean and (biased) variance of the row's `cols` elements in fp32.  x is [rows, cols] with row
+ * stride ldx, y dense, both of type `dtype`; weight and bias [cols] of type `wdtype` (`dtype` or
+ * DCN_DTYPE_F32), each may be NULL.  stats (may be NULL) receives 3 * rows floats for the backward
+ * pass: the mean, what its rounding to fp32 left out, and 1 / sqrt(var + eps).  (The 'LN' entry of
+ * mmcv/cnn/bricks/norm.py:14-26, a library layer there.)
+ *
+ * dcn_layer_norm_backward: gx [rows, cols] dense of type `dtype`, gw and gb [cols] of type
+ * `wdtype`; each may be NULL.  gw and gb are sums over the rows in a fixed order.  Workspace:
+ * dcn_layer_norm_workspace_bytes, 256-byte aligned.  rows may be 0: gw and gb are zero then.
+ */
+int dcn_layer_norm_forward(const void *x, int64_t ldx, const void *weight, const void *bias, void *y,
+                           float *stats, int32_t dtype, int32_t wdtype, int64_t rows, int64_t cols, float eps,
+                           int32_t device, void *stream);
+int dcn_layer_norm_workspace_bytes(int64_t rows, int64_t cols, size_t *bytes);
+int dcn_layer_norm_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
+                            const float *stats, void *gx, void *gw, void *gb, int32_t dtype, int32_t wdtype,
+                            int64_t rows, int64_t cols, int32_t device, void *workspace,
+                            size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,7 @@ DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 MATH_AUTO, MATH_FFMA, MATH_TF32X3, MATH_BF16 = 0, 1, 2, 3
 PATH_TCGEN05, PATH_SIMT_TILED, PATH_SIMT_DIRECT = 1, 2, 3
 ACT_NONE, ACT_SIGMOID = 0, 1
+ACT_RELU, ACT_GELU = 2, 3
 STATIC_SCRATCH_BYTES = 32 << 20
 ABI_VERSION = 6   # DCN_ABI_VERSION of include/dcn_b200.h (DcnFwdParams layout)
 
@@ -23,7 +24,10 @@ EXPORTS = ['dcn_abi_version', 'dcn_last_error', 'dcn_fwd_plan',
            'dcn_pad_channels_last', 'dcn_conv_workspace_bytes', 'dcn_conv_fwd', 'dcn_to_channels_last', 'dcn_bwd_columns', 'dcn_bwd_input',
            'dcn_bwd_coord',
            'dcn_modulated_deform_conv_forward', 'dcn_deform_conv_forward',
-           'dcn_forward_workspace_bytes', 'dcn_msda_forward', 'dcn_msda_backward']
+           'dcn_forward_workspace_bytes', 'dcn_msda_forward', 'dcn_msda_backward',
+           'dcn_linear_workspace_bytes', 'dcn_linear_forward',
+           'dcn_linear_backward_workspace_bytes', 'dcn_linear_backward',
+           'dcn_layer_norm_forward', 'dcn_layer_norm_workspace_bytes', 'dcn_layer_norm_backward']
 
 
 class DcnFwdParams(ctypes.Structure):
@@ -114,6 +118,18 @@ def load():
         [i32, i32] + [i64] * 5 + [i32] * 10 + [P(sz)])
     lib.dcn_msda_forward.argtypes = [vp] * 6 + [i32] + [i64] * 7 + [i32, vp]
     lib.dcn_msda_backward.argtypes = [vp] * 9 + [i32] + [i64] * 7 + [i32, vp]
+    f32 = ctypes.c_float
+    lib.dcn_linear_workspace_bytes.argtypes = [i32] + [i64] * 4 + [P(sz)]
+    lib.dcn_linear_forward.argtypes = (
+        [vp, i64, vp, i64, vp, vp, i64, vp, vp, i32, i32, i64, i64, i64, i32, vp, sz, vp])
+    lib.dcn_linear_backward_workspace_bytes.argtypes = [i32, i32] + [i64] * 4 + [i32, i32, P(sz)]
+    lib.dcn_linear_backward.argtypes = (
+        [vp, i64, vp, i64, vp, i64] + [vp] * 6 + [i32] * 3 + [i64] * 3 + [i32, vp, sz, vp])
+    lib.dcn_layer_norm_forward.argtypes = (
+        [vp, i64, vp, vp, vp, vp, i32, i32, i64, i64, f32, i32, vp])
+    lib.dcn_layer_norm_workspace_bytes.argtypes = [i64, i64, P(sz)]
+    lib.dcn_layer_norm_backward.argtypes = (
+        [vp, i64, vp, i64] + [vp] * 5 + [i32, i32, i64, i64, i32, vp, sz, vp])
     for name in EXPORTS:
         getattr(lib, name)  # raises AttributeError if a declared symbol is missing
         if name not in ('dcn_last_error',):

@@ -1,0 +1,504 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   forward   m = mean(x), d = x - m, c = mean(d), var = mean(d^2) - c^2, rstd = 1 / sqrt(var + eps)
+//             n = (d - c) rstd,  y = n w + b
+//   backward  g = gy w,  gx = rstd (g - mean(g) - n mean(g n)),  gw = sum_rows gy n,  gb = sum_rows gy
+//
+// m is rounded to fp32; c is what that rounding (and the rounding of the sum) left out.  With it a
+// row whose mean is large against its spread keeps its digits: the variance is taken around m + c,
+// never as a difference of large squares.  The statistics kept for the backward pass are m, c, rstd.
+//
+// Both passes read each tensor once: a row lives in the registers of a group of G threads (a warp up
+// to 1024 columns, a block of 256 up to 8192), E elements to a thread, loaded 16 bytes at a time
+// (one element at a time where sizes or alignment forbid it).  Bound: memory.
+// The backward pass keeps gw and gb in registers over all rows that a block takes, adds the warps of
+// a block in order, writes one partial row per block, and a second kernel adds those in order: the
+// result does not depend on when blocks run.
+#include <cstdint>
+#include <type_traits>
+
+#include "dcn_layers.cuh"
+
+namespace dcn {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPartials = 148 * 4;
+
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T *p, float (&o)[V]) {
+  if constexpr (V == 1) {
+    o[0] = ElemOf<T>::to(*p);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(p + i);
+      o[i] = v.x; o[i + 1] = v.y; o[i + 2] = v.z; o[i + 3] = v.w;
+    }
+  } else {
+    static_assert(V == 8, "sixteen bytes");
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        o[2 * i] = __uint_as_float(w[i] << 16);
+        o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        o[2 * i] = f.x;
+        o[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T *p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = ElemOf<T>::from(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4)
+      *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T lo = ElemOf<T>::from(v[2 * i]), hi = ElemOf<T>::from(v[2 * i + 1]);
+      w[i] = (uint32_t)*reinterpret_cast<uint16_t *>(&lo) | ((uint32_t)*reinterpret_cast<uint16_t *>(&hi) << 16);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// V weights (or biases) from either type; `none` where there is no tensor.
+template <typename T, int V>
+__device__ __forceinline__ void load_param(const void *p, bool f32, long long at, float none, float (&o)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = none;
+  } else if (f32) {
+    load_vec<float, V>((const float *)p + at, o);
+  } else {
+    load_vec<T, V>((const T *)p + at, o);
+  }
+}
+
+// Sums of N values over the G threads of a group; every thread gets them.
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float *smem) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+  if constexpr (G > 32) {
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();   // the values of an earlier call have been read
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) smem[warp * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < G / 32; ++w) v[i] += smem[w * N + i];
+    }
+  }
+}
+
+struct NormArgs {
+  const void *x, *gy, *w, *b;
+  void *y;
+  float *stats;        // [3][rows]: m, c, rstd
+  float *part;         // [gridDim.x][2][cols]: a block's sums for gw and gb
+  long long ldx, ldgy, rows;
+  int cols;
+  bool wf32;
+  float eps;
+};
+
+template <typename T, int V, int E, int G>
+__global__ void __launch_bounds__(kThreads) norm_forward(const NormArgs a) {
+  constexpr int NV = E / V;
+  __shared__ float red[(G > 32 ? G / 32 : 1) * 2];
+  const int t = threadIdx.x % G;
+  const long long row = blockIdx.x * (long long)(kThreads / G) + threadIdx.x / G;
+  if (row >= a.rows) return;   // whole groups leave together
+  const T *x = (const T *)a.x + row * a.ldx;
+  float v[NV][V];
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + t) * V;
+    if (c < a.cols) {
+      load_vec<T, V>(x + c, v[i]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] += v[i][e];
+    }
+  }
+  group_sum<G>(s, red);
+  const float inv = 1.f / (float)a.cols, m = s[0] * inv;
+  float q[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + t) * V;
+    if (c < a.cols)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[i][e] -= m;
+        q[0] += v[i][e];
+        q[1] = fmaf(v[i][e], v[i][e], q[1]);
+      }
+  }
+  group_sum<G>(q, red);
+  const float corr = q[0] * inv;
+  const float rstd = 1.f / sqrtf(fmaxf(q[1] * inv - corr * corr, 0.f) + a.eps);
+  // fmaxf drops a NaN; m carries it into every element of the row all the same
+  T *y = (T *)a.y + row * a.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + t) * V;
+    if (c < a.cols) {
+      float w[V], b[V];
+      load_param<T, V>(a.w, a.wf32, c, 1.f, w);
+      load_param<T, V>(a.b, a.wf32, c, 0.f, b);
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = fmaf((v[i][e] - corr) * rstd, w[e], b[e]);
+      store_vec<T, V>(y + c, w);
+    }
+  }
+  if (a.stats && t == 0) {
+    a.stats[row] = m;
+    a.stats[a.rows + row] = corr;
+    a.stats[2 * a.rows + row] = rstd;
+  }
+}
+
+template <typename T, int V, int E, int G, bool kParams>
+__global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
+  constexpr int NV = E / V, RPB = kThreads / G;
+  __shared__ float red[(G > 32 ? G / 32 : 1) * 2];
+  __shared__ float cols_s[G > 32 ? 1 : 2 * G * E];
+  const int t = threadIdx.x % G;
+  const float inv = 1.f / (float)a.cols;
+  float gw[kParams ? NV : 1][V] = {}, gb[kParams ? NV : 1][V] = {};
+  for (long long row = blockIdx.x * (long long)RPB + threadIdx.x / G; row < a.rows; row += (long long)gridDim.x * RPB) {
+    const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * a.ldgy;
+    float n[NV][V], g[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + t) * V;
+      if (c < a.cols) {
+        load_vec<T, V>(x + c, n[i]);
+        load_vec<T, V>(gy + c, g[i]);
+      }
+    }
+    const float m = a.stats[row], corr = a.stats[a.rows + row], rstd = a.stats[2 * a.rows + row];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + t) * V;
+      if (c < a.cols) {
+        float w[V];
+        load_param<T, V>(a.w, a.wf32, c, 1.f, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          n[i][e] = ((n[i][e] - m) - corr) * rstd;
+          if constexpr (kParams) {
+            gw[i][e] = fmaf(g[i][e], n[i][e], gw[i][e]);
+            gb[i][e] += g[i][e];
+          }
+          g[i][e] *= w[e];
+          s[0] += g[i][e];
+          s[1] = fmaf(g[i][e], n[i][e], s[1]);
+        }
+      }
+    }
+    group_sum<G>(s, red);
+    const float mg = s[0] * inv, mgn = s[1] * inv;
+    if (a.y) {
+      T *gx = (T *)a.y + row * a.cols;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + t) * V;
+        if (c < a.cols) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[i][e] = (g[i][e] - mg - n[i][e] * mgn) * rstd;
+          store_vec<T, V>(gx + c, g[i]);
+        }
+      }
+    }
+  }
+  if constexpr (kParams) {
+    float *out = a.part + (long long)blockIdx.x * 2 * a.cols;
+    if constexpr (G > 32) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + t) * V;
+        if (c < a.cols)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            out[c + e] = gw[i][e];
+            out[a.cols + c + e] = gb[i][e];
+          }
+      }
+    } else {
+      for (int w = 0; w < RPB; ++w) {   // the warps in order
+        if (threadIdx.x / G == w)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const int at = (i * G + t) * V + e;
+              cols_s[at] = gw[i][e] + (w ? cols_s[at] : 0.f);
+              cols_s[G * E + at] = gb[i][e] + (w ? cols_s[G * E + at] : 0.f);
+            }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+        out[c] = cols_s[c];
+        out[a.cols + c] = cols_s[G * E + c];
+      }
+    }
+  }
+}
+
+// Rows beyond 8192 columns: a block of 1024 threads reads its row three times (twice from cache).
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_forward_wide(const NormArgs a) {
+  __shared__ float red[32 * 2];
+  const long long row = blockIdx.x;
+  const T *x = (const T *)a.x + row * a.ldx;
+  float s[1] = {0.f};
+  for (int c = threadIdx.x; c < a.cols; c += 1024) s[0] += ElemOf<T>::to(x[c]);
+  group_sum<1024>(s, red);
+  const float inv = 1.f / (float)a.cols, m = s[0] * inv;
+  float q[2] = {0.f, 0.f};
+  for (int c = threadIdx.x; c < a.cols; c += 1024) {
+    const float d = ElemOf<T>::to(x[c]) - m;
+    q[0] += d;
+    q[1] = fmaf(d, d, q[1]);
+  }
+  group_sum<1024>(q, red);
+  const float corr = q[0] * inv;
+  const float rstd = 1.f / sqrtf(fmaxf(q[1] * inv - corr * corr, 0.f) + a.eps);
+  T *y = (T *)a.y + row * a.cols;
+  for (int c = threadIdx.x; c < a.cols; c += 1024) {
+    float w[1], b[1];
+    load_param<T, 1>(a.w, a.wf32, c, 1.f, w);
+    load_param<T, 1>(a.b, a.wf32, c, 0.f, b);
+    y[c] = ElemOf<T>::from(fmaf((ElemOf<T>::to(x[c]) - m - corr) * rstd, w[0], b[0]));
+  }
+  if (a.stats && threadIdx.x == 0) {
+    a.stats[row] = m;
+    a.stats[a.rows + row] = corr;
+    a.stats[2 * a.rows + row] = rstd;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_backward_wide(const NormArgs a) {
+  __shared__ float red[32 * 2];
+  const long long row = blockIdx.x;
+  const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * a.ldgy;
+  const float m = a.stats[row], corr = a.stats[a.rows + row], rstd = a.stats[2 * a.rows + row];
+  float s[2] = {0.f, 0.f};
+  for (int c = threadIdx.x; c < a.cols; c += 1024) {
+    float w[1];
+    load_param<T, 1>(a.w, a.wf32, c, 1.f, w);
+    const float g = ElemOf<T>::to(gy[c]) * w[0];
+    s[0] += g;
+    s[1] = fmaf(g, (ElemOf<T>::to(x[c]) - m - corr) * rstd, s[1]);
+  }
+  group_sum<1024>(s, red);
+  const float inv = 1.f / (float)a.cols, mg = s[0] * inv, mgn = s[1] * inv;
+  T *gx = (T *)a.y + row * a.cols;
+  for (int c = threadIdx.x; c < a.cols; c += 1024) {
+    float w[1];
+    load_param<T, 1>(a.w, a.wf32, c, 1.f, w);
+    const float n = (ElemOf<T>::to(x[c]) - m - corr) * rstd;
+    gx[c] = ElemOf<T>::from((ElemOf<T>::to(gy[c]) * w[0] - mg - n * mgn) * rstd);
+  }
+}
+
+// ... and their gw and gb: a thread owns a column, blockIdx.y a slab of rows
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_columns_wide(const NormArgs a) {
+  const int c = blockIdx.x * kThreads + threadIdx.x;
+  if (c >= a.cols) return;
+  float gw = 0.f, gb = 0.f;
+  for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float g = ElemOf<T>::to(((const T *)a.gy)[row * a.ldgy + c]);
+    const float n = (ElemOf<T>::to(((const T *)a.x)[row * a.ldx + c]) - a.stats[row] - a.stats[a.rows + row]) *
+                    a.stats[2 * a.rows + row];
+    gw = fmaf(g, n, gw);
+    gb += g;
+  }
+  a.part[(long long)blockIdx.y * 2 * a.cols + c] = gw;
+  a.part[((long long)blockIdx.y * 2 + 1) * a.cols + c] = gb;
+}
+
+// out[c] = sum over the partial rows, 32 of them side by side; blockIdx.y: 0 gw, 1 gb
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ part, int parts, int cols, T *gw, T *gb) {
+  __shared__ float s[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
+  T *out = blockIdx.y ? gb : gw;
+  if (!out) return;
+  float v = 0.f;
+  if (c < cols)
+    for (int p = ty; p < parts; p += 32) v += part[((long long)p * 2 + blockIdx.y) * cols + c];
+  s[ty][tx] = v;
+  __syncthreads();
+  for (int d = 16; d > 0; d >>= 1) {
+    if (ty < d) s[ty][tx] += s[ty + d][tx];
+    __syncthreads();
+  }
+  if (ty == 0 && c < cols) out[c] = ElemOf<T>::from(s[0][tx]);
+}
+
+template <typename T, int V, int E, int G>
+cudaError_t run_one(const NormArgs &a, bool backward, bool params, int grid, cudaStream_t s) {
+  if (!backward) norm_forward<T, V, E, G><<<grid, kThreads, 0, s>>>(a);
+  else if (params) norm_backward<T, V, E, G, true><<<grid, kThreads, 0, s>>>(a);
+  else norm_backward<T, V, E, G, false><<<grid, kThreads, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+// E: the fewest elements to a thread that hold the row; G: a warp while that is at most 32.
+template <typename T, int V>
+cudaError_t run_rows(const NormArgs &a, bool backward, bool params, int *parts, cudaStream_t s) {
+  const int G = a.cols <= 1024 ? 32 : 256, E = (a.cols + G - 1) / G;
+  const long long rpb = kThreads / G;
+  long long grid = (a.rows + rpb - 1) / rpb;
+  if (backward && grid > kMaxPartials) grid = kMaxPartials;
+  *parts = (int)grid;
+  if (G == 32) {
+    if (E <= 8) return run_one<T, V, 8, 32>(a, backward, params, (int)grid, s);
+    if (E <= 16) return run_one<T, V, 16, 32>(a, backward, params, (int)grid, s);
+    return run_one<T, V, 32, 32>(a, backward, params, (int)grid, s);
+  }
+  if (E <= 8) return run_one<T, V, 8, 256>(a, backward, params, (int)grid, s);
+  if (E <= 16) return run_one<T, V, 16, 256>(a, backward, params, (int)grid, s);
+  return run_one<T, V, 32, 256>(a, backward, params, (int)grid, s);
+}
+
+template <typename T>
+cudaError_t run(const NormArgs &a, bool backward, bool params, int *parts, cudaStream_t s) {
+  if (a.cols > 8192) {
+    if (!backward) {
+      norm_forward_wide<T><<<(int)a.rows, 1024, 0, s>>>(a);
+      return cudaGetLastError();
+    }
+    if (a.y) norm_backward_wide<T><<<(int)a.rows, 1024, 0, s>>>(a);
+    if (params) {
+      *parts = (int)(a.rows < 64 ? a.rows : 64);
+      norm_columns_wide<T><<<dim3((a.cols + kThreads - 1) / kThreads, *parts), kThreads, 0, s>>>(a);
+    }
+    return cudaGetLastError();
+  }
+  // 16-byte accesses need every row of every tensor to start on 16 bytes; the dense output's does
+  // when cols is a multiple of V
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = a.cols % V == 0 && a.ldx % V == 0 && (!backward || a.ldgy % V == 0) && aligned16(a.x) &&
+                   aligned16(a.y) && aligned16(a.w) && aligned16(a.b) && (!backward || aligned16(a.gy));
+  return vec ? run_rows<T, V>(a, backward, params, parts, s) : run_rows<T, 1>(a, backward, params, parts, s);
+}
+
+cudaError_t run_typed(const NormArgs &a, int dtype, bool backward, bool params, int *parts, cudaStream_t s) {
+  if (dtype == DCN_DTYPE_F32) return run<float>(a, backward, params, parts, s);
+  if (dtype == DCN_DTYPE_BF16) return run<__nv_bfloat16>(a, backward, params, parts, s);
+  return run<__half>(a, backward, params, parts, s);
+}
+
+int check(int32_t dtype, int32_t wdtype, int64_t rows, int64_t cols) {
+  if (dtype != DCN_DTYPE_F32 && dtype != DCN_DTYPE_BF16 && dtype != DCN_DTYPE_F16)
+    return set_error(DCN_ERR_UNSUPPORTED, "layer norm: fp32, bf16 and fp16 tensors only");
+  if (wdtype != dtype && wdtype != DCN_DTYPE_F32)
+    return set_error(DCN_ERR_ARG, "layer norm: weight and bias must have x's type or fp32");
+  if (rows < 0 || cols <= 0) return set_error(DCN_ERR_ARG, "layer norm: cols must be positive, rows must not be negative");
+  if (rows > 2147483647LL || cols > (1 << 24))
+    return set_error(DCN_ERR_UNSUPPORTED, "layer norm: at most 2^31 - 1 rows and 2^24 columns");
+  return DCN_OK;
+}
+
+size_t workspace_of(int64_t rows, int64_t cols) {
+  return (size_t)(rows < kMaxPartials ? rows : kMaxPartials) * 2 * (size_t)cols * sizeof(float);
+}
+
+}  // namespace
+}  // namespace dcn
+
+using namespace dcn;
+
+extern "C" {
+
+int dcn_layer_norm_forward(const void *x, int64_t ldx, const void *weight, const void *bias, void *y,
+                           float *stats, int32_t dtype, int32_t wdtype, int64_t rows, int64_t cols, float eps,
+                           int32_t device, void *stream) {
+  int rc = check(dtype, wdtype, rows, cols);
+  if (rc) return rc;
+  if (rows == 0) return DCN_OK;
+  if (!x || !y) return set_error(DCN_ERR_ARG, "layer norm: x and y must be non-NULL");
+  if (ldx < cols) return set_error(DCN_ERR_ARG, "layer norm: the row stride is smaller than the row");
+  LayerDeviceScope scope(device);
+  if (scope.err != cudaSuccess) return set_error(DCN_ERR_CUDA, cudaGetErrorString(scope.err));
+  NormArgs a = {};
+  a.x = x; a.w = weight; a.b = bias; a.y = y; a.stats = stats;
+  a.ldx = ldx; a.rows = rows; a.cols = (int)cols; a.wf32 = wdtype == DCN_DTYPE_F32; a.eps = eps;
+  int parts = 0;
+  const cudaError_t e = run_typed(a, dtype, false, false, &parts, (cudaStream_t)stream);
+  return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int dcn_layer_norm_workspace_bytes(int64_t rows, int64_t cols, size_t *bytes) {
+  if (!bytes) return set_error(DCN_ERR_ARG, "layer norm: bytes is NULL");
+  int rc = check(DCN_DTYPE_F32, DCN_DTYPE_F32, rows, cols);
+  if (rc) return rc;
+  *bytes = workspace_of(rows, cols);
+  return DCN_OK;
+}
+
+int dcn_layer_norm_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
+                            const float *stats, void *gx, void *gw, void *gb, int32_t dtype, int32_t wdtype,
+                            int64_t rows, int64_t cols, int32_t device, void *workspace,
+                            size_t workspace_bytes, void *stream) {
+  int rc = check(dtype, wdtype, rows, cols);
+  if (rc) return rc;
+  LayerDeviceScope scope(device);
+  if (scope.err != cudaSuccess) return set_error(DCN_ERR_CUDA, cudaGetErrorString(scope.err));
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e = cudaSuccess;
+  if (rows == 0) {
+    const size_t n = (size_t)cols * (wdtype == DCN_DTYPE_F32 ? 4 : 2);
+    if (gw) e = cudaMemsetAsync(gw, 0, n, s);
+    if (e == cudaSuccess && gb) e = cudaMemsetAsync(gb, 0, n, s);
+    return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
+  }
+  if (!gx && !gw && !gb) return DCN_OK;
+  if (!gy || !x || !stats) return set_error(DCN_ERR_ARG, "layer norm backward: gy, x and stats must be non-NULL");
+  if (ldx < cols || ldgy < cols)
+    return set_error(DCN_ERR_ARG, "layer norm backward: a row stride is smaller than the row");
+  const bool params = gw || gb;
+  if (params && (!workspace || workspace_bytes < workspace_of(rows, cols) || ((uintptr_t)workspace & 255)))
+    return set_error(DCN_ERR_WORKSPACE, "layer norm backward: workspace missing, too small or misaligned");
+  NormArgs a = {};
+  a.x = x; a.gy = gy; a.w = weight; a.y = gx; a.stats = const_cast<float *>(stats); a.part = (float *)workspace;
+  a.ldx = ldx; a.ldgy = ldgy; a.rows = rows; a.cols = (int)cols; a.wf32 = wdtype == DCN_DTYPE_F32;
+  int parts = 0;
+  e = run_typed(a, dtype, true, params, &parts, s);
+  if (e == cudaSuccess && params) {
+    const dim3 grid((unsigned)((cols + 31) / 32), 2);
+    if (wdtype == DCN_DTYPE_F32) norm_reduce<float><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (float *)gw, (float *)gb);
+    else if (wdtype == DCN_DTYPE_BF16)
+      norm_reduce<__nv_bfloat16><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (__nv_bfloat16 *)gw, (__nv_bfloat16 *)gb);
+    else norm_reduce<__half><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (__half *)gw, (__half *)gb);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,6 +1,10 @@
 """The deformable-convolution names of ``mmcv.ops`` and their sibling sampler (reference:
-mmcv/ops/__init__.py)."""
+mmcv/ops/__init__.py), and the operators of the transformer layer around that sampler."""
 from .deform_conv import DeformConv2d, DeformConv2dFunction, DeformConv2dPack, deform_conv2d
+from .deformable_encoder_layer import DeformableEncoderLayer
+from .fused_linear import (FFN, FeedForwardFunction, FusedLinear, FusedLinearFunction, feed_forward,
+                           fused_linear)
+from .layer_norm import LayerNorm, LayerNormFunction, layer_norm
 from .modulated_deform_conv import (ModulatedDeformConv2d, ModulatedDeformConv2dFunction,
                                     ModulatedDeformConv2dPack, modulated_deform_conv2d)
 from .multi_scale_deform_attn import (MultiScaleDeformableAttention,
@@ -10,4 +14,7 @@ from .saconv import SAConv2d
 __all__ = ['DeformConv2d', 'DeformConv2dFunction', 'DeformConv2dPack', 'deform_conv2d',
            'ModulatedDeformConv2d', 'ModulatedDeformConv2dFunction',
            'ModulatedDeformConv2dPack', 'modulated_deform_conv2d', 'SAConv2d',
-           'MultiScaleDeformableAttention', 'MultiScaleDeformableAttnFunction']
+           'MultiScaleDeformableAttention', 'MultiScaleDeformableAttnFunction',
+           'DeformableEncoderLayer', 'FFN', 'FeedForwardFunction', 'FusedLinear',
+           'FusedLinearFunction', 'feed_forward', 'fused_linear', 'LayerNorm', 'LayerNormFunction',
+           'layer_norm']

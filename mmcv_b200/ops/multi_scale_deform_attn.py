@@ -15,6 +15,7 @@ import torch.nn as nn
 from torch.autograd.function import Function, once_differentiable
 
 from .. import _ext as ext_module
+from .fused_linear import fused_linear
 from .modulated_deform_conv import register_layer
 
 
@@ -63,12 +64,16 @@ def _is_power_of_2(n):
 class MultiScaleDeformableAttention(nn.Module):
     """The attention module of Deformable DETR: same constructor arguments, parameters
     (``sampling_offsets``, ``attention_weights``, ``value_proj``, ``output_proj``), initialisation
-    and forward arithmetic as the reference layer (mmcv/ops/multi_scale_deform_attn.py:172-384)."""
+    and forward arithmetic as the reference layer (mmcv/ops/multi_scale_deform_attn.py:172-384).
+
+    fused_proj (not in the reference): the four projections run on this library's matrix product
+    (``fused_linear``), the last one with the identity in its epilogue while no dropout is active.
+    The sums are the same, rounded once where the default rounds twice."""
 
     def __init__(self, embed_dims: int = 256, num_heads: int = 8, num_levels: int = 4,
                  num_points: int = 4, im2col_step: int = 64, dropout: float = 0.1,
                  batch_first: bool = False, norm_cfg: Optional[dict] = None, init_cfg=None,
-                 value_proj_ratio: float = 1.0):
+                 value_proj_ratio: float = 1.0, fused_proj: bool = False):
         super().__init__()
         if embed_dims % num_heads != 0:
             raise ValueError(f'embed_dims must be divisible by num_heads, '
@@ -78,6 +83,7 @@ class MultiScaleDeformableAttention(nn.Module):
         self.init_cfg = init_cfg
         self.dropout = nn.Dropout(dropout)
         self.batch_first = batch_first
+        self.fused_proj = fused_proj
         if not _is_power_of_2(dim_per_head):
             warnings.warn("You'd better set embed_dims in MultiScaleDeformAttention to make the "
                           'dimension of each attention head a power of 2 which is more efficient '
@@ -113,6 +119,9 @@ class MultiScaleDeformableAttention(nn.Module):
         nn.init.constant_(self.output_proj.bias, 0.)
         self._is_init = True
 
+    def _project(self, linear, x):
+        return fused_linear(x, linear.weight, linear.bias) if self.fused_proj else linear(x)
+
     def forward(self, query, key=None, value=None, identity=None, query_pos=None,
                 key_padding_mask=None, reference_points=None, spatial_shapes=None,
                 level_start_index=None, **kwargs):
@@ -131,13 +140,13 @@ class MultiScaleDeformableAttention(nn.Module):
         bs, num_value, _ = value.shape
         assert (spatial_shapes[:, 0] * spatial_shapes[:, 1]).sum() == num_value
 
-        value = self.value_proj(value)
+        value = self._project(self.value_proj, value)
         if key_padding_mask is not None:
             value = value.masked_fill(key_padding_mask[..., None], 0.0)
         value = value.view(bs, num_value, self.num_heads, -1)
-        sampling_offsets = self.sampling_offsets(query).view(
+        sampling_offsets = self._project(self.sampling_offsets, query).view(
             bs, num_query, self.num_heads, self.num_levels, self.num_points, 2)
-        attention_weights = self.attention_weights(query).view(
+        attention_weights = self._project(self.attention_weights, query).view(
             bs, num_query, self.num_heads, self.num_levels * self.num_points)
         attention_weights = attention_weights.softmax(-1)
         attention_weights = attention_weights.view(bs, num_query, self.num_heads,
@@ -158,7 +167,12 @@ class MultiScaleDeformableAttention(nn.Module):
         output = MultiScaleDeformableAttnFunction.apply(
             value.contiguous(), spatial_shapes, level_start_index, sampling_locations.contiguous(),
             attention_weights.contiguous(), self.im2col_step)
-        output = self.output_proj(output)
+        if self.fused_proj and (self.dropout.p == 0 or not self.training):
+            if not self.batch_first:
+                identity = identity.permute(1, 0, 2)
+            output = fused_linear(output, self.output_proj.weight, self.output_proj.bias, identity)
+            return output if self.batch_first else output.permute(1, 0, 2)
+        output = self._project(self.output_proj, output)
         if not self.batch_first:
             output = output.permute(1, 0, 2)
         return self.dropout(output) + identity

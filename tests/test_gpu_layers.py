@@ -1,0 +1,455 @@
+"""The transformer-layer operators on the GPU against 64-bit forms, element by element within bounds
+that oracle/layers.py derives from the roundings: fused_linear, feed_forward, layer_norm, the layers
+that call them, and a whole encoder layer."""
+import pytest
+import torch
+
+from mmcv_b200 import ops
+from oracle import layers as plain
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def tensors(seed, dtype, *shapes, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    return [None if s is None else (torch.randn(s, generator=gen) * scale).to(dtype).cuda() for s in shapes]
+
+
+def hold(got, want):
+    for key, value in want.items():
+        over = plain.excess(got[key], value)
+        assert over <= 1.0, f'{key}: {over:.3g} of its bound'
+
+
+def linear_case(rows, cin, cout, dtype, act, bias=True, res=True, seed=0):
+    x, r, gy = tensors(seed, dtype, (rows, cin), (rows, cout) if res else None, (rows, cout))
+    w, b = tensors(seed + 1, dtype, (cout, cin), (cout,) if bias else None, scale=cin ** -0.5)
+    return x, w, b, r, gy
+
+
+def run_linear(x, w, b, r, gy, act):
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w, b, r)]
+    y = ops.fused_linear(leaves[0], leaves[1], leaves[2], residual=leaves[3], activation=act)
+    given = [t for t in leaves if t is not None]
+    grads = dict(zip([n for n, t in zip(('gx', 'gw', 'gb', 'gr'), leaves) if t is not None],
+                     torch.autograd.grad(y, given, gy)))
+    return {'y': y.detach(), **grads}
+
+
+SIZES = [(1, 256, 1024), (1, 1, 1), (3, 8, 8), (5, 7, 3), (8, 100, 130), (9, 64, 64), (64, 40, 200),
+         (129, 72, 136), (300, 256, 1024), (257, 250, 387), (130, 520, 264), (1000, 1032, 72), (2500, 96, 40)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,cout', SIZES)
+def test_linear_forward_and_gradients(rows, cin, cout, dtype):
+    for k, (act, bias, res) in enumerate([(None, True, False), ('relu', True, True), ('gelu', False, True),
+                                          (None, False, False)]):
+        x, w, b, r, gy = linear_case(rows, cin, cout, dtype, act, bias, res, seed=k)
+        want = plain.linear(x, w, b, r, act, gy)
+        if b is None:
+            want.pop('gb')
+        got = run_linear(x, w, b, r, gy, act)
+        hold(got, want)
+        if r is not None:
+            assert torch.equal(got['gr'], gy)
+        with torch.no_grad():   # the serving call gives the same bits
+            assert torch.equal(ops.fused_linear(x, w, b, r, act), got['y'])
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_linear_many_rows_and_splits(dtype):
+    """Enough rows that the weight gradient's sum is divided among blocks."""
+    for rows, cin, cout, act in [(20011, 64, 72, 'gelu'), (6000, 256, 264, 'relu'), (3000, 130, 33, None)]:
+        x, w, b, r, gy = linear_case(rows, cin, cout, dtype, act)
+        got = run_linear(x, w, b, r, gy, act)
+        hold(got, plain.linear(x, w, b, r, act, gy))
+        again = run_linear(x, w, b, r, gy, act)
+        assert all(torch.equal(got[k], again[k]) for k in got)   # no order left to chance
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_linear_strides_and_alignment(dtype):
+    """Row strides, views that start off a 16-byte boundary, a transposed weight, expanded gradients
+    and residuals, leading dimensions."""
+    rows, cin, cout = 77, 48, 56
+    wide, = tensors(3, dtype, (rows, 128))
+    w_big, b, gy = tensors(4, dtype, (64, 80), (cout,), (rows, cout))
+    for x in (wide[:, :cin], wide[:, 8:8 + cin], wide[:, 3:3 + cin], wide[::2][:, 1:1 + cin],
+              wide.t()[:cin].t(), wide[:1, :cin].expand(rows, cin)):
+        for w in (w_big[:cout, :cin], w_big[1:1 + cout, 5:5 + cin], w_big.t()[:cin, :cout].t(),
+                  w_big[:cin, :cout].t()):
+            g = gy[:x.shape[0]]
+            hold(run_linear(x, w, b, None, g, 'gelu'), plain.linear(x, w, b, None, 'gelu', g))
+    x, w = wide[:, :cin].reshape(7, 11, cin), w_big[:cout, :cin]
+    res, = tensors(5, dtype, (11, 1))
+    leaf, rleaf = x.detach().requires_grad_(True), res.detach().requires_grad_(True)
+    y = ops.fused_linear(leaf, w, b[::1], rleaf, 'relu')
+    assert y.shape == (7, 11, cout)
+    y.sum().backward()      # an expanded gradient
+    want = plain.linear(x.reshape(-1, cin), w, b, res.expand(7, 11, cout).reshape(-1, cout), 'relu',
+                        torch.ones(rows, cout, dtype=dtype, device='cuda'))
+    hold({'y': y.detach().reshape(rows, cout), 'gx': leaf.grad.reshape(rows, cin)}, {k: want[k] for k in ('y', 'gx')})
+    assert torch.equal(rleaf.grad, torch.full_like(res, 7 * cout))
+
+
+def test_linear_partial_gradients_and_empty_batch():
+    x, w, b, r, gy = linear_case(40, 24, 32, torch.bfloat16, 'gelu')
+    full = run_linear(x, w, b, r, gy, 'gelu')
+    for mask in range(1, 16):
+        leaves = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b, r))]
+        y = ops.fused_linear(*leaves, activation='gelu')
+        y.backward(gy)
+        for name, t in zip(('gx', 'gw', 'gb', 'gr'), leaves):
+            if t.requires_grad:
+                if name == 'gb' and not leaves[1].requires_grad:
+                    hold({'gb': t.grad}, {'gb': plain.linear(x, w, b, r, 'gelu', gy)['gb']})
+                else:
+                    assert torch.equal(t.grad, full[name]), (mask, name)
+            else:
+                assert t.grad is None
+    leaves = [t.detach().requires_grad_(True) for t in (x[:0], w, b)]
+    y = ops.fused_linear(*leaves, activation='relu')
+    assert y.shape == (0, 32)
+    y.sum().backward()
+    assert leaves[0].grad.shape == (0, 24) and not leaves[1].grad.any() and not leaves[2].grad.any()
+
+
+def test_linear_non_finite_rows_stay_alone():
+    """A NaN row of x reaches its own row of y only; NaN passes relu and gelu."""
+    for dtype in DTYPES:
+        x, w, b, _, _ = linear_case(200, 64, 136, dtype, 'relu')
+        x = x.clone()
+        x[37] = float('nan')
+        for act in (None, 'relu', 'gelu'):
+            y = ops.fused_linear(x, w, b, activation=act)
+            bad = torch.isnan(y).all(1)
+            assert bad[37] and int(torch.isnan(y).any(1).sum()) == 1
+
+
+def test_linear_gradient_against_differences():
+    """The directional derivative of sum(y * gy) along random directions, by central differences of
+    the 64-bit form; the gradients are fp32: relative error of a sum of n products, and the
+    differences' own h^2."""
+    x, w, b, r, gy = linear_case(50, 40, 30, torch.float32, 'gelu')
+    got = run_linear(x, w, b, r, gy, 'gelu')
+    d = tensors(9, torch.float64, x.shape, w.shape, b.shape)
+    h = 1e-4
+
+    def f(s):
+        z = (x.double() + s * d[0]) @ (w.double() + s * d[1]).t() + b.double() + s * d[2]
+        return (plain.activation(z, 'gelu')[0] * gy.double()).sum()
+
+    slope = ((f(h) - f(-h)) / (2 * h)).item()
+    mine = sum((got[k].double() * v).sum().item() for k, v in zip(('gx', 'gw', 'gb'), d))
+    size = sum((got[k].double() * v).abs().sum().item() for k, v in zip(('gx', 'gw', 'gb'), d))
+    assert abs(mine - slope) <= 1e-5 * size
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,hidden', [(1, 16, 32), (300, 256, 1024), (45, 33, 70), (2049, 64, 96)])
+def test_feed_forward(rows, cin, hidden, dtype):
+    for act in ('relu', 'gelu'):
+        x, r, gy = tensors(1, dtype, (rows, cin), (rows, cin), (rows, cin))
+        w1, w2 = tensors(2, dtype, (hidden, cin), (cin, hidden), scale=(cin + hidden) ** -0.5)
+        b1, b2 = tensors(3, dtype, (hidden,), (cin,), scale=0.1)
+        want = plain.feed_forward(x, w1, b1, w2, b2, r, act, gy)
+        leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2, r)]
+        y = ops.feed_forward(*leaves, activation=act)
+        grads = torch.autograd.grad(y, leaves, gy)
+        hold({'y': y.detach(), **dict(zip(('gx', 'gw1', 'gb1', 'gw2', 'gb2'), grads))}, want)
+        assert torch.equal(grads[5], gy)
+        with torch.no_grad():
+            assert torch.equal(ops.feed_forward(x, w1, b1, w2, b2, r, act), y.detach())
+        # the input as its own residual: one gradient, both parts in it
+        leaf = x.detach().requires_grad_(True)
+        y = ops.feed_forward(leaf, w1, b1, w2, b2, leaf, act)
+        g, = torch.autograd.grad(y, leaf, gy)
+        both = plain.feed_forward(x, w1, b1, w2, b2, x, act, gy)
+        gx = plain.add(plain.Value(both['gx'].v, both['gx'].e), gy.double())
+        hold({'y': y.detach(), 'gx': g}, {'y': both['y'], 'gx': gx.rounded(dtype)})
+
+
+NORM_SIZES = [(1, 1), (1, 256), (3, 8), (300, 256), (77, 100), (9, 1024), (5, 1537), (40, 2048), (3, 8192), (2, 8200),
+              (3, 9001), (5000, 64), (1203, 384), (700, 4096)]
+
+
+def norm_case(rows, cols, dtype, wdtype=None, shift=0.0, seed=0):
+    x, gy = tensors(seed, dtype, (rows, cols), (rows, cols))
+    w, b = tensors(seed + 1, wdtype or dtype, (cols,), (cols,))
+    return x + shift, w, b, gy
+
+
+def run_norm(x, w, b, gy, eps=1e-5):
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w, b)]
+    y = ops.layer_norm(leaves[0], x.shape[1:], leaves[1], leaves[2], eps)
+    given = [t for t in leaves if t is not None]
+    grads = dict(zip([n for n, t in zip(('gx', 'gw', 'gb'), leaves) if t is not None],
+                     torch.autograd.grad(y, given, gy)))
+    return {'y': y.detach(), **grads}
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cols', NORM_SIZES)
+def test_norm_forward_and_gradients(rows, cols, dtype):
+    x, w, b, gy = norm_case(rows, cols, dtype)
+    got = run_norm(x, w, b, gy)
+    hold(got, plain.layer_norm(x, w, b, 1e-5, gy))
+    with torch.no_grad():
+        assert torch.equal(ops.layer_norm(x, (cols,), w, b), got['y'])
+    again = run_norm(x, w, b, gy)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+    plain_only = run_norm(x, None, None, gy)
+    hold(plain_only, {k: v for k, v in plain.layer_norm(x, None, None, 1e-5, gy).items() if k in ('y', 'gx')})
+
+
+def test_norm_mixed_parameter_type_and_partial_gradients():
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w, b, gy = norm_case(70, 264, dtype, torch.float32)
+        got = run_norm(x, w, b, gy)
+        assert got['gw'].dtype == torch.float32 and got['y'].dtype == dtype
+        hold(got, plain.layer_norm(x, w, b, 1e-5, gy))
+    for mask in range(1, 8):
+        leaves = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        ops.layer_norm(leaves[0], (264,), leaves[1], leaves[2]).backward(gy)
+        for name, t in zip(('gx', 'gw', 'gb'), leaves):
+            assert (t.grad is None) == (not t.requires_grad)
+            if t.requires_grad:
+                assert torch.equal(t.grad, got[name]), (mask, name)
+    hold(run_norm(x, w, None, gy), {k: v for k, v in plain.layer_norm(x, w, None, 1e-5, gy).items() if k != 'gb'})
+
+
+def test_norm_large_means_constant_rows_and_non_finite_rows():
+    # a mean 10000 times the spread: the input itself is exact in fp32, so the statistics must be too
+    x, w, b, gy = norm_case(60, 256, torch.float32)
+    x = (x * 64).round() / 64 + 10000.0
+    hold(run_norm(x, w, b, gy), plain.layer_norm(x, w, b, 1e-5, gy))
+    # constant rows: variance 0, the result is the bias (to what (x - mean) leaves: nothing)
+    flat = torch.full((5, 256), 3.25, device='cuda')
+    y = ops.layer_norm(flat, (256,), w, b)
+    assert torch.equal(y, b.expand(5, 256))
+    x[7, 3] = float('inf')
+    x[9, 0] = float('nan')
+    y = ops.layer_norm(x, (256,), w, b)
+    bad = torch.isnan(y).any(1)
+    assert bad[7] and bad[9] and int(bad.sum()) == 2
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_strides_shapes_and_empty(dtype):
+    big, = tensors(0, dtype, (50, 300))
+    w, b, gy = tensors(1, dtype, (256,), (256,), (50, 256))
+    for x in (big[:, :256], big[:, 40:296], big[:, 3:259], big[::2, 1:257], big[:1, :256].expand(50, 256)):
+        g = gy[:x.shape[0]]
+        hold(run_norm(x, w, b, g), plain.layer_norm(x, w, b, 1e-5, g))
+        wm = torch.cat([w, w])[5:261]     # parameters off a 16-byte boundary
+        hold(run_norm(x, wm, b, g), plain.layer_norm(x, wm, b, 1e-5, g))
+    x4 = big[:, :256].reshape(5, 10, 16, 16)
+    y = ops.layer_norm(x4, (16, 16), w.view(16, 16), b.view(16, 16))
+    assert torch.equal(y.view(50, 256), ops.layer_norm(big[:, :256], 256, w, b))
+    leaves = [t.detach().requires_grad_(True) for t in (big[:0, :256], w, b)]
+    y = ops.layer_norm(leaves[0], (256,), leaves[1], leaves[2])
+    y.sum().backward()
+    assert y.shape == (0, 256) and not leaves[1].grad.any() and not leaves[2].grad.any()
+    leaf = big[:, :256].detach().requires_grad_(True)
+    ops.layer_norm(leaf, (256,), w, b).sum().backward()    # an expanded gradient
+    one = torch.ones(50, 256, dtype=dtype, device='cuda')
+    hold({'gx': leaf.grad}, {'gx': plain.layer_norm(big[:, :256], w, b, 1e-5, one)['gx']})
+
+
+def test_norm_gradient_against_differences():
+    x, w, b, gy = norm_case(30, 40, torch.float32)
+    got = run_norm(x, w, b, gy)
+    d = tensors(9, torch.float64, x.shape, w.shape, b.shape)
+    h = 1e-4
+
+    def f(s):
+        t = x.double() + s * d[0]
+        c = t - t.mean(1, keepdim=True)
+        y = c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5) * (w.double() + s * d[1]) + b.double() + s * d[2]
+        return (y * gy.double()).sum()
+
+    slope = ((f(h) - f(-h)) / (2 * h)).item()
+    mine = sum((got[k].double() * v).sum().item() for k, v in zip(('gx', 'gw', 'gb'), d))
+    size = sum((got[k].double() * v).abs().sum().item() for k, v in zip(('gx', 'gw', 'gb'), d))
+    assert abs(mine - slope) <= 1e-5 * size
+
+
+def block_inputs(dtype, rows=70, cin=64, hidden=96, seed=0):
+    x, gy = tensors(seed, dtype, (rows, cin), (rows, cin))
+    w1, w2 = tensors(seed + 1, dtype, (hidden, cin), (cin, hidden), scale=0.1)
+    b1, b2, g, b = tensors(seed + 2, dtype, (hidden,), (cin,), (cin,), (cin,))
+    return x, gy, w1, b1, w2, b2, g, b
+
+
+def block(x, w1, b1, w2, b2, g, b):
+    return ops.layer_norm(ops.feed_forward(x, w1, b1, w2, b2, x, 'gelu'), (x.shape[-1],), g, b)
+
+
+def test_another_stream_and_two_at_once():
+    """Two streams at once, each with its own tensors; results equal to those of one stream."""
+    sets = [block_inputs(torch.bfloat16, rows=3000, seed=10 * k) for k in range(2)]
+    want = [block(s[0], *s[2:]) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(block(sets[k][0], *sets[k][2:]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(o, want[k]) for o in got[k])
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_captured_training_step(dtype):
+    """Forward and backward in a CUDA graph while an eager graph of the same leaves lives (made on a side
+    stream: torch cannot capture a backward pass over leaves whose accumulation node belongs to the
+    default stream, whatever the operators); replayed on new values it gives the eager results."""
+    x, gy, *params = block_inputs(dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (x, *params)]
+
+    def step():
+        y = block(*leaves)
+        return (y, *torch.autograd.grad(y, leaves, gy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = block(*leaves)          # an eager graph that outlives the capture
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    del alive
+    for seed in (20, 30):
+        nx, ngy, *nparams = block_inputs(dtype, seed=seed)
+        with torch.no_grad():
+            for t, v in zip((*leaves, gy), (nx, *nparams, ngy)):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_autocast_follows_torch():
+    x, gy, w1, b1, w2, b2, g, b = block_inputs(torch.float32)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1)]
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        y = ops.fused_linear(*leaves, activation='relu')
+        n = ops.layer_norm(y, (96,))
+        z = ops.feed_forward(x, w1, b1, w2, b2, x)
+    assert y.dtype == torch.bfloat16 and n.dtype == torch.float32 and z.dtype == torch.float32
+    y.sum().backward()
+    assert all(t.grad.dtype == torch.float32 for t in leaves)
+    ref = ops.fused_linear(x.bfloat16(), w1.bfloat16(), b1.bfloat16(), activation='relu')
+    assert torch.equal(y, ref)
+
+
+def test_layers_match_their_torch_forms():
+    torch.manual_seed(0)
+    for act in ('ReLU', 'GELU'):
+        ffn = ops.FFN(64, 160, act_cfg=dict(type=act)).cuda()
+        assert set(ffn.state_dict()) == {'layers.0.0.weight', 'layers.0.0.bias', 'layers.1.weight', 'layers.1.bias'}
+        x = torch.randn(3, 50, 64, device='cuda')
+        other = torch.randn_like(x)
+        ref = ffn.double().layers(x.double())
+        ffn.float()
+        for ident, want in ((None, x + ref), (other, other + ref)):
+            assert torch.allclose(ffn(x, ident).double(), want, rtol=0, atol=2e-5)
+    drop = ops.FFN(64, 160, ffn_drop=0.5, dropout_layer=dict(type='Dropout', drop_prob=0.25)).cuda()
+    y = drop(x)
+    y.sum().backward()
+    assert drop.layers[1].weight.grad is not None and not torch.equal(y, drop(x))
+    drop.eval()
+    assert torch.equal(drop(x), drop(x))
+    norm = ops.LayerNorm(64).cuda()
+    assert torch.allclose(norm(x), torch.nn.functional.layer_norm(x, (64,)), atol=1e-5)
+    lin = ops.FusedLinear(64, 24, activation='relu').cuda()
+    res = torch.randn(3, 50, 24, device='cuda')
+    assert torch.allclose(lin(x, res), torch.relu(x @ lin.weight.t() + lin.bias) + res, atol=2e-5)
+
+
+@pytest.mark.parametrize('batch_first', [True, False])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_encoder_layer_runs_the_operators_together(batch_first, dtype):
+    """The encoder layer against the same layer built from the default attention layer and 64-bit
+    torch, forward and gradients.  fp32: the operators' own errors are below 1e-6 of a row's size and
+    four follow one another, the sampler's tolerance is 1e-4.  bf16: relative L2 within six roundings
+    of 2^-8 along the path."""
+    from oracle.msda import msda_forward
+    torch.manual_seed(0)
+    layer = ops.DeformableEncoderLayer(64, num_heads=4, num_levels=2, num_points=3, feedforward_channels=160,
+                                       batch_first=batch_first)
+    att = layer.attentions[0]
+    for p in (att.sampling_offsets.weight, att.attention_weights.weight):
+        p.data.normal_(0, 0.05)
+    layer = layer.to(dtype).cuda()
+    shapes = torch.tensor([[6, 5], [3, 2]])
+    S = 36
+    x, gy = tensors(0, dtype, (2, S, 64), (2, S, 64))
+    pos, = tensors(1, dtype, (2, S, 64), scale=0.1)
+    refp = torch.rand(2, S, 2, 2, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    mask = torch.zeros(2, S, dtype=torch.bool, device='cuda')
+    mask[1, 30:] = True                                     # a padded batch
+    flip = (lambda t: t) if batch_first else (lambda t: t.transpose(0, 1))
+    leaf = flip(x).contiguous().detach().requires_grad_(True)
+    y = layer(leaf, query_pos=flip(pos), key_padding_mask=mask, reference_points=refp,
+              spatial_shapes=shapes.cuda(), level_start_index=torch.tensor([0, 30]).cuda())
+    params = dict(layer.named_parameters())
+    grads = torch.autograd.grad(y, [leaf, *params.values()], flip(gy).contiguous())
+    # 64 bits, on the CPU
+    P = {k: v.detach().double().cpu().requires_grad_(True) for k, v in params.items()}
+    X = x.double().cpu().requires_grad_(True)
+
+    def lin(t, name):
+        return t @ P[name + '.weight'].t() + P[name + '.bias']
+
+    def norm(t, name):
+        return torch.nn.functional.layer_norm(t, (64,), P[name + '.weight'], P[name + '.bias'])
+
+    q = X + pos.double().cpu()
+    v = lin(X, 'attentions.0.value_proj').masked_fill(mask.cpu()[..., None], 0.0).view(2, S, 4, 16)
+    off = lin(q, 'attentions.0.sampling_offsets').view(2, S, 4, 2, 3, 2)
+    aw = lin(q, 'attentions.0.attention_weights').view(2, S, 4, 6).softmax(-1).view(2, S, 4, 2, 3)
+    scale = torch.stack([shapes[:, 1], shapes[:, 0]], -1).double()
+    loc = refp.double().cpu()[:, :, None, :, None, :] + off / scale[None, None, None, :, None, :]
+    a = norm(lin(msda_forward(v, shapes, loc, aw), 'attentions.0.output_proj') + X, 'norms.0')
+    h = torch.relu(lin(a, 'ffns.0.layers.0.0'))
+    want = norm(a + lin(h, 'ffns.0.layers.1'), 'norms.1')
+    wgrads = torch.autograd.grad(want, [X, *P.values()], gy.double().cpu())
+    tol = 1e-4 if dtype == torch.float32 else 6 * 2.0 ** -8
+    rel = lambda g, w: ((g.double().cpu() - w).norm() / w.norm()).item()   # noqa: E731
+    assert rel(flip(y.detach()), want.detach()) <= tol
+    # the sampler's location gradients jump at cell borders, which rounded locations cross: the
+    # gradients that do not pass through them are compared.  In bf16 a location is off by up to 2^-9
+    # of a map, 0.01 pixels, and the gradients of the attention weights are differences of samples.
+    names = [None, *params]
+    for name, g, w in zip(names, grads, wgrads):
+        if name is None:
+            g = flip(g)
+        if name is None or 'sampling_offsets' in name or (dtype != torch.float32 and 'attention_weights' in name):
+            assert torch.isfinite(g).all()
+            continue
+        assert rel(g, w) <= (tol if dtype == torch.float32 else 2 * tol), name
+
+
+def test_fused_projections_of_the_attention_layer():
+    """fused_proj changes roundings only; the default layer is untouched."""
+    torch.manual_seed(1)
+    a = ops.MultiScaleDeformableAttention(64, 4, 2, 3, dropout=0.1, batch_first=True).cuda()
+    b = ops.MultiScaleDeformableAttention(64, 4, 2, 3, dropout=0.1, batch_first=True, fused_proj=True).cuda()
+    b.load_state_dict(a.state_dict())
+    assert a.fused_proj is False
+    q, = tensors(0, torch.float32, (2, 36, 64))
+    kw = dict(reference_points=torch.rand(2, 36, 2, 2, device='cuda'), spatial_shapes=torch.tensor([[6, 5], [3, 2]]).cuda(),
+              level_start_index=torch.tensor([0, 30]).cuda())
+    a.eval(), b.eval()
+    assert torch.allclose(a(q, **kw), b(q, **kw), atol=2e-5)
+    b.train()
+    assert torch.isfinite(b(q, **kw)).all()     # dropout active: the identity is added outside

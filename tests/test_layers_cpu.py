@@ -1,0 +1,112 @@
+"""The transformer-layer operators without a GPU: refusals, argument checks of the C entries, layer
+construction, and the 64-bit forms against torch."""
+import ctypes
+
+import pytest
+import torch
+
+from mmcv_b200 import _layers, _lib, ops
+from oracle import layers as plain
+
+
+def test_cpu_tensors_fail_loudly():
+    x, w = torch.randn(3, 4), torch.randn(5, 4)
+    with pytest.raises(RuntimeError, match='CUDA tensor'):
+        ops.fused_linear(x, w)
+    with pytest.raises(RuntimeError, match='CUDA tensor'):
+        ops.feed_forward(x, w, None, torch.randn(4, 5), None)
+    with pytest.raises(RuntimeError, match='CUDA tensor'):
+        ops.layer_norm(x, (4,))
+    with pytest.raises(RuntimeError, match='CUDA tensor'):
+        ops.FFN(4, 8)(x)
+
+
+def test_types_and_names_are_checked():
+    with pytest.raises(RuntimeError, match='unsupported dtype'):
+        ops.fused_linear(torch.randn(3, 4).double(), torch.randn(5, 4).double())
+    with pytest.raises(RuntimeError, match='unsupported dtype'):
+        ops.layer_norm(torch.randn(3, 4).double(), (4,))
+    for bad in ('silu', 1, []):
+        with pytest.raises(ValueError, match='unknown activation'):
+            ops.fused_linear(torch.randn(3, 4), torch.randn(5, 4), activation=bad)
+    with pytest.raises(ValueError, match='unknown activation'):
+        ops.FusedLinear(4, 4, activation='tanh')
+    for kw in (dict(num_fcs=3), dict(act_cfg=dict(type='SiLU')), dict(dropout_layer=dict(type='DropPath'))):
+        with pytest.raises(ValueError):
+            ops.FFN(4, 8, **kw)
+
+
+def test_c_entries_reject_bad_arguments_without_a_device():
+    lib = _lib.load()
+    n = ctypes.c_size_t(0)
+
+    def last():
+        return lib.dcn_last_error().decode()
+
+    assert lib.dcn_linear_workspace_bytes(7, 1, 8, 8, 0, ctypes.byref(n)) == -2
+    assert lib.dcn_linear_workspace_bytes(1, 1, 0, 8, 0, ctypes.byref(n)) == -1 and 'positive' in last()
+    assert lib.dcn_linear_workspace_bytes(1, -1, 8, 8, 0, ctypes.byref(n)) == -1
+    assert lib.dcn_linear_workspace_bytes(1, 1, 8, 1 << 21, 0, ctypes.byref(n)) == -2
+    assert lib.dcn_linear_workspace_bytes(1, 1, 8, 8, 0, None) == -1
+    assert lib.dcn_linear_backward_workspace_bytes(1, 9, 1, 8, 8, 0, 1, 1, ctypes.byref(n)) == -1
+    p = 4096   # never dereferenced: the checks come first
+    fwd = lib.dcn_linear_forward
+    assert fwd(None, 8, p, 8, None, None, 0, p, None, 1, 0, 4, 8, 8, 0, None, 0, None) == -1 and 'non-NULL' in last()
+    assert fwd(p, 7, p, 8, None, None, 0, p, None, 1, 0, 4, 8, 8, 0, None, 0, None) == -1 and 'stride' in last()
+    assert fwd(p, 8, p, 8, None, p, 7, p, None, 1, 0, 4, 8, 8, 0, None, 0, None) == -1 and 'stride' in last()
+    assert fwd(p, 8, p, 8, None, None, 0, p, None, 1, 1, 4, 8, 8, 0, None, 0, None) == -1 and 'activation' in last()
+    assert fwd(None, 8, None, 8, None, None, 0, None, None, 1, 0, 0, 8, 8, 0, None, 0, None) == 0   # no rows
+    norm = lib.dcn_layer_norm_forward
+    assert norm(None, 8, None, None, p, None, 0, 0, 4, 8, 1e-5, 0, None) == -1
+    assert norm(p, 7, None, None, p, None, 0, 0, 4, 8, 1e-5, 0, None) == -1 and 'stride' in last()
+    assert norm(p, 8, None, None, p, None, 0, 1, 4, 8, 1e-5, 0, None) == -1 and 'type' in last()
+    assert norm(p, 8, None, None, p, None, 5, 5, 4, 8, 1e-5, 0, None) == -2
+    assert norm(p, 0, None, None, p, None, 0, 0, 4, 0, 1e-5, 0, None) == -1
+    assert lib.dcn_layer_norm_workspace_bytes(10, 16, ctypes.byref(n)) == 0 and n.value >= 10 * 2 * 16 * 4
+
+
+def test_row_views_are_taken_as_they_lie_or_copied():
+    t = torch.arange(60.).view(6, 10)
+    for v, cols, ld, same in [(t, 10, 10, True), (t[:, 2:7], 5, 10, True), (t[::2], 10, 20, True),
+                              (t.t(), 6, 6, False), (t[:1].expand(6, 10), 10, 10, False), (t[:1, 3:5], 2, 2, True),
+                              (t[:, :1], 1, 10, True), (t.view(2, 3, 10)[:, :, 1:9], 8, 10, True)]:
+        rows, got = _layers.as_rows(v, cols)
+        assert rows.shape == (v.numel() // cols, cols) and got == ld
+        assert torch.equal(rows, v.reshape(-1, cols)) and (rows.data_ptr() == v.data_ptr()) == same
+
+
+def test_plain_forms_against_torch():
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, dtype=torch.float64).float()   # noqa: E731
+    x, w, b, res, gy = r(7, 5), r(6, 5), r(6), r(7, 6), r(7, 6)
+    for act, f in ((None, lambda t: t), ('relu', torch.relu), ('gelu', torch.nn.functional.gelu)):
+        leaves = [t.double().requires_grad_(True) for t in (x, w, b)]
+        y = f(torch.nn.functional.linear(*leaves)) + res.double()
+        grads = torch.autograd.grad(y, leaves, gy.double())
+        out = plain.linear(x, w, b, res, act, gy)
+        for key, ref in zip(('y', 'gx', 'gw', 'gb'), (y, *grads)):
+            assert torch.allclose(out[key].v, ref.detach(), rtol=1e-12, atol=1e-12)
+    w2, b2, gx = r(5, 6), r(5), r(7, 5)
+    leaves = [t.double().requires_grad_(True) for t in (x, w, b, w2, b2)]
+    y = torch.nn.functional.linear(torch.relu(torch.nn.functional.linear(*leaves[:3])), *leaves[3:]) + x.double()
+    grads = torch.autograd.grad(y, leaves, gx.double())
+    out = plain.feed_forward(x, w, b, w2, b2, x, 'relu', gx)
+    for key, ref in zip(('y', 'gx', 'gw1', 'gb1', 'gw2', 'gb2'), (y, *grads)):
+        assert torch.allclose(out[key].v, ref.detach(), rtol=1e-12, atol=1e-12)
+    g, c = r(5), r(5)
+    leaves = [t.double().requires_grad_(True) for t in (x, g, c)]
+    y = torch.nn.functional.layer_norm(leaves[0], (5,), leaves[1], leaves[2], 1e-5)
+    grads = torch.autograd.grad(y, leaves, gx.double())
+    out = plain.layer_norm(x, g, c, 1e-5, gx)
+    for key, ref in zip(('y', 'gx', 'gw', 'gb'), (y, *grads)):
+        assert torch.allclose(out[key].v, ref.detach(), rtol=1e-12, atol=1e-12)
+
+
+def test_layer_parameters_carry_the_reference_names():
+    layer = ops.DeformableEncoderLayer(32, num_heads=4, num_levels=2, num_points=2, feedforward_channels=48)
+    names = set(layer.state_dict())
+    assert {'attentions.0.value_proj.weight', 'ffns.0.layers.0.0.weight', 'ffns.0.layers.1.bias', 'norms.0.weight',
+            'norms.1.bias'} <= names
+    assert layer.attentions[0].fused_proj and layer.ffns[0].feedforward_channels == 48
+    with pytest.raises(ValueError, match='divisible'):
+        ops.DeformableEncoderLayer(30, num_heads=4)
