@@ -368,7 +368,8 @@ int dcn_msda_backward(const void *value, const int64_t *spatial_shapes, const in
  * saved (may be NULL): what the activation's derivative needs, for dcn_linear_backward.
  *   RELU  uint32 words [rows][(cout + 31) / 32]; bit j % 32 of word j / 32 is set where the
  *         pre-activation is not <= 0;
- *   GELU  the pre-activation, [rows, cout] dense, element type `dtype`; NONE: not written.
+ *   GELU  the pre-activation, [rows][(cout + 7) / 8 * 8] of element type `dtype`, 16-byte aligned;
+ *   NONE  not written.
  *
  * dcn_linear_backward, from gy = dL/dy [rows, cout] (row stride ldgy) and gz = gy * act'(z):
  *     gx = (gz weight) * in_act'(in_saved) + gx_add      [rows, cin] dense
@@ -397,6 +398,11 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
                         void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
                         int64_t cin, int64_t cout, int32_t device, void *workspace, size_t workspace_bytes,
                         void *stream);
+
+/* Synchronises `stream`, then returns and clears the device's status word of the products: 0 ok;
+ * non-zero = a bounded device-side wait gave up in some call since the last reading (its output is
+ * not valid). */
+int dcn_linear_read_status(int32_t device, void *stream, int32_t *status);
 
 /*
  * Layer norm over the last dimension: n = (x - mean) / sqrt(var + eps), y = n * weight + bias,

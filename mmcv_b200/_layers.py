@@ -84,6 +84,13 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _check_waits(device):
+    status = ctypes.c_int32(0)
+    _lib.check(_lib.load().dcn_linear_read_status(device.index, _raw_stream(device.index), ctypes.byref(status)))
+    if status.value:
+        raise RuntimeError(f'dcn_b200: device-side wait {status.value} timed out; the output is not valid')
+
+
 def linear_forward(x, weight, bias, residual, act, save):
     """act(x weight^T + bias) + residual of checked tensors; with `save`, what the activation's
     derivative needs as well.  Returns (y, saved)."""
@@ -101,13 +108,15 @@ def linear_forward(x, weight, bias, residual, act, save):
     if save and act == _lib.ACT_RELU:
         saved = torch.empty((rows, (cout + 31) // 32), dtype=torch.int32, device=dev)
     elif save and act == _lib.ACT_GELU:
-        saved = x.new_empty((rows, cout))
+        saved = x.new_empty((rows, (cout + 7) // 8 * 8))
     xp, wp = x2.data_ptr(), w2.data_ptr()
     nbytes = _linear_bytes(code, rows, cin, cout, (xp | wp | (ldx | ldw) * esize) & 15)
     ws = _workspace(nbytes, dev)
     _lib.check(lib.dcn_linear_forward(xp, ldx, wp, ldw, _ptr(bias), _ptr(r2), ldr, y.data_ptr(), _ptr(saved),
                                       code, act, rows, cin, cout, dev.index, _ptr(ws), nbytes,
                                       _raw_stream(dev.index)))
+    if _ext._check_status:
+        _check_waits(dev)
     return y, saved
 
 
@@ -136,6 +145,8 @@ def linear_backward(gy, x, weight, saved, act, want, in_saved=None, in_act=_lib.
     _lib.check(lib.dcn_linear_backward(gp, ldg, xp, ldx, wp, ldw, _ptr(saved), _ptr(in_saved), _ptr(gx_add),
                                        _ptr(gx), _ptr(gw), _ptr(gb), code, act, in_act, rows, cin, cout,
                                        dev.index, _ptr(ws), nbytes, _raw_stream(dev.index)))
+    if _ext._check_status:
+        _check_waits(dev)
     return gx, gw, gb
 
 

@@ -26,7 +26,7 @@ EXPORTS = ['dcn_abi_version', 'dcn_last_error', 'dcn_fwd_plan',
            'dcn_modulated_deform_conv_forward', 'dcn_deform_conv_forward',
            'dcn_forward_workspace_bytes', 'dcn_msda_forward', 'dcn_msda_backward',
            'dcn_linear_workspace_bytes', 'dcn_linear_forward',
-           'dcn_linear_backward_workspace_bytes', 'dcn_linear_backward',
+           'dcn_linear_backward_workspace_bytes', 'dcn_linear_backward', 'dcn_linear_read_status',
            'dcn_layer_norm_forward', 'dcn_layer_norm_workspace_bytes', 'dcn_layer_norm_backward']
 
 
@@ -125,6 +125,7 @@ def load():
     lib.dcn_linear_backward_workspace_bytes.argtypes = [i32, i32] + [i64] * 4 + [i32, i32, P(sz)]
     lib.dcn_linear_backward.argtypes = (
         [vp, i64, vp, i64, vp, i64] + [vp] * 6 + [i32] * 3 + [i64] * 3 + [i32, vp, sz, vp])
+    lib.dcn_linear_read_status.argtypes = [i32, vp, P(i32)]
     lib.dcn_layer_norm_forward.argtypes = (
         [vp, i64, vp, vp, vp, vp, i32, i32, i64, i64, f32, i32, vp])
     lib.dcn_layer_norm_workspace_bytes.argtypes = [i64, i64, P(sz)]

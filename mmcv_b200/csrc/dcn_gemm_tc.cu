@@ -1,0 +1,939 @@
+// Matrix product with an epilogue on the tensor cores (sm_100a):
+//   out[i, j] = epilogue(sum_k A[i, k] * B[j, k])
+// for the three products of a linear layer.  Forward reads both operands with k contiguous; the
+// gradient of the input reads the weight, and the gradient of the weight both operands, with the
+// output index contiguous.  Tensor maps and tcgen05 descriptors take either order, so nothing is
+// transposed in memory.
+//
+// One persistent block per SM: a loader lane fills a ring of stages (64 values of k of a 128-row A
+// tile and a BN-row B tile, 128-byte swizzle) with cp.async.bulk.tensor; one warp issues tcgen05.mma
+// into fp32 accumulators in tensor memory, double-buffered so that the epilogue of a tile runs under
+// the main loop of the next; eight warps run the epilogue: tcgen05.ld, bias, activation, derivative,
+// residual, one rounding, a 32-row chunk in shared memory, a tensor store.  The residual arrives by
+// tensor load in the chunk that the result leaves from.  Every wait is bounded.
+//
+// 16-bit tensors: one plane (PL = 1).  fp32 tensors: every operand is the exact sum of three bf16
+// planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_split writes them), and the product is
+//   x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1);
+// what is left out is below 2^-24 of |x||y|.  A tensor core truncates where it adds to its
+// accumulator, so long fp32 sums would drift by 2^-24 a step: the leading product and the five small
+// ones have accumulators of their own, and every 256 values of k the epilogue warps take both out
+// into registers, where the additions round to nearest.
+//
+// The weight gradient's sum over the rows is cut into `splits` ranges when its tiles alone do not
+// fill the SMs; the fp32 parts are added in order by dcn_gemm_reduce.  Its bias gradient (row sums
+// of A) costs one more 128x16 instruction a step: a product with a tile of ones.
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
+#include <cuda.h>
+
+#include "dcn_gemm.cuh"
+#include "dcn_ptx.cuh"
+
+namespace dcn {
+
+namespace {
+
+constexpr int kGemmThreads = 10 * 32;   // 8 epilogue warps, MMA warp, loader warp
+constexpr int kEpiWarps = 8;
+constexpr int kChunkBytes = 4096;       // 32 rows x 128 bytes of staging
+constexpr int kUnitBlocks = 4;          // PL = 3: 64-value blocks between two drains of the accumulators
+
+__device__ int g_gemm_status;           // the first wait that ran out (0: none), until it is read
+
+struct alignas(64) GemmTc {
+  CUtensorMap a, b, out, res, aux;
+  GemmArgs g;
+  int tiles_m, tiles_n, splits, kb_total, kb_split;
+  int stages;
+  int out_tma, res_tma;            // 0: element by element
+  int nbuf;                        // staging chunks of a warp
+  long long ldz;                   // row stride of kept pre-activations: a multiple of 8
+  float *row_part;                 // [splits][m], with splits > 1
+  unsigned long long wait_limit_ns;
+};
+
+__device__ __forceinline__ bool g_wait(uint32_t bar, uint32_t parity, volatile int *abort_s, int code,
+                                       unsigned long long limit, unsigned backoff) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (backoff) __nanosleep(backoff);
+    if ((it & 15u) == 0u) {
+      if (*abort_s) return false;
+      if (globaltimer_ns() - t0 > limit) {
+        *abort_s = 1;
+        atomicCAS(&g_gemm_status, 0, code);
+        return false;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+               ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  return r;
+}
+
+// Shared-memory descriptor of a tile with the 128-byte swizzle whose rows of 128 bytes hold 64
+// values of the row (or column) index, one row per k: 8 k are 1024 bytes, the next 64 rows of the
+// tile 8192 bytes away.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(8192 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+struct Item {
+  int m0, n0, split, kb0, kb1;
+};
+__device__ __forceinline__ Item decode(uint32_t item, const GemmTc &p, int BN) {
+  const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+  Item it;
+  it.split = (int)(item / tiles);
+  const uint32_t t = item - (uint32_t)it.split * tiles;
+  const uint32_t tm = t / (uint32_t)p.tiles_n;   // column tiles of one row tile are neighbours: A stays in L2
+  it.m0 = (int)tm * 128;
+  it.n0 = (int)(t - tm * (uint32_t)p.tiles_n) * BN;
+  it.kb0 = it.split * p.kb_split;
+  it.kb1 = min(p.kb_total, it.kb0 + p.kb_split);
+  return it;
+}
+
+// 32 values of a staging row (128-byte swizzled, 16-byte pieces q0, q0 + 1, ...) as floats, and back.
+template <typename TO>
+__device__ __forceinline__ void stage_load(const uint8_t *row, int sw, int q0, float (&v)[32]) {
+  if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 f = *reinterpret_cast<const float4 *>(row + ((q ^ sw) << 4));
+      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(row + (((q0 + q) ^ sw) << 4));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
+          v[8 * q + 2 * i] = __uint_as_float(w[i] << 16);
+          v[8 * q + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+          v[8 * q + 2 * i] = f.x;
+          v[8 * q + 2 * i + 1] = f.y;
+        }
+      }
+    }
+  }
+}
+template <typename TO>
+__device__ __forceinline__ void stage_store(uint8_t *row, int sw, int q0, const float (&v)[32]) {
+  if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4 *>(row + ((q ^ sw) << 4)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+          const __half2 h = __floats2half2_rn(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      *reinterpret_cast<uint4 *>(row + (((q0 + q) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// The element-by-element forms of the chunk's tensor load and store, for tensors whose rows do not
+// start on 16 bytes: the warp walks the 32 rows, neighbouring lanes on neighbouring columns.
+template <typename TO>
+__device__ __forceinline__ void chunk_in(uint8_t *chunk, const TO *src, long long ld, long long i0, long long m,
+                                         long long j0, long long n, int lane) {
+  constexpr int CW = 128 / (int)sizeof(TO);
+  for (int r = 0; r < 32 && i0 + r < m; ++r)
+#pragma unroll
+    for (int c = lane; c < CW; c += 32)
+      if (j0 + c < n) {
+        const int at = c * (int)sizeof(TO);
+        *reinterpret_cast<TO *>(chunk + r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4))) = src[(i0 + r) * ld + j0 + c];
+      }
+}
+template <typename TO>
+__device__ __forceinline__ void chunk_out(const uint8_t *chunk, TO *dst, long long ld, long long i0, long long m,
+                                          long long j0, long long n, int lane) {
+  constexpr int CW = 128 / (int)sizeof(TO);
+  for (int r = 0; r < 32 && i0 + r < m; ++r)
+#pragma unroll
+    for (int c = lane; c < CW; c += 32)
+      if (j0 + c < n) {
+        const int at = c * (int)sizeof(TO);
+        dst[(i0 + r) * ld + j0 + c] =
+            *reinterpret_cast<const TO *>(chunk + r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4)));
+      }
+}
+
+}  // namespace
+
+// PL planes per operand; TI the 16-bit type of the planes, TO the output's (and residual's) type;
+// AMN / BMN: the operand lies with its row index contiguous.
+template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN>
+__global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_constant__ GemmTc p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t kABytes = PL * 16384u, kBBytes = PL * BN * 128u, kStage = kABytes + kBBytes;
+  constexpr bool kRowSum = AMN && PL == 1;             // only the weight gradient asks for row sums
+  constexpr int kBufs = (kRowSum && BN == 256) ? 1 : 2;   // accumulator buffers that fit beside the row sums
+  constexpr int kBufCols = PL == 3 ? 2 * BN : BN;
+  constexpr int kCols = kBufs * kBufCols + (kRowSum ? 16 * kBufs : 0);
+  constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kCols <= 512, "tensor memory");
+  constexpr int CW = 128 / (int)sizeof(TO);            // columns of a staging chunk
+  // 16-bit pre-activations pass through a second chunk; fp32 ones, whose rings leave no room for it,
+  // go straight between a lane's row (128 bytes of it at a time) and its registers
+  constexpr bool kAuxStaged = PL == 1;
+  constexpr int kWarpCols = BN / 2 > CW ? BN / 2 : CW; // columns of an epilogue warp
+
+  const GemmArgs &g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ST = p.stages;
+  const uint32_t bar0 = smem_u32(smem);
+  const uint32_t full = bar0, empty = full + 8 * ST, tmem_full = empty + 8 * ST, tmem_empty = tmem_full + 16,
+                 res_bar = tmem_empty + 16;            // two per epilogue warp
+  uint32_t *tmem_slot = (uint32_t *)(smem + 896);
+  volatile int *abort_s = (volatile int *)(smem + 904);
+  uint8_t *ring = smem + 1024;
+  uint8_t *staging = ring + (size_t)ST * kStage;
+  uint8_t *ones = staging + (size_t)kEpiWarps * p.nbuf * kChunkBytes;
+  const unsigned long long limit = p.wait_limit_ns;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tmem_full + 8 * i, 1);
+      mbar_init(tmem_empty + 8 * i, kEpiWarps);
+    }
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_bar + 8 * i, 1);
+    *abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (kRowSum && g.row_sum) {
+    // 16 rows x 64 values, all one: the same in every layout
+    for (int i = threadIdx.x; i < 1024; i += kGemmThreads) ((TI *)ones)[i] = ElemOf<TI>::from(1.f);
+    fence_proxy_async_smem();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(tmem_slot), kAlloc);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t items = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
+
+  if (warp < kEpiWarps) {
+    // ------------------------------ epilogue ------------------------------
+    const int q = warp & 3, h = warp >> 2;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16);
+    uint8_t *chunk = staging + (size_t)warp * p.nbuf * kChunkBytes;   // residual in, result out
+    uint8_t *aux = chunk + kChunkBytes;                               // pre-activations in or out
+    const uint32_t chunk_u = smem_u32(chunk), aux_u = smem_u32(aux);
+    const uint32_t rb = res_bar + 16 * warp, ab = rb + 8;
+    uint32_t rph = 0, aph = 0, unit = 0;
+    const bool mine = h * kWarpCols < BN;
+    const long long words = (g.n + 31) / 32;
+    const bool aux_in = g.slope_act == DCN_ACT_GELU, aux_out = g.saved && g.act == DCN_ACT_GELU;
+    bool ok = true;
+    for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const Item it = decode(item, p, BN);
+      const long long i0 = it.m0 + q * 32, row = i0 + lane;
+      float facc[PL == 3 ? kWarpCols : 1];
+      const int units = PL == 3 ? (it.kb1 - it.kb0 + kUnitBlocks - 1) / kUnitBlocks : 1;
+      int buf = 0;
+      for (int u = 0; u < units && ok; ++u, ++unit) {
+        buf = kBufs == 2 ? (int)(unit & 1) : 0;
+        const uint32_t ph = kBufs == 2 ? (unit >> 1) & 1u : unit & 1u;
+        ok = __all_sync(0xffffffffu, g_wait(tmem_full + 8 * buf, ph, abort_s, 3, 2 * limit, 64));
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (PL == 3) {
+          if (mine) {
+            const uint32_t t = lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols);
+#pragma unroll
+            for (int c = 0; c < kWarpCols; c += 32) {
+              uint32_t a[32], b[32];
+              tmem_ld32(t + c, a);
+              tmem_ld32(t + BN + c, b);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float v = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+                facc[c + j] = u ? facc[c + j] + v : v;
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+        }
+      }
+      if (!ok) break;
+      if (kRowSum && g.row_sum && it.n0 == 0 && h == 0) {
+        const float v = __uint_as_float(tmem_ld1(lane_base + (uint32_t)(kBufs * kBufCols + 16 * buf)));
+        tmem_ld_wait();
+        if (row < g.m) {
+          if (p.splits > 1) p.row_part[(long long)it.split * g.m + row] = v;
+          else ((TI *)g.row_sum)[row] = ElemOf<TI>::from(v);
+        }
+      }
+      if (mine) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < kWarpCols; c0 += CW) {
+          const long long j0 = it.n0 + h * kWarpCols + c0;
+          if (j0 >= g.n) break;
+          const int sw = lane & 7;
+          uint8_t *my = chunk + lane * 128, *my_aux = aux + lane * 128;
+          // the chunk's last store has been read
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+          if (g.res) {
+            if (p.res_tma) {
+              if (lane == 0) {
+                fence_proxy_async_smem();
+                mbar_arrive_expect_tx(rb, kChunkBytes);
+                tma_load_3d(chunk_u, &p.res, (int)j0, (int)i0, 0, rb);
+              }
+            } else {
+              chunk_in<TO>(chunk, (const TO *)g.res, g.ldr, i0, g.m, j0, g.n, lane);
+            }
+          }
+          if (kAuxStaged && aux_in && lane == 0) {
+            fence_proxy_async_smem();
+            mbar_arrive_expect_tx(ab, kChunkBytes);
+            tma_load_3d(aux_u, &p.aux, (int)j0, (int)i0, 0, ab);
+          }
+          if (g.res && p.res_tma) {
+            ok = __all_sync(0xffffffffu, g_wait(rb, rph, abort_s, 8, 2 * limit, 0));
+            rph ^= 1u;
+          }
+          if (kAuxStaged && aux_in) {
+            ok = __all_sync(0xffffffffu, g_wait(ab, aph, abort_s, 9, 2 * limit, 0)) && ok;
+            aph ^= 1u;
+          }
+          if (!ok) break;
+          __syncwarp();
+#pragma unroll
+          for (int c1 = 0; c1 < CW; c1 += 32) {
+            const int q0 = c1 / 8;   // first 16-byte piece (16-bit types; fp32 chunks hold one group of 32)
+            float v[32];
+            if constexpr (PL == 3) {
+              // c0 is a runtime index: pick the group without indexing registers dynamically
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                v[j] = facc[j];
+                if constexpr (kWarpCols > 32) v[j] = c0 ? facc[32 + j] : v[j];
+              }
+            } else {
+              uint32_t r[32];
+              tmem_ld32(lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols + c0 + c1), r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            }
+            const long long j1 = j0 + c1;
+            if (g.bias) {
+              const TO *bp = (const TO *)g.bias + j1;
+              if (j1 + 32 <= g.n) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += ElemOf<TO>::to(__ldg(bp + j));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += j1 + j < g.n ? ElemOf<TO>::to(__ldg(bp + j)) : 0.f;
+              }
+            }
+            if (g.act != DCN_ACT_NONE) {
+              if (g.saved) {
+                if (g.act == DCN_ACT_RELU) {
+                  uint32_t bits = 0;
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) bits |= (uint32_t)relu_bit(v[j]) << j;
+                  if (row < g.m && j1 < g.n) ((uint32_t *)g.saved)[row * words + (j1 >> 5)] = bits;
+                } else {
+                  if constexpr (kAuxStaged) {
+                    stage_store<TO>(my_aux, sw, q0, v);
+                  } else if (row < g.m) {
+                    float4 *zp = reinterpret_cast<float4 *>((float *)g.saved + row * p.ldz + j1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                      if (j1 + 4 * i < p.ldz) zp[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                  }
+                }
+              }
+              if (g.act == DCN_ACT_RELU) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = act_value(DCN_ACT_GELU, v[j]);
+              }
+            }
+            if (g.slope_act == DCN_ACT_RELU) {
+              const uint32_t bits =
+                  row < g.m && j1 < g.n ? __ldg((const uint32_t *)g.slope + row * words + (j1 >> 5)) : 0u;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.f;
+            } else if (aux_in) {
+              if constexpr (kAuxStaged) {
+                float z[32];
+                stage_load<TO>(my_aux, sw, q0, z);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= gelu_slope(z[j]);
+              } else if (row < g.m) {
+                const float4 *zp = reinterpret_cast<const float4 *>((const float *)g.slope + row * p.ldz + j1);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (j1 + 4 * i < p.ldz) {
+                    const float4 z = __ldg(zp + i);
+                    v[4 * i] *= gelu_slope(z.x);
+                    v[4 * i + 1] *= gelu_slope(z.y);
+                    v[4 * i + 2] *= gelu_slope(z.z);
+                    v[4 * i + 3] *= gelu_slope(z.w);
+                  }
+              }
+            }
+            if (g.res) {
+              float r[32];
+              stage_load<TO>(my, sw, q0, r);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] += r[j];
+            }
+            stage_store<TO>(my, sw, q0, v);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (p.out_tma) {
+            if (lane == 0) tma_store_3d(&p.out, chunk_u, (int)j0, (int)i0, it.split);
+          } else {
+            chunk_out<TO>(chunk, (TO *)g.out, g.n, i0, g.m, j0, g.n, lane);
+          }
+          if (kAuxStaged && aux_out && lane == 0) tma_store_3d(&p.aux, aux_u, (int)j0, (int)i0, 0);
+          if (lane == 0) bulk_commit();
+          __syncwarp();
+        }
+      }
+      if constexpr (PL == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  } else if (warp == 8) {
+    // ------------------------------ MMA issuer ------------------------------
+    constexpr uint32_t kFmt = std::is_same_v<TI, __nv_bfloat16> ? 1u : 0u;
+    constexpr uint32_t kDesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((AMN ? 1u : 0u) << 15) | ((128u >> 4) << 24);
+    constexpr uint32_t idesc = kDesc | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17);
+    constexpr uint32_t idesc_ones = kDesc | ((16u >> 3) << 17);
+    constexpr uint32_t kAStep = AMN ? 2048 >> 4 : 32 >> 4, kBStep = BMN ? 2048 >> 4 : 32 >> 4;
+    const uint64_t ones_desc = smem_desc_sw128(smem_u32(ones));
+    uint32_t st = 0, ph = 0, unit = 0;
+    bool ok = true;
+    for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const Item it = decode(item, p, BN);
+      const bool sums = kRowSum && g.row_sum && it.n0 == 0;
+      uint32_t d = 0;
+      int buf = 0;
+      for (int kb = it.kb0; kb < it.kb1; ++kb) {
+        const bool first = PL == 3 ? (kb - it.kb0) % kUnitBlocks == 0 : kb == it.kb0;
+        const bool last = PL == 3 ? (kb - it.kb0) % kUnitBlocks == kUnitBlocks - 1 || kb == it.kb1 - 1 : kb == it.kb1 - 1;
+        if (first) {
+          buf = kBufs == 2 ? (int)(unit & 1) : 0;
+          const uint32_t eph = (kBufs == 2 ? (unit >> 1) & 1u : unit & 1u) ^ 1u;
+          ok = __all_sync(0xffffffffu, g_wait(tmem_empty + 8 * buf, eph, abort_s, 4, limit, 0));
+          if (!ok) break;
+          d = tmem_base + (uint32_t)(buf * kBufCols);
+          ++unit;
+        }
+        ok = __all_sync(0xffffffffu, g_wait(full + 8 * st, ph, abort_s, 5, limit, 0));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t sa = smem_u32(ring) + st * kStage, sb = sa + kABytes;
+          uint64_t ad[PL], bd[PL];
+#pragma unroll
+          for (int i = 0; i < PL; ++i) {
+            ad[i] = AMN ? smem_desc_mn(sa + i * 16384u) : smem_desc_sw128(sa + i * 16384u);
+            bd[i] = BMN ? smem_desc_mn(sb + i * BN * 128u) : smem_desc_sw128(sb + i * BN * 128u);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t ka = (uint64_t)(k * kAStep), kb_ = (uint64_t)(k * kBStep);
+            const uint32_t more = !first || k ? 1u : 0u;
+            umma_bf16(d, ad[0] + ka, bd[0] + kb_, idesc, more);
+            if constexpr (PL == 3) {
+              umma_bf16(d + BN, ad[0] + ka, bd[2] + kb_, idesc, more);
+              umma_bf16(d + BN, ad[2] + ka, bd[0] + kb_, idesc, 1u);
+              umma_bf16(d + BN, ad[1] + ka, bd[1] + kb_, idesc, 1u);
+              umma_bf16(d + BN, ad[0] + ka, bd[1] + kb_, idesc, 1u);
+              umma_bf16(d + BN, ad[1] + ka, bd[0] + kb_, idesc, 1u);
+            }
+            if (kRowSum && sums)
+              umma_bf16(tmem_base + (uint32_t)(kBufs * kBufCols + 16 * buf), ad[0] + ka, ones_desc, idesc_ones, more);
+          }
+          umma_commit(empty + 8 * st);
+          if (last) umma_commit(tmem_full + 8 * buf);
+        }
+        __syncwarp();
+        if (++st == (uint32_t)ST) { st = 0; ph ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------ loader ------------------------------
+    if (lane == 0) {
+      uint32_t st = 0, ph = 0;
+      bool ok = true;
+      for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        const Item it = decode(item, p, BN);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          ok = g_wait(empty + 8 * st, ph ^ 1u, abort_s, 7, 2 * limit, 32);
+          if (!ok) break;
+          const uint32_t bar = full + 8 * st, sa = smem_u32(ring) + st * kStage, sb = sa + kABytes;
+          mbar_arrive_expect_tx(bar, kStage);
+          const int k0 = kb * 64;
+#pragma unroll
+          for (int i = 0; i < PL; ++i) {
+            if constexpr (AMN) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) tma_load_3d(sa + i * 16384u + j * 8192u, &p.a, it.m0 + 64 * j, k0, i, bar);
+            } else {
+              tma_load_3d(sa + i * 16384u, &p.a, k0, it.m0, i, bar);
+            }
+            if constexpr (BMN) {
+#pragma unroll
+              for (int j = 0; j < BN / 64; ++j)
+                tma_load_3d(sb + i * BN * 128u + j * 8192u, &p.b, it.n0 + 64 * j, k0, i, bar);
+            } else {
+              tma_load_3d(sb + i * BN * 128u, &p.b, k0, it.n0, i, bar);
+            }
+          }
+          if (++st == (uint32_t)ST) { st = 0; ph ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  if (*abort_s) {
+    for (int i = 0; i < 20; ++i) __nanosleep(50000);   // copies and products in flight land
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kAlloc);
+  }
+}
+
+namespace {
+
+// out[i, j] = sum over the ranges of part [splits][m][ldp], in order; four columns a thread
+template <typename T>
+__global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__ part, int splits, long long m,
+                                                       long long n, long long ldp, T *__restrict__ out) {
+  const long long per_row = ldp / 4, idx = blockIdx.x * 256LL + threadIdx.x;
+  if (idx >= m * per_row) return;
+  const long long i = idx / per_row, j = (idx - i * per_row) * 4;
+  const float4 *p = reinterpret_cast<const float4 *>(part + i * ldp + j);
+  const long long step = m * ldp / 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float4 a = p[s * step];
+    v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+  }
+  T *o = out + i * n + j;
+  if (j < n) o[0] = ElemOf<T>::from(v.x);
+  if (j + 1 < n) o[1] = ElemOf<T>::from(v.y);
+  if (j + 2 < n) o[2] = ElemOf<T>::from(v.z);
+  if (j + 3 < n) o[3] = ElemOf<T>::from(v.w);
+}
+
+// out[c] = sum over the parts, 32 of them side by side, joined in a tree
+template <typename T>
+__global__ void __launch_bounds__(1024) dcn_column_reduce(const float *__restrict__ part, int parts, long long cols, T *out) {
+  __shared__ float sm[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long c = blockIdx.x * 32LL + tx;
+  float v = 0.f;
+  if (c < cols)
+    for (int p = ty; p < parts; p += 32) v += part[p * cols + c];
+  sm[ty][tx] = v;
+  __syncthreads();
+  for (int d = 16; d > 0; d >>= 1) {
+    if (ty < d) sm[ty][tx] += sm[ty + d][tx];
+    __syncthreads();
+  }
+  if (ty == 0 && c < cols) out[c] = ElemOf<T>::from(sm[0][tx]);
+}
+
+// x = x1 + x2 + x3, 8 bits each (truncated, so that nothing overflows); an infinity or NaN stays in x1
+__device__ __forceinline__ void split3(float x, uint32_t (&b)[3]) {
+  b[0] = __float_as_uint(x) & 0xffff0000u;
+  const float r1 = x - __uint_as_float(b[0]);
+  const bool finite = (b[0] & 0x7f800000u) != 0x7f800000u;
+  b[1] = finite ? __float_as_uint(r1) & 0xffff0000u : 0u;
+  const float r2 = r1 - __uint_as_float(b[1]);
+  b[2] = finite ? __float_as_uint(r2) & 0xffff0000u : 0u;
+  // a NaN whose payload lies in the low bits must not turn into an infinity
+  if (x != x) b[0] |= 0x00400000u;
+}
+
+struct StageArgs {
+  const void *src, *saved;
+  void *dst;
+  float *sums;
+  long long ld, rows, cols, pitch;
+  int act;
+  int vec_src;   // rows start on 16 bytes
+};
+
+// blockDim.x threads of 8 columns each, blockDim.y rows at a time; blockIdx.y: a slab of rows
+template <typename T, int PL>
+__global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
+  __shared__ float red[256 * 8];
+  const long long c = (blockIdx.x * (long long)blockDim.x + threadIdx.x) * 8;
+  const long long words = (a.cols + 31) / 32;
+  float sum[8] = {};
+  if (c < a.pitch) {
+    for (long long r = blockIdx.y * (long long)blockDim.y + threadIdx.y; r < a.rows; r += (long long)gridDim.y * blockDim.y) {
+      float v[8];
+      const T *src = (const T *)a.src + r * a.ld + c;
+      if (a.vec_src && c + 8 <= a.cols) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 4);
+          v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+          v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4 *>(src);
+          const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = ElemOf<T>::to(e[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < a.cols ? ElemOf<T>::to(src[i]) : 0.f;
+      }
+      if (a.act == DCN_ACT_RELU) {
+        const uint32_t bits = c < a.cols ? ((const uint32_t *)a.saved)[r * words + (c >> 5)] >> (c & 31) : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (bits >> i) & 1u ? v[i] : 0.f;
+      } else if (a.act == DCN_ACT_GELU) {
+        const T *z = (const T *)a.saved + r * a.pitch + c;   // kept with the same pitch
+        uint4 u[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4 *>(z)[i];
+        const T *e = reinterpret_cast<const T *>(u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope(ElemOf<T>::to(e[i]));
+      }
+      if constexpr (PL == 1) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          T lo = ElemOf<T>::from(v[2 * i]), hi = ElemOf<T>::from(v[2 * i + 1]);
+          w[i] = (uint32_t)*reinterpret_cast<uint16_t *>(&lo) | ((uint32_t)*reinterpret_cast<uint16_t *>(&hi) << 16);
+        }
+        *reinterpret_cast<uint4 *>((T *)a.dst + r * a.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t lo[3], hi[3];
+          split3(v[2 * i], lo);
+          split3(v[2 * i + 1], hi);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) w[k][i] = (lo[k] >> 16) | hi[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<uint4 *>((uint16_t *)a.dst + (k * a.rows + r) * a.pitch + c) =
+              make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += v[i];
+    }
+  }
+  if (!a.sums) return;
+  // the block's rows in order, one row of threads after another
+  for (int y = 0; y < (int)blockDim.y; ++y) {
+    if ((int)threadIdx.y == y)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float *s = red + threadIdx.x * 8 + i;
+        *s = y ? *s + sum[i] : sum[i];
+      }
+    __syncthreads();
+  }
+  if (threadIdx.y == 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < a.cols) a.sums[blockIdx.y * a.cols + c + i] = red[threadIdx.x * 8 + i];
+}
+
+void stage_shape(long long rows, long long pitch, int *tx, int *ty, int *gx, int *gy) {
+  int x = 1;
+  while (x < 32 && x * 8 < pitch) x *= 2;
+  *tx = x;
+  *ty = 256 / x;
+  *gx = (int)((pitch + x * 8 - 1) / (x * 8));
+  const long long want = (rows + *ty - 1) / *ty;
+  long long most = 148 * 8 / *gx;
+  if (most < 1) most = 1;
+  *gy = (int)(want < 1 ? 1 : want < most ? want : most);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static std::atomic<EncodeTiledFn> fn{nullptr};
+  EncodeTiledFn f = fn.load(std::memory_order_acquire);
+  if (f) return f;
+  void *p = nullptr;
+  cudaDriverEntryPointQueryResult qres;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) != cudaSuccess ||
+      qres != cudaDriverEntryPointSuccess || !p) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  f = (EncodeTiledFn)p;
+  fn.store(f, std::memory_order_release);
+  return f;
+}
+
+// [depth][rows][inner] with the given row stride (elements), boxes of box_inner x box_rows x 1
+bool encode3(CUtensorMap *map, CUtensorMapDataType type, int esize, const void *base, long long inner, long long rows,
+             long long depth, long long ld, unsigned box_inner, unsigned box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)depth};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * esize), (cuuint64_t)(rows * ld * esize)};
+  const cuuint32_t box[3] = {box_inner, box_rows, 1}, estr[3] = {1, 1, 1};
+  return enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN>
+cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
+  auto kern = dcn_gemm_tc<TI, TO, PL, BN, AMN, BMN>;
+  static std::atomic<unsigned long long> done_mask{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  constexpr size_t kMost = 232448;
+  if (!(done_mask.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
+    if (e != cudaSuccess) return e;
+    done_mask.fetch_or(bit, std::memory_order_release);
+  }
+  constexpr size_t stage = (size_t)PL * (16384 + BN * 128);
+  const size_t fixed = 1024 + 1024 + (size_t)kEpiWarps * p.nbuf * kChunkBytes + (AMN && PL == 1 ? 2048 : 0);
+  int stages = (int)((kMost - fixed) / stage);
+  if (stages > 8) stages = 8;
+  p.stages = stages;
+  const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
+  const int grid = (int)(items < 148 ? items : 148);
+  kern<<<grid, kGemmThreads, fixed + stages * stage, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename TI, typename TO, int PL, bool AMN, bool BMN>
+cudaError_t run_bn(GemmTc &p, int bn, cudaStream_t s) {
+  if constexpr (PL == 1)
+    if (bn == 256) return run_tc<TI, TO, PL, 256, AMN, BMN>(p, s);
+  if (bn == 128) return run_tc<TI, TO, PL, 128, AMN, BMN>(p, s);
+  return run_tc<TI, TO, PL, 64, AMN, BMN>(p, s);
+}
+
+template <typename TI, typename T, int PL>
+cudaError_t run_order(GemmTc &p, int bn, bool parts, cudaStream_t s) {
+  const GemmArgs &g = p.g;
+  if (!g.a_mn && !g.b_mn) return run_bn<TI, T, PL, false, false>(p, bn, s);
+  if (!g.a_mn) return run_bn<TI, T, PL, false, true>(p, bn, s);
+  if (parts) return run_bn<TI, float, PL, true, true>(p, bn, s);
+  return run_bn<TI, T, PL, true, true>(p, bn, s);
+}
+
+template <typename T>
+cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &g, cudaStream_t s) {
+  const long long n = g.m * (plan.ldp / 4);
+  dcn_gemm_reduce<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(part, plan.splits, g.m, g.n, plan.ldp, (T *)g.out);
+  return cudaGetLastError();
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weight_gradient) {
+  GemmPlan p = {};
+  const long long tm = (m + 127) / 128;
+  auto tiles = [&](int bn) { return tm * ((n + bn - 1) / bn); };
+  p.kb_total = (int)((k + 63) / 64);
+  p.splits = 1;
+  if (weight_gradient) {
+    p.bn = planes == 1 && n > 128 ? 256 : n > 64 ? 128 : 64;
+    long long splits = 148 / tiles(p.bn);
+    if (splits > p.kb_total / 4) splits = p.kb_total / 4;
+    if (splits < 1) splits = 1;
+    p.kb_split = (int)((p.kb_total + splits - 1) / splits);
+    p.splits = (p.kb_total + p.kb_split - 1) / p.kb_split;
+  } else {
+    p.bn = planes == 1 && n > 128 && tiles(256) >= 148 ? 256 : n > 64 && tiles(128) >= 148 ? 128 : 64;
+    p.kb_split = p.kb_total;
+  }
+  p.ldp = (n + 3) / 4 * 4;
+  if (p.splits > 1) {
+    p.part_bytes = up256((size_t)p.splits * m * p.ldp * 4);
+    p.row_part_bytes = up256((size_t)p.splits * m * 4);
+  }
+  return p;
+}
+
+cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, float *part, float *row_part,
+                           cudaStream_t s) {
+  GemmTc p;
+  memset(&p, 0, sizeof(p));
+  p.g = g;
+  const int planes = dtype == DCN_DTYPE_F32 ? 3 : 1, esize = dtype == DCN_DTYPE_F32 ? 4 : 2;
+  const bool parts = plan.splits > 1;
+  const CUtensorMapDataType t16 = dtype == DCN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType tio = dtype == DCN_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : t16;
+  p.tiles_m = (int)((g.m + 127) / 128);
+  p.tiles_n = (int)((g.n + plan.bn - 1) / plan.bn);
+  p.splits = plan.splits;
+  p.kb_total = plan.kb_total;
+  p.kb_split = plan.kb_split;
+  p.row_part = row_part;
+  p.wait_limit_ns = kWaitLimitNs;
+  bool ok = g.a_mn ? encode3(&p.a, t16, 2, g.a, g.m, g.kk, planes, g.lda, 64, 64)
+                   : encode3(&p.a, t16, 2, g.a, g.kk, g.m, planes, g.lda, 64, 128);
+  ok = ok && (g.b_mn ? encode3(&p.b, t16, 2, g.b, g.n, g.kk, planes, g.ldb, 64, 64)
+                     : encode3(&p.b, t16, 2, g.b, g.kk, g.n, planes, g.ldb, 64, plan.bn));
+  const bool rows16 = g.n * esize % 16 == 0;
+  const unsigned cw = (unsigned)(128 / esize);
+  p.nbuf = 1;
+  if (parts) {
+    p.out_tma = 1;
+    ok = ok && encode3(&p.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, g.n, g.m, plan.splits, plan.ldp, 32, 32);
+  } else if (rows16 && aligned16(g.out)) {
+    p.out_tma = 1;
+    ok = ok && encode3(&p.out, tio, esize, g.out, g.n, g.m, 1, g.n, cw, 32);
+  }
+  if (g.res && aligned16(g.res) && g.ldr * esize % 16 == 0) {
+    p.res_tma = 1;
+    ok = ok && encode3(&p.res, tio, esize, g.res, g.n, g.m, 1, g.ldr, cw, 32);
+  }
+  const void *aux = g.slope_act == DCN_ACT_GELU ? g.slope : g.act == DCN_ACT_GELU ? g.saved : nullptr;
+  p.ldz = (g.n + 7) / 8 * 8;
+  if (aux && planes == 1) {
+    p.nbuf = 2;
+    ok = ok && encode3(&p.aux, tio, esize, aux, p.ldz, g.m, 1, p.ldz, cw, 32);
+  }
+  if (!ok) return cudaErrorInvalidValue;
+  cudaError_t e;
+  if (dtype == DCN_DTYPE_F32) e = run_order<__nv_bfloat16, float, 3>(p, plan.bn, parts, s);
+  else if (dtype == DCN_DTYPE_BF16) e = run_order<__nv_bfloat16, __nv_bfloat16, 1>(p, plan.bn, parts, s);
+  else e = run_order<__half, __half, 1>(p, plan.bn, parts, s);
+  if (e != cudaSuccess || !parts) return e;
+  if (dtype == DCN_DTYPE_F32) e = run_reduce<float>(part, plan, g, s);
+  else if (dtype == DCN_DTYPE_BF16) e = run_reduce<__nv_bfloat16>(part, plan, g, s);
+  else e = run_reduce<__half>(part, plan, g, s);
+  if (e == cudaSuccess && g.row_sum) e = launch_column_reduce(row_part, plan.splits, g.m, dtype, g.row_sum, s);
+  return e;
+}
+
+int stage_slabs(long long rows, long long cols) {
+  int tx, ty, gx, gy;
+  stage_shape(rows, (cols + 7) / 8 * 8, &tx, &ty, &gx, &gy);
+  return gy;
+}
+
+cudaError_t launch_gemm_stage(const void *src, long long ld, const void *saved, int act, long long rows,
+                              long long cols, int dtype, void *planes, long long pitch, float *sums, int *slabs,
+                              cudaStream_t s) {
+  StageArgs a = {};
+  a.src = src; a.saved = saved; a.dst = planes; a.sums = sums;
+  a.ld = ld; a.rows = rows; a.cols = cols; a.pitch = pitch; a.act = act;
+  const int esize = dtype == DCN_DTYPE_F32 ? 4 : 2;
+  a.vec_src = aligned16(src) && ld * esize % 16 == 0;
+  int tx, ty, gx, gy;
+  stage_shape(rows, pitch, &tx, &ty, &gx, &gy);
+  if (slabs) *slabs = gy;
+  const dim3 grid(gx, gy), block(tx, ty);
+  if (dtype == DCN_DTYPE_F32) dcn_gemm_stage<float, 3><<<grid, block, 0, s>>>(a);
+  else if (dtype == DCN_DTYPE_BF16) dcn_gemm_stage<__nv_bfloat16, 1><<<grid, block, 0, s>>>(a);
+  else dcn_gemm_stage<__half, 1><<<grid, block, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s) {
+  const unsigned grid = (unsigned)((cols + 31) / 32);
+  if (dtype == DCN_DTYPE_F32) dcn_column_reduce<float><<<grid, 1024, 0, s>>>(part, parts, cols, (float *)out);
+  else if (dtype == DCN_DTYPE_BF16)
+    dcn_column_reduce<__nv_bfloat16><<<grid, 1024, 0, s>>>(part, parts, cols, (__nv_bfloat16 *)out);
+  else dcn_column_reduce<__half><<<grid, 1024, 0, s>>>(part, parts, cols, (__half *)out);
+  return cudaGetLastError();
+}
+
+// Reads and clears the status word of the current device, after the work on `s`.
+cudaError_t read_gemm_status(cudaStream_t s, int *status) {
+  int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_gemm_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_gemm_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e;
+}
+
+}  // namespace dcn

@@ -4,64 +4,63 @@
 //   backward  gz = gy * act'(z)                            element-wise, only with an activation
 //             gx = gz W  (times the derivative of the activation before, plus gx_add)
 //             gW = gz^T x,  gb = column sums of gz
-#include "dcn_layers.cuh"
+// 16-bit operands whose rows start on 16 bytes are read where they lie; others are first copied to
+// rows that do, and fp32 operands are split into three bf16 planes (dcn_gemm_stage, both).
+#include "dcn_gemm.cuh"
 
 namespace dcn {
-
-cudaError_t launch_gemm_simple(const GemmArgs &g, int dtype, cudaStream_t s);
 
 namespace {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 size_t esize(int dtype) { return dtype == DCN_DTYPE_F32 ? 4 : 2; }
+int planes_of(int dtype) { return dtype == DCN_DTYPE_F32 ? 3 : 1; }
+long long pitch_of(long long cols) { return (cols + 7) / 8 * 8; }
+size_t plane_bytes(int dtype, long long rows, long long cols) {
+  return up256((size_t)planes_of(dtype) * rows * pitch_of(cols) * 2);
+}
 
-// gz = gy * act'(z), dense [rows, cols]; one thread per element, rows in blockIdx.y strides
-template <typename T>
-__global__ void __launch_bounds__(256) linear_gz(const T *__restrict__ gy, long long ldgy, const void *saved,
-                                                 int act, long long rows, long long cols, T *__restrict__ gz) {
-  const long long words = (cols + 31) / 32;
-  for (long long idx = blockIdx.x * 256LL + threadIdx.x; idx < rows * cols; idx += gridDim.x * 256LL) {
-    const long long r = idx / cols, c = idx - r * cols;
-    float v = ElemOf<T>::to(gy[r * ldgy + c]);
-    if (act == DCN_ACT_RELU)
-      v = ((((const uint32_t *)saved)[r * words + c / 32] >> (c & 31)) & 1u) ? v : 0.f;
-    else
-      v *= gelu_slope(ElemOf<T>::to(((const T *)saved)[idx]));
-    gz[idx] = ElemOf<T>::from(v);
+// Byte offsets of a pass's scratch tensors; total in `bytes`.
+struct Layout {
+  size_t gz = 0, x = 0, w = 0, part = 0, row_part = 0, sums = 0, bytes = 0;
+  bool stage_gz = false, stage_x = false, stage_w = false;
+  GemmPlan gx_plan = {}, gw_plan = {};
+};
+size_t take(Layout *l, size_t n) {
+  const size_t at = l->bytes;
+  l->bytes += up256(n);
+  return at;
+}
+bool needs_stage(int dtype, int64_t alignment) { return dtype == DCN_DTYPE_F32 || (alignment & 15) != 0; }
+
+Layout forward_layout(int dtype, long long rows, long long cin, long long cout, int64_t alignment) {
+  Layout l;
+  l.stage_x = l.stage_w = needs_stage(dtype, alignment);
+  if (l.stage_x) {
+    l.x = take(&l, plane_bytes(dtype, rows, cin));
+    l.w = take(&l, plane_bytes(dtype, cout, cin));
   }
+  return l;
 }
 
-// gb[c] = sum_r gz[r, c] where the product that could carry it is not run: a block owns 32 columns
-template <typename T>
-__global__ void __launch_bounds__(1024) linear_column_sum(const T *__restrict__ gz, long long ld, long long rows,
-                                                          long long cols, T *__restrict__ gb) {
-  __shared__ float part[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long long c = blockIdx.x * 32LL + tx;
-  float s = 0.f;
-  if (c < cols)
-    for (long long r = ty; r < rows; r += 32) s += ElemOf<T>::to(gz[r * ld + c]);
-  part[ty][tx] = s;
-  __syncthreads();
-  for (int d = 16; d > 0; d >>= 1) {
-    if (ty < d) part[ty][tx] += part[ty + d][tx];
-    __syncthreads();
+Layout backward_layout(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment,
+                       bool want_gx, bool want_gw) {
+  Layout l;
+  const bool stage = needs_stage(dtype, alignment);
+  l.stage_gz = stage || act != DCN_ACT_NONE || !want_gw;   // the last: column sums come from that pass
+  l.stage_x = stage && want_gw;
+  l.stage_w = stage && want_gx;
+  if (l.stage_gz) l.gz = take(&l, plane_bytes(dtype, rows, cout));
+  if (l.stage_x) l.x = take(&l, plane_bytes(dtype, rows, cin));
+  if (l.stage_w) l.w = take(&l, plane_bytes(dtype, cout, cin));
+  if (want_gx) l.gx_plan = plan_gemm(planes_of(dtype), rows, cin, cout, false);
+  if (want_gw) {
+    l.gw_plan = plan_gemm(planes_of(dtype), cout, cin, rows, true);
+    l.part = take(&l, l.gw_plan.part_bytes);
+    l.row_part = take(&l, l.gw_plan.row_part_bytes);
   }
-  if (ty == 0 && c < cols) gb[c] = ElemOf<T>::from(part[0][tx]);
-}
-
-template <typename T>
-cudaError_t run_gz(const void *gy, long long ldgy, const void *saved, int act, long long rows, long long cols,
-                   void *gz, cudaStream_t s) {
-  const long long blocks = (rows * cols + 255) / 256;
-  linear_gz<T><<<(int)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, s>>>((const T *)gy, ldgy, saved, act, rows,
-                                                                            cols, (T *)gz);
-  return cudaGetLastError();
-}
-template <typename T>
-cudaError_t run_column_sum(const void *gz, long long ld, long long rows, long long cols, void *gb, cudaStream_t s) {
-  linear_column_sum<T><<<(int)((cols + 31) / 32), 1024, 0, s>>>((const T *)gz, ld, rows, cols, (T *)gb);
-  return cudaGetLastError();
+  if (l.stage_gz) l.sums = take(&l, (size_t)stage_slabs(rows, cout) * cout * 4);
+  return l;
 }
 
 int check_sizes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t cout) {
@@ -75,6 +74,13 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t c
   if (rows > most || cin > (1 << 20) || cout > (1 << 20))
     return set_error(DCN_ERR_UNSUPPORTED, "linear: at most 2^31 rows and 2^20 channels");
   return DCN_OK;
+}
+
+cudaError_t stage_operand(const void *src, long long ld, long long rows, long long cols, int dtype, void *dst,
+                          cudaStream_t s, const void **at, long long *pitch) {
+  *at = dst;
+  *pitch = pitch_of(cols);
+  return launch_gemm_stage(src, ld, nullptr, DCN_ACT_NONE, rows, cols, dtype, dst, *pitch, nullptr, nullptr, s);
 }
 
 int cuda_error(cudaError_t e) { return set_error(DCN_ERR_CUDA, cudaGetErrorString(e)); }
@@ -91,8 +97,7 @@ int dcn_linear_workspace_bytes(int32_t dtype, int64_t rows, int64_t cin, int64_t
   if (!bytes) return set_error(DCN_ERR_ARG, "linear: bytes is NULL");
   int rc = check_sizes(dtype, DCN_ACT_NONE, rows, cin, cout);
   if (rc) return rc;
-  (void)alignment;
-  *bytes = 0;
+  *bytes = forward_layout(dtype, rows, cin, cout, alignment).bytes;
   return DCN_OK;
 }
 
@@ -106,13 +111,28 @@ int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t l
   if (!x || !weight || !y) return set_error(DCN_ERR_ARG, "linear: x, weight and y must be non-NULL");
   if (ldx < cin || ldw < cin || (residual && ldr < cout))
     return set_error(DCN_ERR_ARG, "linear: a row stride is smaller than the row");
+  if (act == DCN_ACT_GELU && !aligned16(saved)) return set_error(DCN_ERR_ARG, "linear: saved must be 16-byte aligned");
   LayerDeviceScope scope(device);
   if (scope.err != cudaSuccess) return cuda_error(scope.err);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t es = (int64_t)esize(dtype);
+  if (rows == 1) ldx = pitch_of(cin);   // a single row has no stride
+  const int64_t alignment = (int64_t)(uintptr_t)x | (int64_t)(uintptr_t)weight | ((ldx | ldw) * es);
+  const Layout l = forward_layout(dtype, rows, cin, cout, alignment);
+  if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
+    return set_error(DCN_ERR_WORKSPACE, "linear: workspace missing, too small or misaligned");
+  uint8_t *ws = (uint8_t *)workspace;
+  cudaError_t e = cudaSuccess;
   GemmArgs g = {};
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = ldw;
   g.m = rows; g.n = cout; g.kk = cin;
   g.bias = bias; g.act = act; g.saved = saved; g.res = residual; g.ldr = ldr; g.out = y;
-  cudaError_t e = launch_gemm_simple(g, dtype, (cudaStream_t)stream);
+  if (l.stage_x) {
+    e = stage_operand(x, ldx, rows, cin, dtype, ws + l.x, s, &g.a, &g.lda);
+    if (e == cudaSuccess) e = stage_operand(weight, ldw, cout, cin, dtype, ws + l.w, s, &g.b, &g.ldb);
+    if (e != cudaSuccess) return cuda_error(e);
+  }
+  e = launch_gemm_tc(g, plan_gemm(planes_of(dtype), rows, cout, cin, false), dtype, nullptr, nullptr, s);
   return e == cudaSuccess ? DCN_OK : cuda_error(e);
 }
 
@@ -121,8 +141,7 @@ int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows
   if (!bytes) return set_error(DCN_ERR_ARG, "linear: bytes is NULL");
   int rc = check_sizes(dtype, act, rows, cin, cout);
   if (rc) return rc;
-  (void)alignment; (void)want_gx; (void)want_gw;
-  *bytes = act == DCN_ACT_NONE ? 0 : up256((size_t)rows * cout * esize(dtype));
+  *bytes = rows ? backward_layout(dtype, act, rows, cin, cout, alignment, want_gx != 0, want_gw != 0).bytes : 0;
   return DCN_OK;
 }
 
@@ -148,43 +167,58 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
     return set_error(DCN_ERR_ARG, "linear backward: a needed pointer is NULL");
   if (ldgy < cout || (gw && ldx < cin) || (gx && ldw < cin))
     return set_error(DCN_ERR_ARG, "linear backward: a row stride is smaller than the row");
-  size_t need = 0;
-  dcn_linear_backward_workspace_bytes(dtype, act, rows, cin, cout, 0, gx != nullptr, gw != nullptr, &need);
-  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
-    return set_error(DCN_ERR_WORKSPACE, "linear backward: workspace missing, too small or misaligned");
+  if ((act == DCN_ACT_GELU && !aligned16(saved)) || (in_act == DCN_ACT_GELU && !aligned16(in_saved)))
+    return set_error(DCN_ERR_ARG, "linear backward: saved and in_saved must be 16-byte aligned");
   if (!gx && !gw && !gb) return DCN_OK;
-  const void *gz = gy;
-  long long ldgz = ldgy;
-  if (act != DCN_ACT_NONE) {
-    if (dtype == DCN_DTYPE_F32) e = run_gz<float>(gy, ldgy, saved, act, rows, cout, workspace, s);
-    else if (dtype == DCN_DTYPE_BF16) e = run_gz<__nv_bfloat16>(gy, ldgy, saved, act, rows, cout, workspace, s);
-    else e = run_gz<__half>(gy, ldgy, saved, act, rows, cout, workspace, s);
-    if (e != cudaSuccess) return cuda_error(e);
-    gz = workspace;
-    ldgz = cout;
+  const int64_t es = (int64_t)esize(dtype);
+  if (rows == 1) { ldgy = pitch_of(cout); ldx = pitch_of(cin); }   // a single row has no stride
+  const int64_t alignment = (int64_t)(uintptr_t)gy | (gw ? (int64_t)(uintptr_t)x | ldx * es : 0) |
+                            (gx ? (int64_t)(uintptr_t)weight | ldw * es : 0) | ldgy * es;
+  const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr);
+  if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
+    return set_error(DCN_ERR_WORKSPACE, "linear backward: workspace missing, too small or misaligned");
+  uint8_t *ws = (uint8_t *)workspace;
+  const void *gz = gy, *xs = x, *wt = weight;
+  long long ldgz = ldgy, ldxs = ldx, ldwt = ldw;
+  // the bias gradient: column sums from the staging pass (fp32, or without a weight gradient), else row
+  // sums of the weight gradient's A operand
+  const bool sums = gb && l.stage_gz && (dtype == DCN_DTYPE_F32 || !gw);
+  if (l.stage_gz) {
+    int slabs = 0;
+    ldgz = pitch_of(cout);
+    e = launch_gemm_stage(gy, ldgy, saved, act, rows, cout, dtype, ws + l.gz, ldgz,
+                          sums ? (float *)(ws + l.sums) : nullptr, &slabs, s);
+    if (e == cudaSuccess && sums) e = launch_column_reduce((const float *)(ws + l.sums), slabs, cout, dtype, gb, s);
+    gz = ws + l.gz;
   }
+  if (e == cudaSuccess && l.stage_x) e = stage_operand(x, ldx, rows, cin, dtype, ws + l.x, s, &xs, &ldxs);
+  if (e == cudaSuccess && l.stage_w) e = stage_operand(weight, ldw, cout, cin, dtype, ws + l.w, s, &wt, &ldwt);
+  if (e != cudaSuccess) return cuda_error(e);
   if (gx) {
     GemmArgs g = {};
-    g.a = gz; g.lda = ldgz; g.b = weight; g.ldb = ldw; g.b_mn = true;
+    g.a = gz; g.lda = ldgz; g.b = wt; g.ldb = ldwt; g.b_mn = true;
     g.m = rows; g.n = cin; g.kk = cout;
     g.slope = in_saved; g.slope_act = in_act; g.res = gx_add; g.ldr = cin; g.out = gx;
-    e = launch_gemm_simple(g, dtype, s);
+    e = launch_gemm_tc(g, l.gx_plan, dtype, nullptr, nullptr, s);
     if (e != cudaSuccess) return cuda_error(e);
   }
   if (gw) {
     GemmArgs g = {};
-    g.a = gz; g.lda = ldgz; g.a_mn = true; g.b = x; g.ldb = ldx; g.b_mn = true;
+    g.a = gz; g.lda = ldgz; g.a_mn = true; g.b = xs; g.ldb = ldxs; g.b_mn = true;
     g.m = cout; g.n = cin; g.kk = rows;
-    g.out = gw; g.row_sum = gb;
-    e = launch_gemm_simple(g, dtype, s);
-    if (e != cudaSuccess) return cuda_error(e);
-  } else if (gb) {
-    if (dtype == DCN_DTYPE_F32) e = run_column_sum<float>(gz, ldgz, rows, cout, gb, s);
-    else if (dtype == DCN_DTYPE_BF16) e = run_column_sum<__nv_bfloat16>(gz, ldgz, rows, cout, gb, s);
-    else e = run_column_sum<__half>(gz, ldgz, rows, cout, gb, s);
+    g.out = gw; g.row_sum = sums ? nullptr : gb;
+    e = launch_gemm_tc(g, l.gw_plan, dtype, (float *)(ws + l.part), (float *)(ws + l.row_part), s);
     if (e != cudaSuccess) return cuda_error(e);
   }
   return DCN_OK;
+}
+
+int dcn_linear_read_status(int32_t device, void *stream, int32_t *status) {
+  if (!status) return set_error(DCN_ERR_ARG, "linear: status is NULL");
+  LayerDeviceScope scope(device);
+  if (scope.err != cudaSuccess) return cuda_error(scope.err);
+  const cudaError_t e = read_gemm_status((cudaStream_t)stream, status);
+  return e == cudaSuccess ? DCN_OK : cuda_error(e);
 }
 
 }  // extern "C"
