@@ -18,6 +18,7 @@ from . import _lib
 _FP32_MATH = {'ffma': _lib.MATH_FFMA, 'tf32x3': _lib.MATH_TF32X3}
 _fp32_math = os.environ.get('DCN_B200_FP32_MATH', 'tf32x3').lower()
 _check_status = os.environ.get('DCN_B200_CHECK_STATUS', '0') == '1'
+_status_listeners = []   # told when the flag changes
 
 
 def set_fp32_math(mode: str) -> None:
@@ -33,6 +34,8 @@ def set_check_status(flag: bool) -> None:
     """Read the device status word after every call (synchronises)."""
     global _check_status
     _check_status = bool(flag)
+    for listener in _status_listeners:
+        listener(_check_status)
 
 
 def _dtype_code(t):

@@ -1,4 +1,6 @@
-"""Compile the CUDA sources into ``mmcv_b200/lib/libdcn_b200.so`` (sm_100a only).
+"""Compile the CUDA sources into ``mmcv_b200/lib/libdcn_b200.so`` (sm_100a only) and the tensor front
+of the transformer-layer operators into ``mmcv_b200/lib/_layers_native.so`` (host code, linked against
+torch and that library).
 
 ``python -m mmcv_b200.build_ext [--force] [--verbose]``.  nvcc cross-compiles
 without a GPU; the resulting library is loaded through ctypes by ``_lib.py``.
@@ -19,6 +21,11 @@ NVCC = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
 EXTRA_FLAGS = os.environ.get('DCN_B200_NVCC_FLAGS', '').split()   # e.g. -DDCN_TC2_ABLATE for experiments
 
 
+BINDING_SRC = os.path.join(CSRC, 'layers_binding.cpp')
+BINDING = os.path.join(LIB_DIR, '_layers_native.so')
+CXX = os.environ.get('CXX', 'g++')
+
+
 def _deps():
     out = [os.path.join(ROOT, 'include', 'dcn_b200.h')]
     for f in sorted(os.listdir(CSRC)):
@@ -32,6 +39,31 @@ def up_to_date():
         return False
     t = os.path.getmtime(LIB)
     return all(os.path.getmtime(d) <= t for d in _deps())
+
+
+def build_binding(force=False):
+    """layers_binding.cpp -> _layers_native.so; it calls the C ABI, so only the header and its own source
+    make it stale."""
+    deps = [BINDING_SRC, os.path.join(ROOT, 'include', 'dcn_b200.h')]
+    if not force and os.path.exists(BINDING) and all(
+            os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    include = cpp_extension.include_paths() + [sysconfig.get_paths()['include'], '/usr/local/cuda/include',
+                                               os.path.join(ROOT, 'include')]
+    cmd = [CXX, '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}']
+    for i in include:
+        cmd += ['-isystem', i]
+    cmd += [BINDING_SRC, '-o', BINDING, '-L', LIB_DIR, '-l:libdcn_b200.so', '-L', torch_lib, '-lc10', '-lc10_cuda',
+            '-ltorch_cpu', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f'{CXX} failed on {BINDING_SRC}:\n{r.stdout}{r.stderr}')
+    return BINDING
 
 
 def _compile(src, obj, verbose):
@@ -53,6 +85,7 @@ def _compile(src, obj, verbose):
 
 def build(force=False, verbose=False):
     if not force and up_to_date():
+        build_binding()
         return LIB
     from concurrent.futures import ThreadPoolExecutor
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -75,6 +108,7 @@ def build(force=False, verbose=False):
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError('nvcc failed linking libdcn_b200.so')
+    build_binding(force)
     return LIB
 
 

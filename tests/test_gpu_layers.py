@@ -351,6 +351,16 @@ def test_autocast_follows_torch():
     assert torch.equal(y, ref)
 
 
+def test_a_second_derivative_is_refused():
+    x, gy, w1, b1, w2, b2, g, b = block_inputs(torch.float32)
+    for f in (lambda t: ops.fused_linear(t, w1, b1, activation='gelu'), lambda t: ops.layer_norm(t, (64,), g, b),
+              lambda t: ops.feed_forward(t, w1, b1, w2, b2, t)):
+        leaf = x.detach().requires_grad_(True)
+        first, = torch.autograd.grad(f(leaf).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match='cannot be differentiated again'):
+            first.sum().backward()
+
+
 def test_layers_match_their_torch_forms():
     torch.manual_seed(0)
     for act in ('ReLU', 'GELU'):

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from mmcv_b200 import _layers, _lib, ops
+from mmcv_b200 import _lib, ops
 from oracle import layers as plain
 
 
@@ -63,16 +63,6 @@ def test_c_entries_reject_bad_arguments_without_a_device():
     assert norm(p, 8, None, None, p, None, 5, 5, 4, 8, 1e-5, 0, None) == -2
     assert norm(p, 0, None, None, p, None, 0, 0, 4, 0, 1e-5, 0, None) == -1
     assert lib.dcn_layer_norm_workspace_bytes(10, 16, ctypes.byref(n)) == 0 and n.value >= 10 * 2 * 16 * 4
-
-
-def test_row_views_are_taken_as_they_lie_or_copied():
-    t = torch.arange(60.).view(6, 10)
-    for v, cols, ld, same in [(t, 10, 10, True), (t[:, 2:7], 5, 10, True), (t[::2], 10, 20, True),
-                              (t.t(), 6, 6, False), (t[:1].expand(6, 10), 10, 10, False), (t[:1, 3:5], 2, 2, True),
-                              (t[:, :1], 1, 10, True), (t.view(2, 3, 10)[:, :, 1:9], 8, 10, True)]:
-        rows, got = _layers.as_rows(v, cols)
-        assert rows.shape == (v.numel() // cols, cols) and got == ld
-        assert torch.equal(rows, v.reshape(-1, cols)) and (rows.data_ptr() == v.data_ptr()) == same
 
 
 def test_plain_forms_against_torch():
