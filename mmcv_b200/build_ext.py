@@ -23,7 +23,7 @@ EXTRA_FLAGS = os.environ.get('DCN_B200_NVCC_FLAGS', '').split()   # e.g. -DDCN_T
 
 BINDING_SRC = os.path.join(CSRC, 'layers_binding.cpp')
 BINDING = os.path.join(LIB_DIR, '_layers_native.so')
-CXX = os.environ.get('CXX', 'g++')
+CXX = os.environ.get('DCN_B200_CXX', 'g++')   # the compiler nvcc uses too: one C++ runtime in the process
 
 
 def _deps():

@@ -49,6 +49,7 @@ struct alignas(64) GemmTc {
   int tiles_m, tiles_n, splits, kb_total, kb_split;
   int stages;
   int out_tma, res_tma;            // 0: element by element
+  int bias16;                      // the bias starts on 16 bytes
   int nbuf;                        // staging chunks of a warp
   long long ldz;                   // row stride of kept pre-activations: a multiple of 8
   float *row_part;                 // [splits][m], with splits > 1
@@ -177,32 +178,78 @@ __device__ __forceinline__ void stage_store(uint8_t *row, int sw, int q0, const 
   }
 }
 
+// v[0..31] += bias[j1 ..]; whole groups of a bias that starts on 16 bytes by 16-byte loads (the same
+// address in every lane)
+template <typename TO>
+__device__ __forceinline__ void add_bias(const TO *bias, long long j1, long long n, bool vec, float (&v)[32]) {
+  if (vec && j1 + 32 <= n) {
+    constexpr int E = 16 / (int)sizeof(TO);
+    uint4 u[32 / E];
+#pragma unroll
+    for (int i = 0; i < 32 / E; ++i) u[i] = __ldg(reinterpret_cast<const uint4 *>(bias + j1) + i);
+#pragma unroll
+    for (int i = 0; i < 32 / E; ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(TO) == 4) {
+          v[4 * i + k] += __uint_as_float(w[k]);
+        } else if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
+          v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
+          v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+          v[8 * i + 2 * k] += f.x;
+          v[8 * i + 2 * k + 1] += f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += j1 + j < n ? ElemOf<TO>::to(__ldg(bias + j1 + j)) : 0.f;
+  }
+}
+
 // The element-by-element forms of the chunk's tensor load and store, for tensors whose rows do not
 // start on 16 bytes: the warp walks the 32 rows, neighbouring lanes on neighbouring columns.
 template <typename TO>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  const int at = c * (int)sizeof(TO);
+  return r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4));
+}
+template <typename TO>
 __device__ __forceinline__ void chunk_in(uint8_t *chunk, const TO *src, long long ld, long long i0, long long m,
                                          long long j0, long long n, int lane) {
-  constexpr int CW = 128 / (int)sizeof(TO);
-  for (int r = 0; r < 32 && i0 + r < m; ++r)
+  constexpr int CW = 128 / (int)sizeof(TO), P = CW / 32;
+  const int rows = (int)min(32LL, m - i0);
+  src += i0 * ld + j0;
+  for (int r0 = 0; r0 < rows; r0 += 8) {   // eight rows in flight
+    TO v[8][P];
 #pragma unroll
-    for (int c = lane; c < CW; c += 32)
-      if (j0 + c < n) {
-        const int at = c * (int)sizeof(TO);
-        *reinterpret_cast<TO *>(chunk + r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4))) = src[(i0 + r) * ld + j0 + c];
-      }
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < P; ++c)
+        if (r0 + r < rows && j0 + c * 32 + lane < n) v[r][c] = src[(r0 + r) * ld + c * 32 + lane];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < P; ++c)
+        if (r0 + r < rows && j0 + c * 32 + lane < n)
+          *reinterpret_cast<TO *>(chunk + chunk_at<TO>(r0 + r, c * 32 + lane)) = v[r][c];
+  }
 }
 template <typename TO>
 __device__ __forceinline__ void chunk_out(const uint8_t *chunk, TO *dst, long long ld, long long i0, long long m,
                                           long long j0, long long n, int lane) {
-  constexpr int CW = 128 / (int)sizeof(TO);
-  for (int r = 0; r < 32 && i0 + r < m; ++r)
+  constexpr int CW = 128 / (int)sizeof(TO), P = CW / 32;
+  const int rows = (int)min(32LL, m - i0);
+  dst += i0 * ld + j0;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r)
 #pragma unroll
-    for (int c = lane; c < CW; c += 32)
-      if (j0 + c < n) {
-        const int at = c * (int)sizeof(TO);
-        dst[(i0 + r) * ld + j0 + c] =
-            *reinterpret_cast<const TO *>(chunk + r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4)));
-      }
+    for (int c = 0; c < P; ++c)
+      if (j0 + c * 32 + lane < n)
+        dst[r * ld + c * 32 + lane] = *reinterpret_cast<const TO *>(chunk + chunk_at<TO>(r, c * 32 + lane));
 }
 
 }  // namespace
@@ -264,6 +311,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();
+  pdl_launch();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t items = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
 
@@ -283,13 +332,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
     for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const Item it = decode(item, p, BN);
       const long long i0 = it.m0 + q * 32, row = i0 + lane;
+      const long long jw = it.n0 + h * kWarpCols;   // this warp's first column
+      const int chunks = mine && jw < g.n ? (int)((min(g.n - jw, (long long)kWarpCols) + CW - 1) / CW) : 0;
+      // what a chunk takes in, from the chunk's own place: asked for as soon as the store of the result
+      // that lay there has been read, the first chunk's under the main loop
+      auto fetch = [&](long long j0) {
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+        if (g.res) {
+          if (!p.res_tma) {
+            chunk_in<TO>(chunk, (const TO *)g.res, g.ldr, i0, g.m, j0, g.n, lane);
+          } else if (lane == 0) {
+            fence_proxy_async_smem();
+            mbar_arrive_expect_tx(rb, kChunkBytes);
+            tma_load_3d(chunk_u, &p.res, (int)j0, (int)i0, 0, rb);
+          }
+        }
+        if (kAuxStaged && aux_in && lane == 0) {
+          fence_proxy_async_smem();
+          mbar_arrive_expect_tx(ab, kChunkBytes);
+          tma_load_3d(aux_u, &p.aux, (int)j0, (int)i0, 0, ab);
+        }
+      };
+      if (chunks) fetch(jw);
       float facc[PL == 3 ? kWarpCols : 1];
       const int units = PL == 3 ? (it.kb1 - it.kb0 + kUnitBlocks - 1) / kUnitBlocks : 1;
       int buf = 0;
       for (int u = 0; u < units && ok; ++u, ++unit) {
         buf = kBufs == 2 ? (int)(unit & 1) : 0;
         const uint32_t ph = kBufs == 2 ? (unit >> 1) & 1u : unit & 1u;
-        ok = __all_sync(0xffffffffu, g_wait(tmem_full + 8 * buf, ph, abort_s, 3, 2 * limit, 64));
+        ok = __all_sync(0xffffffffu, g_wait(tmem_full + 8 * buf, ph, abort_s, 3, 2 * limit, 32));
         if (!ok) break;
         tc_fence_after();
         if constexpr (PL == 3) {
@@ -322,145 +394,124 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
           else ((TI *)g.row_sum)[row] = ElemOf<TI>::from(v);
         }
       }
-      if (mine) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < kWarpCols; c0 += CW) {
-          const long long j0 = it.n0 + h * kWarpCols + c0;
-          if (j0 >= g.n) break;
-          const int sw = lane & 7;
-          uint8_t *my = chunk + lane * 128, *my_aux = aux + lane * 128;
-          // the chunk's last store has been read
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-          if (g.res) {
-            if (p.res_tma) {
-              if (lane == 0) {
-                fence_proxy_async_smem();
-                mbar_arrive_expect_tx(rb, kChunkBytes);
-                tma_load_3d(chunk_u, &p.res, (int)j0, (int)i0, 0, rb);
-              }
-            } else {
-              chunk_in<TO>(chunk, (const TO *)g.res, g.ldr, i0, g.m, j0, g.n, lane);
+      for (int ch = 0; ch < chunks; ++ch) {
+        const long long j0 = jw + ch * CW;
+        const int sw = lane & 7;
+        uint8_t *my = chunk + lane * 128, *my_aux = aux + lane * 128;
+        if (ch) fetch(j0);
+        uint32_t acc[PL == 1 ? CW : 1];
+        if constexpr (PL == 1) {
+          const uint32_t t = lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols + ch * CW);
+#pragma unroll
+          for (int c = 0; c < CW; c += 32) tmem_ld32(t + c, *reinterpret_cast<uint32_t(*)[32]>(acc + c));
+        }
+        if (g.res && p.res_tma) {
+          ok = __all_sync(0xffffffffu, g_wait(rb, rph, abort_s, 8, 2 * limit, 0));
+          rph ^= 1u;
+        }
+        if (kAuxStaged && aux_in) {
+          ok = __all_sync(0xffffffffu, g_wait(ab, aph, abort_s, 9, 2 * limit, 0)) && ok;
+          aph ^= 1u;
+        }
+        if constexpr (PL == 1) {
+          tmem_ld_wait();
+          if (ch == chunks - 1) {   // the accumulator is in registers: the next tile may have its place
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+          }
+        }
+        if (!ok) break;
+        __syncwarp();
+#pragma unroll
+        for (int c1 = 0; c1 < CW; c1 += 32) {
+          const int q0 = c1 / 8;   // first 16-byte piece (16-bit types; fp32 chunks hold one group of 32)
+          const long long j1 = j0 + c1;
+          float v[32];
+          if constexpr (PL == 3) {
+            // ch is a runtime index: pick the group without indexing registers dynamically
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              v[j] = facc[j];
+              if constexpr (kWarpCols > 32) v[j] = ch ? facc[32 + j] : v[j];
             }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[c1 + j]);
           }
-          if (kAuxStaged && aux_in && lane == 0) {
-            fence_proxy_async_smem();
-            mbar_arrive_expect_tx(ab, kChunkBytes);
-            tma_load_3d(aux_u, &p.aux, (int)j0, (int)i0, 0, ab);
-          }
-          if (g.res && p.res_tma) {
-            ok = __all_sync(0xffffffffu, g_wait(rb, rph, abort_s, 8, 2 * limit, 0));
-            rph ^= 1u;
-          }
-          if (kAuxStaged && aux_in) {
-            ok = __all_sync(0xffffffffu, g_wait(ab, aph, abort_s, 9, 2 * limit, 0)) && ok;
-            aph ^= 1u;
-          }
-          if (!ok) break;
-          __syncwarp();
-#pragma unroll
-          for (int c1 = 0; c1 < CW; c1 += 32) {
-            const int q0 = c1 / 8;   // first 16-byte piece (16-bit types; fp32 chunks hold one group of 32)
-            float v[32];
-            if constexpr (PL == 3) {
-              // c0 is a runtime index: pick the group without indexing registers dynamically
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                v[j] = facc[j];
-                if constexpr (kWarpCols > 32) v[j] = c0 ? facc[32 + j] : v[j];
-              }
-            } else {
-              uint32_t r[32];
-              tmem_ld32(lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols + c0 + c1), r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-            }
-            const long long j1 = j0 + c1;
-            if (g.bias) {
-              const TO *bp = (const TO *)g.bias + j1;
-              if (j1 + 32 <= g.n) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += ElemOf<TO>::to(__ldg(bp + j));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += j1 + j < g.n ? ElemOf<TO>::to(__ldg(bp + j)) : 0.f;
-              }
-            }
-            if (g.act != DCN_ACT_NONE) {
-              if (g.saved) {
-                if (g.act == DCN_ACT_RELU) {
-                  uint32_t bits = 0;
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) bits |= (uint32_t)relu_bit(v[j]) << j;
-                  if (row < g.m && j1 < g.n) ((uint32_t *)g.saved)[row * words + (j1 >> 5)] = bits;
-                } else {
-                  if constexpr (kAuxStaged) {
-                    stage_store<TO>(my_aux, sw, q0, v);
-                  } else if (row < g.m) {
-                    float4 *zp = reinterpret_cast<float4 *>((float *)g.saved + row * p.ldz + j1);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                      if (j1 + 4 * i < p.ldz) zp[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                  }
-                }
-              }
+          if (g.bias) add_bias<TO>((const TO *)g.bias, j1, g.n, p.bias16 != 0, v);
+          if (g.act != DCN_ACT_NONE) {
+            if (g.saved) {
               if (g.act == DCN_ACT_RELU) {
+                uint32_t bits = 0;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = act_value(DCN_ACT_GELU, v[j]);
-              }
-            }
-            if (g.slope_act == DCN_ACT_RELU) {
-              const uint32_t bits =
-                  row < g.m && j1 < g.n ? __ldg((const uint32_t *)g.slope + row * words + (j1 >> 5)) : 0u;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.f;
-            } else if (aux_in) {
-              if constexpr (kAuxStaged) {
-                float z[32];
-                stage_load<TO>(my_aux, sw, q0, z);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= gelu_slope(z[j]);
+                for (int j = 0; j < 32; ++j) bits |= relu_bit(v[j]) ? 1u << j : 0u;
+                if (row < g.m && j1 < g.n) ((uint32_t *)g.saved)[row * words + (j1 >> 5)] = bits;
+              } else if constexpr (kAuxStaged) {
+                stage_store<TO>(my_aux, sw, q0, v);
               } else if (row < g.m) {
-                const float4 *zp = reinterpret_cast<const float4 *>((const float *)g.slope + row * p.ldz + j1);
+                float4 *zp = reinterpret_cast<float4 *>((float *)g.saved + row * p.ldz + j1);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                  if (j1 + 4 * i < p.ldz) {
-                    const float4 z = __ldg(zp + i);
-                    v[4 * i] *= gelu_slope(z.x);
-                    v[4 * i + 1] *= gelu_slope(z.y);
-                    v[4 * i + 2] *= gelu_slope(z.z);
-                    v[4 * i + 3] *= gelu_slope(z.w);
-                  }
+                  if (j1 + 4 * i < p.ldz) zp[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
               }
             }
-            if (g.res) {
-              float r[32];
-              stage_load<TO>(my, sw, q0, r);
+            if (g.act == DCN_ACT_RELU) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] += r[j];
+              for (int j = 0; j < 32; ++j) v[j] = relu_value(v[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = gelu_value<PL == 3>(v[j]);
             }
-            stage_store<TO>(my, sw, q0, v);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (p.out_tma) {
-            if (lane == 0) tma_store_3d(&p.out, chunk_u, (int)j0, (int)i0, it.split);
-          } else {
-            chunk_out<TO>(chunk, (TO *)g.out, g.n, i0, g.m, j0, g.n, lane);
+          if (g.slope_act == DCN_ACT_RELU) {
+            const uint32_t bits = row < g.m && j1 < g.n ? __ldg((const uint32_t *)g.slope + row * words + (j1 >> 5)) : 0u;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.f;
+          } else if (aux_in) {
+            if constexpr (kAuxStaged) {
+              float z[32];
+              stage_load<TO>(my_aux, sw, q0, z);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= gelu_slope<PL == 3>(z[j]);
+            } else if (row < g.m) {
+              const float4 *zp = reinterpret_cast<const float4 *>((const float *)g.slope + row * p.ldz + j1);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (j1 + 4 * i < p.ldz) {
+                  const float4 z = __ldg(zp + i);
+                  v[4 * i] *= gelu_slope<true>(z.x);
+                  v[4 * i + 1] *= gelu_slope<true>(z.y);
+                  v[4 * i + 2] *= gelu_slope<true>(z.z);
+                  v[4 * i + 3] *= gelu_slope<true>(z.w);
+                }
+            }
           }
-          if (kAuxStaged && aux_out && lane == 0) tma_store_3d(&p.aux, aux_u, (int)j0, (int)i0, 0);
-          if (lane == 0) bulk_commit();
-          __syncwarp();
+          if (g.res) {
+            float r[32];
+            stage_load<TO>(my, sw, q0, r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += r[j];
+          }
+          stage_store<TO>(my, sw, q0, v);
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (!p.out_tma) chunk_out<TO>(chunk, (TO *)g.out, g.n, i0, g.m, j0, g.n, lane);
+        if (lane == 0) {
+          if (p.out_tma) tma_store_3d(&p.out, chunk_u, (int)j0, (int)i0, it.split);
+          if (kAuxStaged && aux_out) tma_store_3d(&p.aux, aux_u, (int)j0, (int)i0, 0);
+          bulk_commit();
+        }
+        __syncwarp();
       }
       if constexpr (PL == 1) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+        if (!chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+        }
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -579,6 +630,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__ part, int splits, long long m,
                                                        long long n, long long ldp, T *__restrict__ out) {
   const long long per_row = ldp / 4, idx = blockIdx.x * 256LL + threadIdx.x;
+  pdl_wait();
+  pdl_launch();
   if (idx >= m * per_row) return;
   const long long i = idx / per_row, j = (idx - i * per_row) * 4;
   const float4 *p = reinterpret_cast<const float4 *>(part + i * ldp + j);
@@ -603,6 +656,8 @@ __global__ void __launch_bounds__(1024) dcn_column_reduce(const float *__restric
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const long long c = blockIdx.x * 32LL + tx;
   float v = 0.f;
+  pdl_wait();
+  pdl_launch();
   if (c < cols)
     for (int p = ty; p < parts; p += 32) v += part[p * cols + c];
   sm[ty][tx] = v;
@@ -641,6 +696,8 @@ __global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
   __shared__ float red[256 * 8];
   const long long c = (blockIdx.x * (long long)blockDim.x + threadIdx.x) * 8;
   const long long words = (a.cols + 31) / 32;
+  pdl_wait();
+  pdl_launch();
   float sum[8] = {};
   if (c < a.pitch) {
     for (long long r = blockIdx.y * (long long)blockDim.y + threadIdx.y; r < a.rows; r += (long long)gridDim.y * blockDim.y) {
@@ -672,7 +729,7 @@ __global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4 *>(z)[i];
         const T *e = reinterpret_cast<const T *>(u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope(ElemOf<T>::to(e[i]));
+        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope<PL == 3>(ElemOf<T>::to(e[i]));
       }
       if constexpr (PL == 1) {
         uint32_t w[4];
@@ -784,8 +841,7 @@ cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
   p.stages = stages;
   const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
   const int grid = (int)(items < 148 ? items : 148);
-  kern<<<grid, kGemmThreads, fixed + stages * stage, s>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(kern, grid, kGemmThreads, fixed + stages * stage, s, p);
 }
 
 template <typename TI, typename TO, int PL, bool AMN, bool BMN>
@@ -808,8 +864,8 @@ cudaError_t run_order(GemmTc &p, int bn, bool parts, cudaStream_t s) {
 template <typename T>
 cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &g, cudaStream_t s) {
   const long long n = g.m * (plan.ldp / 4);
-  dcn_gemm_reduce<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(part, plan.splits, g.m, g.n, plan.ldp, (T *)g.out);
-  return cudaGetLastError();
+  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + 255) / 256), 256, 0, s, part, plan.splits, g.m, g.n, plan.ldp,
+                    (T *)g.out);
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -857,6 +913,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   p.kb_split = plan.kb_split;
   p.row_part = row_part;
   p.wait_limit_ns = kWaitLimitNs;
+  p.bias16 = aligned16(g.bias);
   bool ok = g.a_mn ? encode3(&p.a, t16, 2, g.a, g.m, g.kk, planes, g.lda, 64, 64)
                    : encode3(&p.a, t16, 2, g.a, g.kk, g.m, planes, g.lda, 64, 128);
   ok = ok && (g.b_mn ? encode3(&p.b, t16, 2, g.b, g.n, g.kk, planes, g.ldb, 64, 64)
@@ -912,19 +969,17 @@ cudaError_t launch_gemm_stage(const void *src, long long ld, const void *saved, 
   stage_shape(rows, pitch, &tx, &ty, &gx, &gy);
   if (slabs) *slabs = gy;
   const dim3 grid(gx, gy), block(tx, ty);
-  if (dtype == DCN_DTYPE_F32) dcn_gemm_stage<float, 3><<<grid, block, 0, s>>>(a);
-  else if (dtype == DCN_DTYPE_BF16) dcn_gemm_stage<__nv_bfloat16, 1><<<grid, block, 0, s>>>(a);
-  else dcn_gemm_stage<__half, 1><<<grid, block, 0, s>>>(a);
-  return cudaGetLastError();
+  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_gemm_stage<float, 3>, grid, block, 0, s, a);
+  if (dtype == DCN_DTYPE_BF16) return launch_pdl(dcn_gemm_stage<__nv_bfloat16, 1>, grid, block, 0, s, a);
+  return launch_pdl(dcn_gemm_stage<__half, 1>, grid, block, 0, s, a);
 }
 
 cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s) {
   const unsigned grid = (unsigned)((cols + 31) / 32);
-  if (dtype == DCN_DTYPE_F32) dcn_column_reduce<float><<<grid, 1024, 0, s>>>(part, parts, cols, (float *)out);
-  else if (dtype == DCN_DTYPE_BF16)
-    dcn_column_reduce<__nv_bfloat16><<<grid, 1024, 0, s>>>(part, parts, cols, (__nv_bfloat16 *)out);
-  else dcn_column_reduce<__half><<<grid, 1024, 0, s>>>(part, parts, cols, (__half *)out);
-  return cudaGetLastError();
+  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_column_reduce<float>, grid, 1024, 0, s, part, parts, cols, (float *)out);
+  if (dtype == DCN_DTYPE_BF16)
+    return launch_pdl(dcn_column_reduce<__nv_bfloat16>, grid, 1024, 0, s, part, parts, cols, (__nv_bfloat16 *)out);
+  return launch_pdl(dcn_column_reduce<__half>, grid, 1024, 0, s, part, parts, cols, (__half *)out);
 }
 
 // Reads and clears the status word of the current device, after the work on `s`.

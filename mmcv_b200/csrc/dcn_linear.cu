@@ -180,9 +180,9 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
   uint8_t *ws = (uint8_t *)workspace;
   const void *gz = gy, *xs = x, *wt = weight;
   long long ldgz = ldgy, ldxs = ldx, ldwt = ldw;
-  // the bias gradient: column sums from the staging pass (fp32, or without a weight gradient), else row
-  // sums of the weight gradient's A operand
-  const bool sums = gb && l.stage_gz && (dtype == DCN_DTYPE_F32 || !gw);
+  // the bias gradient: column sums of the staging pass, taken before gz is rounded, where there is one,
+  // else row sums of the weight gradient's A operand
+  const bool sums = gb && l.stage_gz;
   if (l.stage_gz) {
     int slabs = 0;
     ldgz = pitch_of(cout);

@@ -125,6 +125,8 @@ __global__ void __launch_bounds__(kThreads) norm_forward(const NormArgs a) {
   __shared__ float red[(G > 32 ? G / 32 : 1) * 2];
   const int t = threadIdx.x % G;
   const long long row = blockIdx.x * (long long)(kThreads / G) + threadIdx.x / G;
+  pdl_wait();
+  pdl_launch();
   if (row >= a.rows) return;   // whole groups leave together
   const T *x = (const T *)a.x + row * a.ldx;
   float v[NV][V];
@@ -184,6 +186,8 @@ __global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
   const int t = threadIdx.x % G;
   const float inv = 1.f / (float)a.cols;
   float gw[kParams ? NV : 1][V] = {}, gb[kParams ? NV : 1][V] = {};
+  pdl_wait();
+  pdl_launch();
   for (long long row = blockIdx.x * (long long)RPB + threadIdx.x / G; row < a.rows; row += (long long)gridDim.x * RPB) {
     const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * a.ldgy;
     float n[NV][V], g[NV][V];
@@ -270,6 +274,8 @@ template <typename T>
 __global__ void __launch_bounds__(1024) norm_forward_wide(const NormArgs a) {
   __shared__ float red[32 * 2];
   const long long row = blockIdx.x;
+  pdl_wait();
+  pdl_launch();
   const T *x = (const T *)a.x + row * a.ldx;
   float s[1] = {0.f};
   for (int c = threadIdx.x; c < a.cols; c += 1024) s[0] += ElemOf<T>::to(x[c]);
@@ -302,6 +308,8 @@ template <typename T>
 __global__ void __launch_bounds__(1024) norm_backward_wide(const NormArgs a) {
   __shared__ float red[32 * 2];
   const long long row = blockIdx.x;
+  pdl_wait();
+  pdl_launch();
   const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * a.ldgy;
   const float m = a.stats[row], corr = a.stats[a.rows + row], rstd = a.stats[2 * a.rows + row];
   float s[2] = {0.f, 0.f};
@@ -327,6 +335,8 @@ __global__ void __launch_bounds__(1024) norm_backward_wide(const NormArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_columns_wide(const NormArgs a) {
   const int c = blockIdx.x * kThreads + threadIdx.x;
+  pdl_wait();
+  pdl_launch();
   if (c >= a.cols) return;
   float gw = 0.f, gb = 0.f;
   for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -347,6 +357,8 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   T *out = blockIdx.y ? gb : gw;
+  pdl_wait();
+  pdl_launch();
   if (!out) return;
   float v = 0.f;
   if (c < cols)
@@ -362,10 +374,9 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
 
 template <typename T, int V, int E, int G>
 cudaError_t run_one(const NormArgs &a, bool backward, bool params, int grid, cudaStream_t s) {
-  if (!backward) norm_forward<T, V, E, G><<<grid, kThreads, 0, s>>>(a);
-  else if (params) norm_backward<T, V, E, G, true><<<grid, kThreads, 0, s>>>(a);
-  else norm_backward<T, V, E, G, false><<<grid, kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  if (!backward) return launch_pdl(norm_forward<T, V, E, G>, grid, kThreads, 0, s, a);
+  if (params) return launch_pdl(norm_backward<T, V, E, G, true>, grid, kThreads, 0, s, a);
+  return launch_pdl(norm_backward<T, V, E, G, false>, grid, kThreads, 0, s, a);
 }
 
 // E: the fewest elements to a thread that hold the row; G: a warp while that is at most 32.
@@ -389,16 +400,14 @@ cudaError_t run_rows(const NormArgs &a, bool backward, bool params, int *parts, 
 template <typename T>
 cudaError_t run(const NormArgs &a, bool backward, bool params, int *parts, cudaStream_t s) {
   if (a.cols > 8192) {
-    if (!backward) {
-      norm_forward_wide<T><<<(int)a.rows, 1024, 0, s>>>(a);
-      return cudaGetLastError();
-    }
-    if (a.y) norm_backward_wide<T><<<(int)a.rows, 1024, 0, s>>>(a);
-    if (params) {
+    if (!backward) return launch_pdl(norm_forward_wide<T>, (unsigned)a.rows, 1024, 0, s, a);
+    cudaError_t e = cudaSuccess;
+    if (a.y) e = launch_pdl(norm_backward_wide<T>, (unsigned)a.rows, 1024, 0, s, a);
+    if (e == cudaSuccess && params) {
       *parts = (int)(a.rows < 64 ? a.rows : 64);
-      norm_columns_wide<T><<<dim3((a.cols + kThreads - 1) / kThreads, *parts), kThreads, 0, s>>>(a);
+      e = launch_pdl(norm_columns_wide<T>, dim3((a.cols + kThreads - 1) / kThreads, *parts), kThreads, 0, s, a);
     }
-    return cudaGetLastError();
+    return e;
   }
   // 16-byte accesses need every row of every tensor to start on 16 bytes; the dense output's does
   // when cols is a multiple of V
@@ -492,11 +501,13 @@ int dcn_layer_norm_backward(const void *gy, int64_t ldgy, const void *x, int64_t
   e = run_typed(a, dtype, true, params, &parts, s);
   if (e == cudaSuccess && params) {
     const dim3 grid((unsigned)((cols + 31) / 32), 2);
-    if (wdtype == DCN_DTYPE_F32) norm_reduce<float><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (float *)gw, (float *)gb);
+    if (wdtype == DCN_DTYPE_F32)
+      e = launch_pdl(norm_reduce<float>, grid, 1024, 0, s, a.part, parts, a.cols, (float *)gw, (float *)gb);
     else if (wdtype == DCN_DTYPE_BF16)
-      norm_reduce<__nv_bfloat16><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (__nv_bfloat16 *)gw, (__nv_bfloat16 *)gb);
-    else norm_reduce<__half><<<grid, 1024, 0, s>>>(a.part, parts, a.cols, (__half *)gw, (__half *)gb);
-    e = cudaGetLastError();
+      e = launch_pdl(norm_reduce<__nv_bfloat16>, grid, 1024, 0, s, a.part, parts, a.cols, (__nv_bfloat16 *)gw,
+                     (__nv_bfloat16 *)gb);
+    else
+      e = launch_pdl(norm_reduce<__half>, grid, 1024, 0, s, a.part, parts, a.cols, (__half *)gw, (__half *)gb);
   }
   return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
 }

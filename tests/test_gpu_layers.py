@@ -59,6 +59,43 @@ def test_linear_forward_and_gradients(rows, cin, cout, dtype):
             assert torch.equal(ops.fused_linear(x, w, b, r, act), got['y'])
 
 
+def test_first_call_of_a_thread():
+    """A new thread has no CUDA context bound to it; a call that allocates nothing binds none before the
+    tensor maps are encoded."""
+    import threading
+    x, w, b, _, _ = linear_case(64, 64, 64, torch.bfloat16, None)
+    want, got = ops.fused_linear(x, w, b), []
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream()
+
+    def call():
+        got.append(ops.fused_linear(x, w, b))
+
+    for _ in range(2):
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+    stream.synchronize()
+    assert len(got) == 2 and all(torch.equal(g, want) for g in got)
+
+
+def test_backward_as_the_first_work_of_the_process():
+    """The engine's thread starts with this backward pass: nothing has bound a context to it."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\nfrom mmcv_b200 import ops\n"
+            "x, w, b, g = (torch.randn(s, device='cuda').bfloat16() for s in ((300, 256), (1024, 256), (1024,), (300, 1024)))\n"
+            "x.requires_grad_(True); w.requires_grad_(True); b.requires_grad_(True)\n"
+            "gx, gw, gb = torch.autograd.grad(ops.fused_linear(x, w, b), [x, w, b], g)\n"
+            "err = ((gw.double() - g.double().t() @ x.double()).norm() / gw.double().norm()).item()\n"
+            "assert err < 2 ** -8, err\n"
+            "print('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and 'done' in r.stdout, r.stdout + r.stderr
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_linear_many_rows_and_splits(dtype):
     """Enough rows that the weight gradient's sum is divided among blocks."""
