@@ -10,7 +10,10 @@
 // into fp32 accumulators in tensor memory, double-buffered so that the epilogue of a tile runs under
 // the main loop of the next; eight warps run the epilogue: tcgen05.ld, bias, activation, derivative,
 // residual, one rounding, a 32-row chunk in shared memory, a tensor store.  The residual arrives by
-// tensor load in the chunk that the result leaves from.  Every wait is bounded.
+// tensor load in the chunk that the result leaves from, as do the kept pre-activations of a derivative.
+// Sixteen epilogue warps (eight with fp32 tensors) and not four: a warp's share of a tile is a chain of waits (tensor memory,
+// loads, the store of its last chunk), and the products around an embedding of 256 have main loops of
+// four steps only (35642 x 256 x 1024 bf16 with relu: 42 us with eight warps).  Every wait is bounded.
 //
 // 16-bit tensors: one plane (PL = 1).  fp32 tensors: every operand is the exact sum of three bf16
 // planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_split writes them), and the product is
@@ -36,9 +39,17 @@ namespace dcn {
 
 namespace {
 
-constexpr int kGemmThreads = 10 * 32;   // 8 epilogue warps, MMA warp, loader warp
-constexpr int kEpiWarps = 8;
-constexpr int kChunkBytes = 4096;       // 32 rows x 128 bytes of staging
+// Epilogue warps: four to each quarter of the accumulator's rows, two where three planes take the shared
+// memory that their staging would need.  With them the MMA warp and the loader warp.
+template <int PL>
+constexpr int kEpi = PL == 3 ? 8 : 16;
+template <int PL>
+constexpr int kThreadsOf = (kEpi<PL> + 2) * 32;
+
+// Bytes of a row of an epilogue warp's staging chunk (32 rows): with 16-bit results a warp has 64
+// columns of a 256-column tile, else (at least) 32.
+template <typename TO, int BN>
+constexpr int kChunkRow = sizeof(TO) == 4 || BN == 256 ? 128 : 64;
 constexpr int kUnitBlocks = 4;          // PL = 3: 64-value blocks between two drains of the accumulators
 
 __device__ int g_gemm_status;           // the first wait that ran out (0: none), until it is read
@@ -50,7 +61,6 @@ struct alignas(64) GemmTc {
   int stages;
   int out_tma, res_tma;            // 0: element by element
   int bias16;                      // the bias starts on 16 bytes
-  int nbuf;                        // staging chunks of a warp
   long long ldz;                   // row stride of kept pre-activations: a multiple of 8
   float *row_part;                 // [splits][m], with splits > 1
   unsigned long long wait_limit_ns;
@@ -91,6 +101,16 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
@@ -125,57 +145,54 @@ __device__ __forceinline__ Item decode(uint32_t item, const GemmTc &p, int BN) {
   return it;
 }
 
-// 32 values of a staging row (128-byte swizzled, 16-byte pieces q0, q0 + 1, ...) as floats, and back.
+// A staging chunk: 32 rows of RB bytes, 16-byte pieces permuted within a row as the tensor maps'
+// swizzles of that width have them, so that the lanes of a warp, a row each, meet no bank conflicts.
+template <int RB>
+__device__ __forceinline__ int chunk_piece(int row, int q) {
+  return row * RB + ((q ^ (RB == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+}
+// 16 bytes of elements as floats, and back
 template <typename TO>
-__device__ __forceinline__ void stage_load(const uint8_t *row, int sw, int q0, float (&v)[32]) {
-  if constexpr (sizeof(TO) == 4) {
+__device__ __forceinline__ void unpack16(const uint4 &u, float *v) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float4 f = *reinterpret_cast<const float4 *>(row + ((q ^ sw) << 4));
-      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(row + (((q0 + q) ^ sw) << 4));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
-          v[8 * q + 2 * i] = __uint_as_float(w[i] << 16);
-          v[8 * q + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-          v[8 * q + 2 * i] = f.x;
-          v[8 * q + 2 * i + 1] = f.y;
-        }
-      }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(TO) == 4) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
     }
   }
 }
 template <typename TO>
-__device__ __forceinline__ void stage_store(uint8_t *row, int sw, int q0, const float (&v)[32]) {
-  if constexpr (sizeof(TO) == 4) {
+__device__ __forceinline__ uint4 pack16(const float *v) {
+  uint32_t w[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<float4 *>(row + ((q ^ sw) << 4)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        } else {
-          const __half2 h = __floats2half2_rn(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-      }
-      *reinterpret_cast<uint4 *>(row + (((q0 + q) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(TO) == 4) {
+      w[i] = __float_as_uint(v[i]);
+    } else if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
     }
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// 32 values from or to a lane's row, q0: the first 16-byte piece
+template <typename TO, int RB>
+__device__ __forceinline__ void stage_store(uint8_t *chunk, int row, int q0, const float (&v)[32]) {
+  constexpr int E = 16 / (int)sizeof(TO);
+#pragma unroll
+  for (int q = 0; q < 32 / E; ++q)
+    *reinterpret_cast<uint4 *>(chunk + chunk_piece<RB>(row, q0 + q)) = pack16<TO>(v + E * q);
 }
 
 // v[0..31] += bias[j1 ..]; whole groups of a bias that starts on 16 bytes by 16-byte loads (the same
@@ -184,25 +201,12 @@ template <typename TO>
 __device__ __forceinline__ void add_bias(const TO *bias, long long j1, long long n, bool vec, float (&v)[32]) {
   if (vec && j1 + 32 <= n) {
     constexpr int E = 16 / (int)sizeof(TO);
-    uint4 u[32 / E];
-#pragma unroll
-    for (int i = 0; i < 32 / E; ++i) u[i] = __ldg(reinterpret_cast<const uint4 *>(bias + j1) + i);
 #pragma unroll
     for (int i = 0; i < 32 / E; ++i) {
-      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      float b[E];
+      unpack16<TO>(__ldg(reinterpret_cast<const uint4 *>(bias + j1) + i), b);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(TO) == 4) {
-          v[4 * i + k] += __uint_as_float(w[k]);
-        } else if constexpr (std::is_same_v<TO, __nv_bfloat16>) {
-          v[8 * i + 2 * k] += __uint_as_float(w[k] << 16);
-          v[8 * i + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-          v[8 * i + 2 * k] += f.x;
-          v[8 * i + 2 * k + 1] += f.y;
-        }
-      }
+      for (int k = 0; k < E; ++k) v[E * i + k] += b[k];
     }
   } else {
 #pragma unroll
@@ -212,15 +216,15 @@ __device__ __forceinline__ void add_bias(const TO *bias, long long j1, long long
 
 // The element-by-element forms of the chunk's tensor load and store, for tensors whose rows do not
 // start on 16 bytes: the warp walks the 32 rows, neighbouring lanes on neighbouring columns.
-template <typename TO>
-__device__ __forceinline__ int chunk_at(int r, int c) {
+template <typename TO, int RB>
+__device__ __forceinline__ TO *chunk_at(uint8_t *chunk, int r, int c) {
   const int at = c * (int)sizeof(TO);
-  return r * 128 + ((at & 15) | (((at >> 4) ^ (r & 7)) << 4));
+  return reinterpret_cast<TO *>(chunk + chunk_piece<RB>(r, at >> 4) + (at & 15));
 }
-template <typename TO>
+template <typename TO, int RB>
 __device__ __forceinline__ void chunk_in(uint8_t *chunk, const TO *src, long long ld, long long i0, long long m,
                                          long long j0, long long n, int lane) {
-  constexpr int CW = 128 / (int)sizeof(TO), P = CW / 32;
+  constexpr int P = RB / (int)sizeof(TO) / 32;
   const int rows = (int)min(32LL, m - i0);
   src += i0 * ld + j0;
   for (int r0 = 0; r0 < rows; r0 += 8) {   // eight rows in flight
@@ -234,22 +238,27 @@ __device__ __forceinline__ void chunk_in(uint8_t *chunk, const TO *src, long lon
     for (int r = 0; r < 8; ++r)
 #pragma unroll
       for (int c = 0; c < P; ++c)
-        if (r0 + r < rows && j0 + c * 32 + lane < n)
-          *reinterpret_cast<TO *>(chunk + chunk_at<TO>(r0 + r, c * 32 + lane)) = v[r][c];
+        if (r0 + r < rows && j0 + c * 32 + lane < n) *chunk_at<TO, RB>(chunk, r0 + r, c * 32 + lane) = v[r][c];
   }
 }
-template <typename TO>
-__device__ __forceinline__ void chunk_out(const uint8_t *chunk, TO *dst, long long ld, long long i0, long long m,
+template <typename TO, int RB>
+__device__ __forceinline__ void chunk_out(uint8_t *chunk, TO *dst, long long ld, long long i0, long long m,
                                           long long j0, long long n, int lane) {
-  constexpr int CW = 128 / (int)sizeof(TO), P = CW / 32;
+  constexpr int P = RB / (int)sizeof(TO) / 32;
   const int rows = (int)min(32LL, m - i0);
   dst += i0 * ld + j0;
 #pragma unroll 8
   for (int r = 0; r < rows; ++r)
 #pragma unroll
     for (int c = 0; c < P; ++c)
-      if (j0 + c * 32 + lane < n)
-        dst[r * ld + c * 32 + lane] = *reinterpret_cast<const TO *>(chunk + chunk_at<TO>(r, c * 32 + lane));
+      if (j0 + c * 32 + lane < n) dst[r * ld + c * 32 + lane] = *chunk_at<TO, RB>(chunk, r, c * 32 + lane);
+}
+// v[0..31] += a lane's own row of the residual, for the rare epilogue whose chunk is taken
+template <typename TO>
+__device__ __forceinline__ void add_row(const TO *src, long long j1, long long n, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j1 + j < n) v[j] += ElemOf<TO>::to(__ldg(src + j));
 }
 
 }  // namespace
@@ -257,33 +266,32 @@ __device__ __forceinline__ void chunk_out(const uint8_t *chunk, TO *dst, long lo
 // PL planes per operand; TI the 16-bit type of the planes, TO the output's (and residual's) type;
 // AMN / BMN: the operand lies with its row index contiguous.
 template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN>
-__global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_constant__ GemmTc p) {
+__global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_constant__ GemmTc p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   constexpr uint32_t kABytes = PL * 16384u, kBBytes = PL * BN * 128u, kStage = kABytes + kBBytes;
+  constexpr int kEpiWarps = kEpi<PL>, kGemmThreads = kThreadsOf<PL>, kGroups = kEpiWarps / 4;
   constexpr bool kRowSum = AMN && PL == 1;             // only the weight gradient asks for row sums
   constexpr int kBufs = (kRowSum && BN == 256) ? 1 : 2;   // accumulator buffers that fit beside the row sums
   constexpr int kBufCols = PL == 3 ? 2 * BN : BN;
   constexpr int kCols = kBufs * kBufCols + (kRowSum ? 16 * kBufs : 0);
   constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512, "tensor memory");
-  constexpr int CW = 128 / (int)sizeof(TO);            // columns of a staging chunk
-  // 16-bit pre-activations pass through a second chunk; fp32 ones, whose rings leave no room for it,
-  // go straight between a lane's row (128 bytes of it at a time) and its registers
-  constexpr bool kAuxStaged = PL == 1;
-  constexpr int kWarpCols = BN / 2 > CW ? BN / 2 : CW; // columns of an epilogue warp
+  constexpr int RB = kChunkRow<TO, BN>, kChunkBytes = 32 * RB;
+  constexpr int CW = RB / (int)sizeof(TO);             // columns of a staging chunk
+  constexpr int kWarpCols = BN / kGroups > CW ? BN / kGroups : CW;   // columns of an epilogue warp
 
   const GemmArgs &g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ST = p.stages;
   const uint32_t bar0 = smem_u32(smem);
   const uint32_t full = bar0, empty = full + 8 * ST, tmem_full = empty + 8 * ST, tmem_empty = tmem_full + 16,
-                 res_bar = tmem_empty + 16;            // two per epilogue warp
+                 in_bar = tmem_empty + 16;             // one per epilogue warp
   uint32_t *tmem_slot = (uint32_t *)(smem + 896);
   volatile int *abort_s = (volatile int *)(smem + 904);
   uint8_t *ring = smem + 1024;
   uint8_t *staging = ring + (size_t)ST * kStage;
-  uint8_t *ones = staging + (size_t)kEpiWarps * p.nbuf * kChunkBytes;
+  uint8_t *ones = staging + (size_t)kEpiWarps * kChunkBytes;
   const unsigned long long limit = p.wait_limit_ns;
 
   if (threadIdx.x == 0) {
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
       mbar_init(tmem_full + 8 * i, 1);
       mbar_init(tmem_empty + 8 * i, kEpiWarps);
     }
-    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_bar + 8 * i, 1);
+    for (int i = 0; i < kEpiWarps; ++i) mbar_init(in_bar + 8 * i, 1);
     *abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
     for (int i = threadIdx.x; i < 1024; i += kGemmThreads) ((TI *)ones)[i] = ElemOf<TI>::from(1.f);
     fence_proxy_async_smem();
   }
-  if (warp == 8) {
+  if (warp == kEpiWarps) {
     tmem_alloc(smem_u32(tmem_slot), kAlloc);
     tmem_relinquish();
   }
@@ -318,40 +326,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
 
   if (warp < kEpiWarps) {
     // ------------------------------ epilogue ------------------------------
-    const int q = warp & 3, h = warp >> 2;
+    const int q = warp & 3, cg = warp >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16);
-    uint8_t *chunk = staging + (size_t)warp * p.nbuf * kChunkBytes;   // residual in, result out
-    uint8_t *aux = chunk + kChunkBytes;                               // pre-activations in or out
-    const uint32_t chunk_u = smem_u32(chunk), aux_u = smem_u32(aux);
-    const uint32_t rb = res_bar + 16 * warp, ab = rb + 8;
-    uint32_t rph = 0, aph = 0, unit = 0;
-    const bool mine = h * kWarpCols < BN;
+    uint8_t *chunk = staging + (size_t)warp * kChunkBytes;
+    const uint32_t chunk_u = smem_u32(chunk), ib = in_bar + 8 * warp;
+    uint32_t iph = 0, unit = 0;
     const long long words = (g.n + 31) / 32;
     const bool aux_in = g.slope_act == DCN_ACT_GELU, aux_out = g.saved && g.act == DCN_ACT_GELU;
+    const bool res_staged = g.res && !aux_in && !aux_out;
+    const bool load_in = aux_in || (res_staged && p.res_tma);
     bool ok = true;
     for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const Item it = decode(item, p, BN);
       const long long i0 = it.m0 + q * 32, row = i0 + lane;
-      const long long jw = it.n0 + h * kWarpCols;   // this warp's first column
-      const int chunks = mine && jw < g.n ? (int)((min(g.n - jw, (long long)kWarpCols) + CW - 1) / CW) : 0;
-      // what a chunk takes in, from the chunk's own place: asked for as soon as the store of the result
-      // that lay there has been read, the first chunk's under the main loop
+      const long long jw = it.n0 + cg * kWarpCols;   // this warp's first column
+      const int chunks =
+          cg * kWarpCols < BN && jw < g.n ? (int)((min(g.n - jw, (long long)kWarpCols) + CW - 1) / CW) : 0;
+      // what a chunk takes in, to its own place: asked for as soon as the store of the result that lay
+      // there has been read, the first chunk's under the main loop
       auto fetch = [&](long long j0) {
         if (lane == 0) bulk_wait_read();
         __syncwarp();
-        if (g.res) {
-          if (!p.res_tma) {
-            chunk_in<TO>(chunk, (const TO *)g.res, g.ldr, i0, g.m, j0, g.n, lane);
-          } else if (lane == 0) {
+        if (load_in) {
+          if (lane == 0) {
             fence_proxy_async_smem();
-            mbar_arrive_expect_tx(rb, kChunkBytes);
-            tma_load_3d(chunk_u, &p.res, (int)j0, (int)i0, 0, rb);
+            mbar_arrive_expect_tx(ib, kChunkBytes);
+            tma_load_3d(chunk_u, aux_in ? &p.aux : &p.res, (int)j0, (int)i0, 0, ib);
           }
-        }
-        if (kAuxStaged && aux_in && lane == 0) {
-          fence_proxy_async_smem();
-          mbar_arrive_expect_tx(ab, kChunkBytes);
-          tma_load_3d(aux_u, &p.aux, (int)j0, (int)i0, 0, ab);
+        } else if (res_staged) {
+          chunk_in<TO, RB>(chunk, (const TO *)g.res, g.ldr, i0, g.m, j0, g.n, lane);
         }
       };
       if (chunks) fetch(jw);
@@ -365,16 +368,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
         if (!ok) break;
         tc_fence_after();
         if constexpr (PL == 3) {
-          if (mine) {
-            const uint32_t t = lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols);
+          if (chunks) {
+            const uint32_t t = lane_base + (uint32_t)(buf * kBufCols + cg * kWarpCols);
 #pragma unroll
-            for (int c = 0; c < kWarpCols; c += 32) {
-              uint32_t a[32], b[32];
-              tmem_ld32(t + c, a);
-              tmem_ld32(t + BN + c, b);
+            for (int c = 0; c < kWarpCols; c += 16) {
+              uint32_t a[16], b[16];
+              tmem_ld16(t + c, a);
+              tmem_ld16(t + BN + c, b);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
+              for (int j = 0; j < 16; ++j) {
                 const float v = __uint_as_float(a[j]) + __uint_as_float(b[j]);
                 facc[c + j] = u ? facc[c + j] + v : v;
               }
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
         }
       }
       if (!ok) break;
-      if (kRowSum && g.row_sum && it.n0 == 0 && h == 0) {
+      if (kRowSum && g.row_sum && it.n0 == 0 && cg == 0) {
         const float v = __uint_as_float(tmem_ld1(lane_base + (uint32_t)(kBufs * kBufCols + 16 * buf)));
         tmem_ld_wait();
         if (row < g.m) {
@@ -394,114 +397,108 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
           else ((TI *)g.row_sum)[row] = ElemOf<TI>::from(v);
         }
       }
+      // the 32 sums of a group of columns, with the bias
+      auto sums = [&](long long j1, int c, float (&v)[32]) {
+        if constexpr (PL == 3) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {   // c is a runtime index: pick without indexing registers by it
+            v[j] = facc[j];
+            if constexpr (kWarpCols > 32) v[j] = c ? facc[32 + j] : v[j];
+          }
+        } else {
+          uint32_t r[32];
+          tmem_ld32(lane_base + (uint32_t)(buf * kBufCols + cg * kWarpCols + c), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        }
+        if (g.bias) add_bias<TO>((const TO *)g.bias, j1, g.n, p.bias16 != 0, v);
+      };
+      static_assert(PL == 1 || kWarpCols <= 64, "two groups");
 #pragma unroll 1
       for (int ch = 0; ch < chunks; ++ch) {
         const long long j0 = jw + ch * CW;
-        const int sw = lane & 7;
-        uint8_t *my = chunk + lane * 128, *my_aux = aux + lane * 128;
         if (ch) fetch(j0);
-        uint32_t acc[PL == 1 ? CW : 1];
-        if constexpr (PL == 1) {
-          const uint32_t t = lane_base + (uint32_t)(buf * kBufCols + h * kWarpCols + ch * CW);
-#pragma unroll
-          for (int c = 0; c < CW; c += 32) tmem_ld32(t + c, *reinterpret_cast<uint32_t(*)[32]>(acc + c));
-        }
-        if (g.res && p.res_tma) {
-          ok = __all_sync(0xffffffffu, g_wait(rb, rph, abort_s, 8, 2 * limit, 0));
-          rph ^= 1u;
-        }
-        if (kAuxStaged && aux_in) {
-          ok = __all_sync(0xffffffffu, g_wait(ab, aph, abort_s, 9, 2 * limit, 0)) && ok;
-          aph ^= 1u;
-        }
-        if constexpr (PL == 1) {
-          tmem_ld_wait();
-          if (ch == chunks - 1) {   // the accumulator is in registers: the next tile may have its place
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+        if (aux_out) {   // the pre-activations leave first, through the same chunk
+#pragma unroll 1
+          for (int c1 = 0; c1 < CW; c1 += 32) {
+            float v[32];
+            sums(j0 + c1, ch * CW + c1, v);
+            stage_store<TO, RB>(chunk, lane, c1 * (int)sizeof(TO) / 16, v);
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&p.aux, chunk_u, (int)j0, (int)i0, 0);
+            bulk_commit();
+            bulk_wait_read();
+          }
+          __syncwarp();
         }
-        if (!ok) break;
-        __syncwarp();
-#pragma unroll
+        if (load_in) {
+          ok = __all_sync(0xffffffffu, g_wait(ib, iph, abort_s, 8, 2 * limit, 0));
+          iph ^= 1u;
+          if (!ok) break;
+        }
+#pragma unroll 1
         for (int c1 = 0; c1 < CW; c1 += 32) {
-          const int q0 = c1 / 8;   // first 16-byte piece (16-bit types; fp32 chunks hold one group of 32)
           const long long j1 = j0 + c1;
+          const int q0 = c1 * (int)sizeof(TO) / 16;
           float v[32];
-          if constexpr (PL == 3) {
-            // ch is a runtime index: pick the group without indexing registers dynamically
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              v[j] = facc[j];
-              if constexpr (kWarpCols > 32) v[j] = ch ? facc[32 + j] : v[j];
+          sums(j1, ch * CW + c1, v);
+          if constexpr (PL == 1) {
+            if (ch == chunks - 1 && c1 == CW - 32) {   // all read: the next tile may have the accumulator
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[c1 + j]);
           }
-          if (g.bias) add_bias<TO>((const TO *)g.bias, j1, g.n, p.bias16 != 0, v);
-          if (g.act != DCN_ACT_NONE) {
+          if (g.act == DCN_ACT_RELU) {
             if (g.saved) {
-              if (g.act == DCN_ACT_RELU) {
-                uint32_t bits = 0;
+              uint32_t bits = 0;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) bits |= relu_bit(v[j]) ? 1u << j : 0u;
-                if (row < g.m && j1 < g.n) ((uint32_t *)g.saved)[row * words + (j1 >> 5)] = bits;
-              } else if constexpr (kAuxStaged) {
-                stage_store<TO>(my_aux, sw, q0, v);
-              } else if (row < g.m) {
-                float4 *zp = reinterpret_cast<float4 *>((float *)g.saved + row * p.ldz + j1);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (j1 + 4 * i < p.ldz) zp[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-              }
+              for (int j = 0; j < 32; ++j) bits |= relu_bit(v[j]) ? 1u << j : 0u;
+              if (row < g.m && j1 < g.n) ((uint32_t *)g.saved)[row * words + (j1 >> 5)] = bits;
             }
-            if (g.act == DCN_ACT_RELU) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = relu_value(v[j]);
-            } else {
+            for (int j = 0; j < 32; ++j) v[j] = relu_value(v[j]);
+          } else if (g.act == DCN_ACT_GELU) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = gelu_value<PL == 3>(v[j]);
-            }
+            for (int j = 0; j < 32; ++j) v[j] = gelu_value<PL == 3>(v[j]);
           }
+          constexpr int E = 16 / (int)sizeof(TO);
           if (g.slope_act == DCN_ACT_RELU) {
             const uint32_t bits = row < g.m && j1 < g.n ? __ldg((const uint32_t *)g.slope + row * words + (j1 >> 5)) : 0u;
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.f;
           } else if (aux_in) {
-            if constexpr (kAuxStaged) {
-              float z[32];
-              stage_load<TO>(my_aux, sw, q0, z);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= gelu_slope<PL == 3>(z[j]);
-            } else if (row < g.m) {
-              const float4 *zp = reinterpret_cast<const float4 *>((const float *)g.slope + row * p.ldz + j1);
+            for (int k = 0; k < 32 / E; ++k) {
+              float z[E];
+              unpack16<TO>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), z);
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (j1 + 4 * i < p.ldz) {
-                  const float4 z = __ldg(zp + i);
-                  v[4 * i] *= gelu_slope<true>(z.x);
-                  v[4 * i + 1] *= gelu_slope<true>(z.y);
-                  v[4 * i + 2] *= gelu_slope<true>(z.z);
-                  v[4 * i + 3] *= gelu_slope<true>(z.w);
-                }
+              for (int j = 0; j < E; ++j) v[E * k + j] *= gelu_slope<PL == 3>(z[j]);
             }
           }
-          if (g.res) {
-            float r[32];
-            stage_load<TO>(my, sw, q0, r);
+          if (res_staged) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += r[j];
+            for (int k = 0; k < 32 / E; ++k) {
+              float r[E];
+              unpack16<TO>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), r);
+#pragma unroll
+              for (int j = 0; j < E; ++j) v[E * k + j] += r[j];
+            }
+          } else if (g.res && row < g.m) {
+            add_row<TO>((const TO *)g.res + row * g.ldr + j1, j1, g.n, v);
           }
-          stage_store<TO>(my, sw, q0, v);
+          stage_store<TO, RB>(chunk, lane, q0, v);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (!p.out_tma) chunk_out<TO>(chunk, (TO *)g.out, g.n, i0, g.m, j0, g.n, lane);
-        if (lane == 0) {
-          if (p.out_tma) tma_store_3d(&p.out, chunk_u, (int)j0, (int)i0, it.split);
-          if (kAuxStaged && aux_out) tma_store_3d(&p.aux, aux_u, (int)j0, (int)i0, 0);
+        if (!p.out_tma) {
+          chunk_out<TO, RB>(chunk, (TO *)g.out, g.n, i0, g.m, j0, g.n, lane);
+        } else if (lane == 0) {
+          tma_store_3d(&p.out, chunk_u, (int)j0, (int)i0, it.split);
           bulk_commit();
         }
         __syncwarp();
@@ -516,7 +513,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == kEpiWarps) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t kFmt = std::is_same_v<TI, __nv_bfloat16> ? 1u : 0u;
     constexpr uint32_t kDesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((AMN ? 1u : 0u) << 15) | ((128u >> 4) << 24);
@@ -617,7 +614,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) dcn_gemm_tc(const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kEpiWarps) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kAlloc);
   }
@@ -807,7 +804,8 @@ EncodeTiledFn encode_fn() {
   return f;
 }
 
-// [depth][rows][inner] with the given row stride (elements), boxes of box_inner x box_rows x 1
+// [depth][rows][inner] with the given row stride (elements), boxes of box_inner (128 or 64 bytes, the
+// swizzle's width) x box_rows x 1
 bool encode3(CUtensorMap *map, CUtensorMapDataType type, int esize, const void *base, long long inner, long long rows,
              long long depth, long long ld, unsigned box_inner, unsigned box_rows) {
   EncodeTiledFn enc = encode_fn();
@@ -816,7 +814,8 @@ bool encode3(CUtensorMap *map, CUtensorMapDataType type, int esize, const void *
   const cuuint64_t strides[2] = {(cuuint64_t)(ld * esize), (cuuint64_t)(rows * ld * esize)};
   const cuuint32_t box[3] = {box_inner, box_rows, 1}, estr[3] = {1, 1, 1};
   return enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             box_inner * (unsigned)esize == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -835,13 +834,13 @@ cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
     done_mask.fetch_or(bit, std::memory_order_release);
   }
   constexpr size_t stage = (size_t)PL * (16384 + BN * 128);
-  const size_t fixed = 1024 + 1024 + (size_t)kEpiWarps * p.nbuf * kChunkBytes + (AMN && PL == 1 ? 2048 : 0);
-  int stages = (int)((kMost - fixed) / stage);
-  if (stages > 8) stages = 8;
+  constexpr size_t fixed = 1024 + 1024 + (size_t)kEpi<PL> * 32 * kChunkRow<TO, BN> + (AMN && PL == 1 ? 2048 : 0);
+  constexpr int stages = (kMost - fixed) / stage > 8 ? 8 : (int)((kMost - fixed) / stage);
+  static_assert(stages >= 2, "a ring");
   p.stages = stages;
   const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
   const int grid = (int)(items < 148 ? items : 148);
-  return launch_pdl(kern, grid, kGemmThreads, fixed + stages * stage, s, p);
+  return launch_pdl(kern, grid, kThreadsOf<PL>, fixed + stages * stage, s, p);
 }
 
 template <typename TI, typename TO, int PL, bool AMN, bool BMN>
@@ -919,8 +918,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   ok = ok && (g.b_mn ? encode3(&p.b, t16, 2, g.b, g.n, g.kk, planes, g.ldb, 64, 64)
                      : encode3(&p.b, t16, 2, g.b, g.kk, g.n, planes, g.ldb, 64, plan.bn));
   const bool rows16 = g.n * esize % 16 == 0;
-  const unsigned cw = (unsigned)(128 / esize);
-  p.nbuf = 1;
+  const unsigned cw = esize == 4 || plan.bn < 256 ? 32 : 64;   // kChunkRow
   if (parts) {
     p.out_tma = 1;
     ok = ok && encode3(&p.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, g.n, g.m, plan.splits, plan.ldp, 32, 32);
@@ -934,8 +932,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   }
   const void *aux = g.slope_act == DCN_ACT_GELU ? g.slope : g.act == DCN_ACT_GELU ? g.saved : nullptr;
   p.ldz = (g.n + 7) / 8 * 8;
-  if (aux && planes == 1) {
-    p.nbuf = 2;
+  if (aux) {
     ok = ok && encode3(&p.aux, tio, esize, aux, p.ldz, g.m, 1, p.ldz, cw, 32);
   }
   if (!ok) return cudaErrorInvalidValue;
