@@ -8,6 +8,7 @@ namespace dcn {
 // How a product is cut up; depends on sizes and type only, so that the workspace query and the call agree.
 struct GemmPlan {
   int bn;          // columns of an output tile
+  int cg;          // blocks that share a tile: 1 (128 rows) or a cluster of 2 (256 rows)
   int splits;      // ranges of k, each with fp32 parts of its own
   int kb_total, kb_split;   // 64-value blocks of k, in all and in a range
   long long ldp;   // row stride of the fp32 parts, elements

@@ -5,6 +5,12 @@
 // output index contiguous.  Tensor maps and tcgen05 descriptors take either order, so nothing is
 // transposed in memory.
 //
+// Where there are enough tiles, two blocks of a cluster work on one tile of 256 rows (CG = 2): each loads
+// its own 128 rows of A and half of the rows of B, and one tcgen05.mma.cta_group::2 multiplies what
+// lies in both.  A step of a 256-column tile then brings 32 KB into an SM instead of 48: what bounds
+// the products with few steps or few output columns is the rate at which tiles come in (about 35
+// bytes a cycle and SM measured, from L2 or memory).
+//
 // One persistent block per SM: a loader lane fills a ring of stages (64 values of k of a 128-row A
 // tile and a BN-row B tile, 128-byte swizzle) with cp.async.bulk.tensor; one warp issues tcgen05.mma
 // into fp32 accumulators in tensor memory, double-buffered so that the epilogue of a tile runs under
@@ -84,13 +90,86 @@ __device__ __forceinline__ bool g_wait(uint32_t bar, uint32_t parity, volatile i
   }
 }
 
+// CG = 2: the barrier may be the other block's of the pair.
+template <int CG = 1>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2,
                                             uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+// One block (CG = 1) or the pair of blocks of a cluster (CG = 2) that works on one accumulator.
+template <int CG>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1) {
+    umma_bf16(d, a, b, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// Arrives on `bar` (of both blocks) when the products issued so far have been computed.
+template <int CG>
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    umma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (CG == 1)
+    tmem_dealloc(taddr, cols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pair_sync() {
+  if constexpr (CG == 2) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+// The address of the first block's copy of a shared variable, and an arrival there.
+template <int CG>
+__device__ __forceinline__ uint32_t lead_addr(uint32_t addr) {
+  if constexpr (CG == 1) return addr;
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+template <int CG>
+__device__ __forceinline__ void lead_arrive(uint32_t addr) {
+  if constexpr (CG == 1)
+    mbar_arrive(addr);
+  else
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
@@ -132,13 +211,14 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
 struct Item {
   int m0, n0, split, kb0, kb1;
 };
-__device__ __forceinline__ Item decode(uint32_t item, const GemmTc &p, int BN) {
+// rank: which block of its pair this one is; a pair's tile is 256 rows
+__device__ __forceinline__ Item decode(uint32_t item, const GemmTc &p, int BN, int CG, int rank) {
   const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
   Item it;
   it.split = (int)(item / tiles);
   const uint32_t t = item - (uint32_t)it.split * tiles;
   const uint32_t tm = t / (uint32_t)p.tiles_n;   // column tiles of one row tile are neighbours: A stays in L2
-  it.m0 = (int)tm * 128;
+  it.m0 = ((int)tm * CG + rank) * 128;
   it.n0 = (int)(t - tm * (uint32_t)p.tiles_n) * BN;
   it.kb0 = it.split * p.kb_split;
   it.kb1 = min(p.kb_total, it.kb0 + p.kb_split);
@@ -264,17 +344,18 @@ __device__ __forceinline__ void add_row(const TO *src, long long j1, long long n
 }  // namespace
 
 // PL planes per operand; TI the 16-bit type of the planes, TO the output's (and residual's) type;
-// AMN / BMN: the operand lies with its row index contiguous.
-template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN>
+// AMN / BMN: the operand lies with its row index contiguous; CG blocks to a tile.
+template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN, int CG>
 __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_constant__ GemmTc p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t kABytes = PL * 16384u, kBBytes = PL * BN * 128u, kStage = kABytes + kBBytes;
+  constexpr uint32_t kABytes = PL * 16384u, kBBytes = PL * (BN / CG) * 128u, kStage = kABytes + kBBytes;
   constexpr int kEpiWarps = kEpi<PL>, kGemmThreads = kThreadsOf<PL>, kGroups = kEpiWarps / 4;
   constexpr bool kRowSum = AMN && PL == 1;             // only the weight gradient asks for row sums
   constexpr int kBufs = (kRowSum && BN == 256) ? 1 : 2;   // accumulator buffers that fit beside the row sums
+  constexpr int kOnes = 16 * CG;   // columns of the product with the tile of ones
   constexpr int kBufCols = PL == 3 ? 2 * BN : BN;
-  constexpr int kCols = kBufs * kBufCols + (kRowSum ? 16 * kBufs : 0);
+  constexpr int kCols = kBufs * kBufCols + (kRowSum ? kOnes * kBufs : 0);
   constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512, "tensor memory");
   constexpr int RB = kChunkRow<TO, BN>, kChunkBytes = 32 * RB;
@@ -301,28 +382,31 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tmem_full + 8 * i, 1);
-      mbar_init(tmem_empty + 8 * i, kEpiWarps);
+      mbar_init(tmem_empty + 8 * i, CG * kEpiWarps);
     }
     for (int i = 0; i < kEpiWarps; ++i) mbar_init(in_bar + 8 * i, 1);
     *abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (kRowSum && g.row_sum) {
-    // 16 rows x 64 values, all one: the same in every layout
+    // 16 rows (of each block) x 64 values, all one: the same in every layout
     for (int i = threadIdx.x; i < 1024; i += kGemmThreads) ((TI *)ones)[i] = ElemOf<TI>::from(1.f);
     fence_proxy_async_smem();
   }
   if (warp == kEpiWarps) {
-    tmem_alloc(smem_u32(tmem_slot), kAlloc);
-    tmem_relinquish();
+    pair_tmem_alloc<CG>(smem_u32(tmem_slot), kAlloc);
   }
   tc_fence_before();
   __syncthreads();
+  pair_sync<CG>();
   tc_fence_after();
   pdl_wait();
   pdl_launch();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t items = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
+  const int rank = CG == 1 ? 0 : (int)(blockIdx.x & 1);   // a cluster is two neighbouring blocks
+  const uint32_t first_item = blockIdx.x / CG, item_step = gridDim.x / CG;
+  const uint32_t lead_empty = lead_addr<CG>(tmem_empty), lead_full = lead_addr<CG>(full);
 
   if (warp < kEpiWarps) {
     // ------------------------------ epilogue ------------------------------
@@ -336,8 +420,8 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
     const bool res_staged = g.res && !aux_in && !aux_out;
     const bool load_in = aux_in || (res_staged && p.res_tma);
     bool ok = true;
-    for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item it = decode(item, p, BN);
+    for (uint32_t item = first_item; item < items && ok; item += item_step) {
+      const Item it = decode(item, p, BN, CG, rank);
       const long long i0 = it.m0 + q * 32, row = i0 + lane;
       const long long jw = it.n0 + cg * kWarpCols;   // this warp's first column
       const int chunks =
@@ -385,12 +469,12 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+          if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
         }
       }
       if (!ok) break;
       if (kRowSum && g.row_sum && it.n0 == 0 && cg == 0) {
-        const float v = __uint_as_float(tmem_ld1(lane_base + (uint32_t)(kBufs * kBufCols + 16 * buf)));
+        const float v = __uint_as_float(tmem_ld1(lane_base + (uint32_t)(kBufs * kBufCols + kOnes * buf)));
         tmem_ld_wait();
         if (row < g.m) {
           if (p.splits > 1) p.row_part[(long long)it.split * g.m + row] = v;
@@ -450,7 +534,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
             if (ch == chunks - 1 && c1 == CW - 32) {   // all read: the next tile may have the accumulator
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+              if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
             }
           }
           if (g.act == DCN_ACT_RELU) {
@@ -507,7 +591,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
         if (!chunks) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tmem_empty + 8 * buf);
+          if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
         }
       }
     }
@@ -516,15 +600,15 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   } else if (warp == kEpiWarps) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t kFmt = std::is_same_v<TI, __nv_bfloat16> ? 1u : 0u;
-    constexpr uint32_t kDesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((AMN ? 1u : 0u) << 15) | ((128u >> 4) << 24);
+    constexpr uint32_t kDesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((AMN ? 1u : 0u) << 15) | ((128u * CG >> 4) << 24);
     constexpr uint32_t idesc = kDesc | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17);
-    constexpr uint32_t idesc_ones = kDesc | ((16u >> 3) << 17);
+    constexpr uint32_t idesc_ones = kDesc | (((uint32_t)kOnes >> 3) << 17);
     constexpr uint32_t kAStep = AMN ? 2048 >> 4 : 32 >> 4, kBStep = BMN ? 2048 >> 4 : 32 >> 4;
     const uint64_t ones_desc = smem_desc_sw128(smem_u32(ones));
     uint32_t st = 0, ph = 0, unit = 0;
-    bool ok = true;
-    for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item it = decode(item, p, BN);
+    bool ok = rank == 0;   // the first block of a pair issues for both
+    for (uint32_t item = first_item; item < items && ok; item += item_step) {
+      const Item it = decode(item, p, BN, CG, rank);
       const bool sums = kRowSum && g.row_sum && it.n0 == 0;
       uint32_t d = 0;
       int buf = 0;
@@ -548,25 +632,25 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
 #pragma unroll
           for (int i = 0; i < PL; ++i) {
             ad[i] = AMN ? smem_desc_mn(sa + i * 16384u) : smem_desc_sw128(sa + i * 16384u);
-            bd[i] = BMN ? smem_desc_mn(sb + i * BN * 128u) : smem_desc_sw128(sb + i * BN * 128u);
+            bd[i] = BMN ? smem_desc_mn(sb + i * (BN / CG) * 128u) : smem_desc_sw128(sb + i * (BN / CG) * 128u);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint64_t ka = (uint64_t)(k * kAStep), kb_ = (uint64_t)(k * kBStep);
             const uint32_t more = !first || k ? 1u : 0u;
-            umma_bf16(d, ad[0] + ka, bd[0] + kb_, idesc, more);
+            pair_mma<CG>(d, ad[0] + ka, bd[0] + kb_, idesc, more);
             if constexpr (PL == 3) {
-              umma_bf16(d + BN, ad[0] + ka, bd[2] + kb_, idesc, more);
-              umma_bf16(d + BN, ad[2] + ka, bd[0] + kb_, idesc, 1u);
-              umma_bf16(d + BN, ad[1] + ka, bd[1] + kb_, idesc, 1u);
-              umma_bf16(d + BN, ad[0] + ka, bd[1] + kb_, idesc, 1u);
-              umma_bf16(d + BN, ad[1] + ka, bd[0] + kb_, idesc, 1u);
+              pair_mma<CG>(d + BN, ad[0] + ka, bd[2] + kb_, idesc, more);
+              pair_mma<CG>(d + BN, ad[2] + ka, bd[0] + kb_, idesc, 1u);
+              pair_mma<CG>(d + BN, ad[1] + ka, bd[1] + kb_, idesc, 1u);
+              pair_mma<CG>(d + BN, ad[0] + ka, bd[1] + kb_, idesc, 1u);
+              pair_mma<CG>(d + BN, ad[1] + ka, bd[0] + kb_, idesc, 1u);
             }
             if (kRowSum && sums)
-              umma_bf16(tmem_base + (uint32_t)(kBufs * kBufCols + 16 * buf), ad[0] + ka, ones_desc, idesc_ones, more);
+              pair_mma<CG>(tmem_base + (uint32_t)(kBufs * kBufCols + kOnes * buf), ad[0] + ka, ones_desc, idesc_ones, more);
           }
-          umma_commit(empty + 8 * st);
-          if (last) umma_commit(tmem_full + 8 * buf);
+          pair_commit<CG>(empty + 8 * st);
+          if (last) pair_commit<CG>(tmem_full + 8 * buf);
         }
         __syncwarp();
         if (++st == (uint32_t)ST) { st = 0; ph ^= 1u; }
@@ -578,28 +662,30 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
     if (lane == 0) {
       uint32_t st = 0, ph = 0;
       bool ok = true;
-      for (uint32_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        const Item it = decode(item, p, BN);
+      for (uint32_t item = first_item; item < items && ok; item += item_step) {
+        const Item it = decode(item, p, BN, CG, rank);
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           ok = g_wait(empty + 8 * st, ph ^ 1u, abort_s, 7, 2 * limit, 32);
           if (!ok) break;
-          const uint32_t bar = full + 8 * st, sa = smem_u32(ring) + st * kStage, sb = sa + kABytes;
-          mbar_arrive_expect_tx(bar, kStage);
-          const int k0 = kb * 64;
+          // a pair's loads all count on the first block's barrier
+          const uint32_t bar = lead_full + 8 * st, sa = smem_u32(ring) + st * kStage, sb = sa + kABytes;
+          if (rank == 0) mbar_arrive_expect_tx(full + 8 * st, CG * kStage);
+          const int k0 = kb * 64, nb = it.n0 + rank * (BN / CG);
 #pragma unroll
           for (int i = 0; i < PL; ++i) {
             if constexpr (AMN) {
 #pragma unroll
-              for (int j = 0; j < 2; ++j) tma_load_3d(sa + i * 16384u + j * 8192u, &p.a, it.m0 + 64 * j, k0, i, bar);
+              for (int j = 0; j < 2; ++j)
+                tma_load_3d<CG>(sa + i * 16384u + j * 8192u, &p.a, it.m0 + 64 * j, k0, i, bar);
             } else {
-              tma_load_3d(sa + i * 16384u, &p.a, k0, it.m0, i, bar);
+              tma_load_3d<CG>(sa + i * 16384u, &p.a, k0, it.m0, i, bar);
             }
             if constexpr (BMN) {
 #pragma unroll
-              for (int j = 0; j < BN / 64; ++j)
-                tma_load_3d(sb + i * BN * 128u + j * 8192u, &p.b, it.n0 + 64 * j, k0, i, bar);
+              for (int j = 0; j < BN / CG / 64; ++j)
+                tma_load_3d<CG>(sb + i * (BN / CG) * 128u + j * 8192u, &p.b, nb + 64 * j, k0, i, bar);
             } else {
-              tma_load_3d(sb + i * BN * 128u, &p.b, k0, it.n0, i, bar);
+              tma_load_3d<CG>(sb + i * (BN / CG) * 128u, &p.b, k0, nb, i, bar);
             }
           }
           if (++st == (uint32_t)ST) { st = 0; ph ^= 1u; }
@@ -614,9 +700,10 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
+  pair_sync<CG>();   // no block leaves while the other may still reach into it
   if (warp == kEpiWarps) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, kAlloc);
+    pair_tmem_dealloc<CG>(tmem_base, kAlloc);
   }
 }
 
@@ -819,9 +906,9 @@ bool encode3(CUtensorMap *map, CUtensorMapDataType type, int esize, const void *
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN>
+template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN, int CG>
 cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
-  auto kern = dcn_gemm_tc<TI, TO, PL, BN, AMN, BMN>;
+  auto kern = dcn_gemm_tc<TI, TO, PL, BN, AMN, BMN, CG>;
   static std::atomic<unsigned long long> done_mask{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -833,37 +920,41 @@ cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     done_mask.fetch_or(bit, std::memory_order_release);
   }
-  constexpr size_t stage = (size_t)PL * (16384 + BN * 128);
+  constexpr size_t stage = (size_t)PL * (16384 + BN / CG * 128);
   constexpr size_t fixed = 1024 + 1024 + (size_t)kEpi<PL> * 32 * kChunkRow<TO, BN> + (AMN && PL == 1 ? 2048 : 0);
   constexpr int stages = (kMost - fixed) / stage > 8 ? 8 : (int)((kMost - fixed) / stage);
   static_assert(stages >= 2, "a ring");
   p.stages = stages;
   const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
-  const int grid = (int)(items < 148 ? items : 148);
-  return launch_pdl(kern, grid, kThreadsOf<PL>, fixed + stages * stage, s, p);
+  const int grid = CG * (int)(items < 148 / CG ? items : 148 / CG);
+  return launch_pdl(kern, grid, kThreadsOf<PL>, fixed + stages * stage, s, CG, p);
 }
 
 template <typename TI, typename TO, int PL, bool AMN, bool BMN>
-cudaError_t run_bn(GemmTc &p, int bn, cudaStream_t s) {
-  if constexpr (PL == 1)
-    if (bn == 256) return run_tc<TI, TO, PL, 256, AMN, BMN>(p, s);
-  if (bn == 128) return run_tc<TI, TO, PL, 128, AMN, BMN>(p, s);
-  return run_tc<TI, TO, PL, 64, AMN, BMN>(p, s);
+cudaError_t run_bn(GemmTc &p, int bn, int cg, cudaStream_t s) {
+  if constexpr (PL == 1) {
+    if (cg == 2) return run_tc<TI, TO, PL, 256, AMN, BMN, 2>(p, s);
+    if (bn == 256) return run_tc<TI, TO, PL, 256, AMN, BMN, 1>(p, s);
+  } else {
+    if (cg == 2) return run_tc<TI, TO, PL, 128, AMN, BMN, 2>(p, s);
+  }
+  if (bn == 128) return run_tc<TI, TO, PL, 128, AMN, BMN, 1>(p, s);
+  return run_tc<TI, TO, PL, 64, AMN, BMN, 1>(p, s);
 }
 
 template <typename TI, typename T, int PL>
-cudaError_t run_order(GemmTc &p, int bn, bool parts, cudaStream_t s) {
+cudaError_t run_order(GemmTc &p, int bn, int cg, bool parts, cudaStream_t s) {
   const GemmArgs &g = p.g;
-  if (!g.a_mn && !g.b_mn) return run_bn<TI, T, PL, false, false>(p, bn, s);
-  if (!g.a_mn) return run_bn<TI, T, PL, false, true>(p, bn, s);
-  if (parts) return run_bn<TI, float, PL, true, true>(p, bn, s);
-  return run_bn<TI, T, PL, true, true>(p, bn, s);
+  if (!g.a_mn && !g.b_mn) return run_bn<TI, T, PL, false, false>(p, bn, cg, s);
+  if (!g.a_mn) return run_bn<TI, T, PL, false, true>(p, bn, cg, s);
+  if (parts) return run_bn<TI, float, PL, true, true>(p, bn, cg, s);
+  return run_bn<TI, T, PL, true, true>(p, bn, cg, s);
 }
 
 template <typename T>
 cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &g, cudaStream_t s) {
   const long long n = g.m * (plan.ldp / 4);
-  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + 255) / 256), 256, 0, s, part, plan.splits, g.m, g.n, plan.ldp,
+  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + 255) / 256), 256, 0, s, 1, part, plan.splits, g.m, g.n, plan.ldp,
                     (T *)g.out);
 }
 
@@ -873,19 +964,26 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weight_gradient) {
   GemmPlan p = {};
-  const long long tm = (m + 127) / 128;
-  auto tiles = [&](int bn) { return tm * ((n + bn - 1) / bn); };
+  const int wide = planes == 1 ? 256 : 128;
+  auto tiles = [&](int rows, int bn) { return (m + rows - 1) / rows * ((n + bn - 1) / bn); };
   p.kb_total = (int)((k + 63) / 64);
   p.splits = 1;
+  p.cg = 1;
   if (weight_gradient) {
-    p.bn = planes == 1 && n > 128 ? 256 : n > 64 ? 128 : 64;
-    long long splits = 148 / tiles(p.bn);
+    p.bn = n > wide / 2 ? wide : n > 64 ? 128 : 64;
+    if (m > 128 && p.bn == wide) p.cg = 2;
+    long long splits = 148 / p.cg / tiles(128 * p.cg, p.bn);
     if (splits > p.kb_total / 4) splits = p.kb_total / 4;
     if (splits < 1) splits = 1;
     p.kb_split = (int)((p.kb_total + splits - 1) / splits);
     p.splits = (p.kb_total + p.kb_split - 1) / p.kb_split;
   } else {
-    p.bn = planes == 1 && n > 128 && tiles(256) >= 148 ? 256 : n > 64 && tiles(128) >= 148 ? 128 : 64;
+    if (n > wide / 2 && tiles(256, wide) >= 74) {
+      p.bn = wide;
+      p.cg = 2;
+    } else {
+      p.bn = n > wide / 2 && tiles(128, wide) >= 148 ? wide : n > 64 && tiles(128, 128) >= 148 ? 128 : 64;
+    }
     p.kb_split = p.kb_total;
   }
   p.ldp = (n + 3) / 4 * 4;
@@ -905,7 +1003,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   const bool parts = plan.splits > 1;
   const CUtensorMapDataType t16 = dtype == DCN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapDataType tio = dtype == DCN_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : t16;
-  p.tiles_m = (int)((g.m + 127) / 128);
+  p.tiles_m = (int)((g.m + 128 * plan.cg - 1) / (128 * plan.cg));
   p.tiles_n = (int)((g.n + plan.bn - 1) / plan.bn);
   p.splits = plan.splits;
   p.kb_total = plan.kb_total;
@@ -916,7 +1014,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   bool ok = g.a_mn ? encode3(&p.a, t16, 2, g.a, g.m, g.kk, planes, g.lda, 64, 64)
                    : encode3(&p.a, t16, 2, g.a, g.kk, g.m, planes, g.lda, 64, 128);
   ok = ok && (g.b_mn ? encode3(&p.b, t16, 2, g.b, g.n, g.kk, planes, g.ldb, 64, 64)
-                     : encode3(&p.b, t16, 2, g.b, g.kk, g.n, planes, g.ldb, 64, plan.bn));
+                     : encode3(&p.b, t16, 2, g.b, g.kk, g.n, planes, g.ldb, 64, plan.bn / plan.cg));
   const bool rows16 = g.n * esize % 16 == 0;
   const unsigned cw = esize == 4 || plan.bn < 256 ? 32 : 64;   // kChunkRow
   if (parts) {
@@ -937,9 +1035,9 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   }
   if (!ok) return cudaErrorInvalidValue;
   cudaError_t e;
-  if (dtype == DCN_DTYPE_F32) e = run_order<__nv_bfloat16, float, 3>(p, plan.bn, parts, s);
-  else if (dtype == DCN_DTYPE_BF16) e = run_order<__nv_bfloat16, __nv_bfloat16, 1>(p, plan.bn, parts, s);
-  else e = run_order<__half, __half, 1>(p, plan.bn, parts, s);
+  if (dtype == DCN_DTYPE_F32) e = run_order<__nv_bfloat16, float, 3>(p, plan.bn, plan.cg, parts, s);
+  else if (dtype == DCN_DTYPE_BF16) e = run_order<__nv_bfloat16, __nv_bfloat16, 1>(p, plan.bn, plan.cg, parts, s);
+  else e = run_order<__half, __half, 1>(p, plan.bn, plan.cg, parts, s);
   if (e != cudaSuccess || !parts) return e;
   if (dtype == DCN_DTYPE_F32) e = run_reduce<float>(part, plan, g, s);
   else if (dtype == DCN_DTYPE_BF16) e = run_reduce<__nv_bfloat16>(part, plan, g, s);
@@ -966,17 +1064,17 @@ cudaError_t launch_gemm_stage(const void *src, long long ld, const void *saved, 
   stage_shape(rows, pitch, &tx, &ty, &gx, &gy);
   if (slabs) *slabs = gy;
   const dim3 grid(gx, gy), block(tx, ty);
-  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_gemm_stage<float, 3>, grid, block, 0, s, a);
-  if (dtype == DCN_DTYPE_BF16) return launch_pdl(dcn_gemm_stage<__nv_bfloat16, 1>, grid, block, 0, s, a);
-  return launch_pdl(dcn_gemm_stage<__half, 1>, grid, block, 0, s, a);
+  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_gemm_stage<float, 3>, grid, block, 0, s, 1, a);
+  if (dtype == DCN_DTYPE_BF16) return launch_pdl(dcn_gemm_stage<__nv_bfloat16, 1>, grid, block, 0, s, 1, a);
+  return launch_pdl(dcn_gemm_stage<__half, 1>, grid, block, 0, s, 1, a);
 }
 
 cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s) {
   const unsigned grid = (unsigned)((cols + 31) / 32);
-  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_column_reduce<float>, grid, 1024, 0, s, part, parts, cols, (float *)out);
+  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_column_reduce<float>, grid, 1024, 0, s, 1, part, parts, cols, (float *)out);
   if (dtype == DCN_DTYPE_BF16)
-    return launch_pdl(dcn_column_reduce<__nv_bfloat16>, grid, 1024, 0, s, part, parts, cols, (__nv_bfloat16 *)out);
-  return launch_pdl(dcn_column_reduce<__half>, grid, 1024, 0, s, part, parts, cols, (__half *)out);
+    return launch_pdl(dcn_column_reduce<__nv_bfloat16>, grid, 1024, 0, s, 1, part, parts, cols, (__nv_bfloat16 *)out);
+  return launch_pdl(dcn_column_reduce<__half>, grid, 1024, 0, s, 1, part, parts, cols, (__half *)out);
 }
 
 // Reads and clears the status word of the current device, after the work on `s`.

@@ -374,9 +374,9 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
 
 template <typename T, int V, int E, int G>
 cudaError_t run_one(const NormArgs &a, bool backward, bool params, int grid, cudaStream_t s) {
-  if (!backward) return launch_pdl(norm_forward<T, V, E, G>, grid, kThreads, 0, s, a);
-  if (params) return launch_pdl(norm_backward<T, V, E, G, true>, grid, kThreads, 0, s, a);
-  return launch_pdl(norm_backward<T, V, E, G, false>, grid, kThreads, 0, s, a);
+  if (!backward) return launch_pdl(norm_forward<T, V, E, G>, grid, kThreads, 0, s, 1, a);
+  if (params) return launch_pdl(norm_backward<T, V, E, G, true>, grid, kThreads, 0, s, 1, a);
+  return launch_pdl(norm_backward<T, V, E, G, false>, grid, kThreads, 0, s, 1, a);
 }
 
 // E: the fewest elements to a thread that hold the row; G: a warp while that is at most 32.
@@ -400,12 +400,12 @@ cudaError_t run_rows(const NormArgs &a, bool backward, bool params, int *parts, 
 template <typename T>
 cudaError_t run(const NormArgs &a, bool backward, bool params, int *parts, cudaStream_t s) {
   if (a.cols > 8192) {
-    if (!backward) return launch_pdl(norm_forward_wide<T>, (unsigned)a.rows, 1024, 0, s, a);
+    if (!backward) return launch_pdl(norm_forward_wide<T>, (unsigned)a.rows, 1024, 0, s, 1, a);
     cudaError_t e = cudaSuccess;
-    if (a.y) e = launch_pdl(norm_backward_wide<T>, (unsigned)a.rows, 1024, 0, s, a);
+    if (a.y) e = launch_pdl(norm_backward_wide<T>, (unsigned)a.rows, 1024, 0, s, 1, a);
     if (e == cudaSuccess && params) {
       *parts = (int)(a.rows < 64 ? a.rows : 64);
-      e = launch_pdl(norm_columns_wide<T>, dim3((a.cols + kThreads - 1) / kThreads, *parts), kThreads, 0, s, a);
+      e = launch_pdl(norm_columns_wide<T>, dim3((a.cols + kThreads - 1) / kThreads, *parts), kThreads, 0, s, 1, a);
     }
     return e;
   }
@@ -502,12 +502,12 @@ int dcn_layer_norm_backward(const void *gy, int64_t ldgy, const void *x, int64_t
   if (e == cudaSuccess && params) {
     const dim3 grid((unsigned)((cols + 31) / 32), 2);
     if (wdtype == DCN_DTYPE_F32)
-      e = launch_pdl(norm_reduce<float>, grid, 1024, 0, s, a.part, parts, a.cols, (float *)gw, (float *)gb);
+      e = launch_pdl(norm_reduce<float>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (float *)gw, (float *)gb);
     else if (wdtype == DCN_DTYPE_BF16)
-      e = launch_pdl(norm_reduce<__nv_bfloat16>, grid, 1024, 0, s, a.part, parts, a.cols, (__nv_bfloat16 *)gw,
+      e = launch_pdl(norm_reduce<__nv_bfloat16>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (__nv_bfloat16 *)gw,
                      (__nv_bfloat16 *)gb);
     else
-      e = launch_pdl(norm_reduce<__half>, grid, 1024, 0, s, a.part, parts, a.cols, (__half *)gw, (__half *)gb);
+      e = launch_pdl(norm_reduce<__half>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (__half *)gw, (__half *)gb);
   }
   return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -99,7 +99,8 @@ def test_backward_as_the_first_work_of_the_process():
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_linear_many_rows_and_splits(dtype):
     """Enough rows that the weight gradient's sum is divided among blocks."""
-    for rows, cin, cout, act in [(20011, 64, 72, 'gelu'), (6000, 256, 264, 'relu'), (3000, 130, 33, None)]:
+    for rows, cin, cout, act in [(20011, 64, 72, 'gelu'), (6000, 256, 264, 'relu'), (3000, 130, 33, None),
+                                 (19000, 136, 264, 'gelu'), (9600, 264, 520, 'relu'), (9500, 257, 300, None)]:
         x, w, b, r, gy = linear_case(rows, cin, cout, dtype, act)
         got = run_linear(x, w, b, r, gy, act)
         hold(got, plain.linear(x, w, b, r, act, gy))
