@@ -1,6 +1,8 @@
 // Interface between the linear layer's C entries and the tensor-core product.
 #pragma once
 
+#include <cuda.h>
+
 #include "dcn_layers.cuh"
 
 namespace dcn {
@@ -15,6 +17,29 @@ struct GemmPlan {
   size_t part_bytes, row_part_bytes;   // 0 without splits
 };
 GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weight_gradient);
+
+// One launch of the tensor-core kernel.
+struct alignas(64) GemmTc {
+  CUtensorMap a, b, out, res, aux;
+  GemmArgs g;
+  int m, n;                        // of g
+  int tiles_m, tiles_n, splits, kb_total, kb_split;
+  int step_n, step_m, step_s;      // a block's stride through the items, in column tiles, row tiles and ranges
+  int stages;
+  int out_tma, res_tma;            // 0: element by element
+  int bias16;                      // the bias starts on 16 bytes
+  long long ldz;                   // row stride of kept pre-activations: a multiple of 8
+  float *row_part;                 // [splits][m], with splits > 1
+  unsigned long long wait_limit_ns;
+};
+
+// One tensor type each (dcn_gemm_tc.cuh).
+cudaError_t run_gemm_bf16(GemmTc &p, int bn, int cg, bool parts, cudaStream_t s);
+cudaError_t run_gemm_f16(GemmTc &p, int bn, int cg, bool parts, cudaStream_t s);
+cudaError_t run_gemm_f32(GemmTc &p, int bn, int cg, bool parts, cudaStream_t s);
+cudaError_t read_gemm_status_bf16(cudaStream_t s, int *status);
+cudaError_t read_gemm_status_f16(cudaStream_t s, int *status);
+cudaError_t read_gemm_status_f32(cudaStream_t s, int *status);
 
 // g.a / g.b point at 16-bit planes [planes][rows][ld] whose rows start on 16 bytes; g.out, g.res, g.saved
 // and g.slope have the tensors' own `dtype`.  part / row_part: the plan's scratch.
