@@ -392,7 +392,8 @@ int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t l
                        int64_t rows, int64_t cin, int64_t cout, int32_t device, void *workspace,
                        size_t workspace_bytes, void *stream);
 int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t cout,
-                                        int64_t alignment, int32_t want_gx, int32_t want_gw, size_t *bytes);
+                                        int64_t alignment, int32_t want_gx, int32_t want_gw, int32_t want_gb,
+                                        size_t *bytes);
 int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
                         int64_t ldw, const void *saved, const void *in_saved, const void *gx_add, void *gx,
                         void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,

@@ -235,7 +235,10 @@ GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weigh
     p.kb_split = (int)((p.kb_total + splits - 1) / splits);
     p.splits = (p.kb_total + p.kb_split - 1) / p.kb_split;
   } else {
-    if (n > wide / 2 && tiles(256, wide) >= 74) {
+    // pairs halve the loads of B but tie two epilogues together: with few steps to a tile the epilogues are
+    // what counts (35642 x 256 x 1024 bf16: 27.8 us alone, 31.5 us in pairs; 35642 x 1024 x 256: 24.2 and
+    // 21.3 us; 8192 x 4096 x 4096: 239 and 173 us)
+    if (n > wide / 2 && tiles(256, wide) >= 74 && (planes == 3 || p.kb_total > 6)) {
       p.bn = wide;
       p.cg = 2;
     } else {

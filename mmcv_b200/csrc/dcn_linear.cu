@@ -44,10 +44,10 @@ Layout forward_layout(int dtype, long long rows, long long cin, long long cout, 
 }
 
 Layout backward_layout(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment,
-                       bool want_gx, bool want_gw) {
+                       bool want_gx, bool want_gw, bool want_gb) {
   Layout l;
   const bool stage = needs_stage(dtype, alignment);
-  l.stage_gz = stage || act != DCN_ACT_NONE || !want_gw;   // the last: column sums come from that pass
+  l.stage_gz = stage || act != DCN_ACT_NONE || (want_gb && !want_gw);   // the last: for its column sums
   l.stage_x = stage && want_gw;
   l.stage_w = stage && want_gx;
   if (l.stage_gz) l.gz = take(&l, plane_bytes(dtype, rows, cout));
@@ -137,11 +137,12 @@ int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t l
 }
 
 int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t cout,
-                                        int64_t alignment, int32_t want_gx, int32_t want_gw, size_t *bytes) {
+                                        int64_t alignment, int32_t want_gx, int32_t want_gw, int32_t want_gb,
+                                        size_t *bytes) {
   if (!bytes) return set_error(DCN_ERR_ARG, "linear: bytes is NULL");
   int rc = check_sizes(dtype, act, rows, cin, cout);
   if (rc) return rc;
-  *bytes = rows ? backward_layout(dtype, act, rows, cin, cout, alignment, want_gx != 0, want_gw != 0).bytes : 0;
+  *bytes = rows ? backward_layout(dtype, act, rows, cin, cout, alignment, want_gx != 0, want_gw != 0, want_gb != 0).bytes : 0;
   return DCN_OK;
 }
 
@@ -174,7 +175,7 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
   if (rows == 1) { ldgy = pitch_of(cout); ldx = pitch_of(cin); }   // a single row has no stride
   const int64_t alignment = (int64_t)(uintptr_t)gy | (gw ? (int64_t)(uintptr_t)x | ldx * es : 0) |
                             (gx ? (int64_t)(uintptr_t)weight | ldw * es : 0) | ldgy * es;
-  const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr);
+  const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr, gb != nullptr);
   if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
     return set_error(DCN_ERR_WORKSPACE, "linear backward: workspace missing, too small or misaligned");
   uint8_t *ws = (uint8_t *)workspace;

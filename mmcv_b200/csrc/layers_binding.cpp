@@ -133,7 +133,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor &gy, const Tenso
   const int64_t align = (int64_t)(uintptr_t)gr.p | (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p |
                         ((gr.ld | xr.ld | wr.ld) * es);
   size_t bytes = 0;
-  check(dcn_linear_backward_workspace_bytes(code, act, gr.rows, cin, cout, align, want.x, want.w, &bytes));
+  check(dcn_linear_backward_workspace_bytes(code, act, gr.rows, cin, cout, align, want.x, want.w, want.b, &bytes));
   const Tensor ws = workspace(gy, bytes);
   check(dcn_linear_backward(gr.p, gr.ld, xr.p, xr.ld, wr.p, wr.ld, out_ptr(saved), out_ptr(in_saved), out_ptr(add),
                             out_ptr(gx), out_ptr(gw), out_ptr(gb), code, act, in_act, gr.rows, cin, cout, dev,

@@ -48,7 +48,7 @@ def test_c_entries_reject_bad_arguments_without_a_device():
     assert lib.dcn_linear_workspace_bytes(1, -1, 8, 8, 0, ctypes.byref(n)) == -1
     assert lib.dcn_linear_workspace_bytes(1, 1, 8, 1 << 21, 0, ctypes.byref(n)) == -2
     assert lib.dcn_linear_workspace_bytes(1, 1, 8, 8, 0, None) == -1
-    assert lib.dcn_linear_backward_workspace_bytes(1, 9, 1, 8, 8, 0, 1, 1, ctypes.byref(n)) == -1
+    assert lib.dcn_linear_backward_workspace_bytes(1, 9, 1, 8, 8, 0, 1, 1, 1, ctypes.byref(n)) == -1
     p = 4096   # never dereferenced: the checks come first
     fwd = lib.dcn_linear_forward
     assert fwd(None, 8, p, 8, None, None, 0, p, None, 1, 0, 4, 8, 8, 0, None, 0, None) == -1 and 'non-NULL' in last()
