@@ -480,7 +480,10 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
               tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const float v = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+                // an infinite element has planes inf, 0, 0: the leading product is right, the small ones
+                // may hold inf * 0
+                const float lead = __uint_as_float(a[j]);
+                const float v = isinf(lead) ? lead : lead + __uint_as_float(b[j]);
                 facc[c + j] = u ? facc[c + j] + v : v;
               }
             }

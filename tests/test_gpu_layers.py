@@ -167,6 +167,29 @@ def test_linear_non_finite_rows_stay_alone():
             assert bad[37] and int(torch.isnan(y).any(1).sum()) == 1
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_linear_infinities(dtype):
+    """An infinite element of x makes its row of z infinite with the sign of the weight (NaN where that is
+    zero), whatever the finite ones are; the same in the gradients."""
+    inf = float('inf')
+    x, w, b, _, gy = linear_case(140, 600, 72, dtype, None)
+    w[5] = 1.0                     # nothing below the leading bits
+    x[3, 17], x[9, 400], x[130, 599] = inf, -inf, inf
+    y = ops.fused_linear(x, w, b)
+    want = x.double() @ w.double().t() + b.double()
+    assert not torch.isfinite(want[[3, 9, 130]]).any()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    assert torch.equal(torch.sign(y[[3, 9, 130]]), torch.sign(want[[3, 9, 130]]).to(dtype))
+    x = linear_case(140, 600, 72, dtype, None)[0]
+    gy[70, 5] = inf
+    got = run_linear(x, w, b, None, gy, None)
+    for key, ref in (('gx', gy.double() @ w.double()), ('gw', gy.double().t() @ x.double()), ('gb', gy.double().sum(0))):
+        assert torch.equal(torch.isnan(got[key]), torch.isnan(ref)), key
+        assert torch.equal(got[key][torch.isinf(ref)].double(), ref[torch.isinf(ref)]), key
+    y = ops.fused_linear(torch.full((4, 600), -inf, dtype=dtype, device='cuda'), w.abs() + 0.5, b, activation='gelu')
+    assert torch.equal(y, torch.zeros_like(y))      # gelu(-inf)
+
+
 def test_linear_gradient_against_differences():
     """The directional derivative of sum(y * gy) along random directions, by central differences of
     the 64-bit form; the gradients are fp32: relative error of a sum of n products, and the
