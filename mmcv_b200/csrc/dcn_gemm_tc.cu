@@ -2,6 +2,7 @@
 // element-wise pass that writes operand planes, and the ordered sums of split results.
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include <cuda.h>
 
@@ -109,13 +110,14 @@ __global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (bits >> i) & 1u ? v[i] : 0.f;
       } else if (a.act == DCN_ACT_GELU) {
-        const T *z = (const T *)a.saved + r * a.pitch + c;   // kept with the same pitch
-        uint4 u[sizeof(T) / 2];
+        using Z = std::conditional_t<sizeof(T) == 4, float, __half>;
+        const Z *z = (const Z *)a.saved + r * a.pitch + c;   // kept with the same pitch
+        uint4 u[sizeof(Z) / 2];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4 *>(z)[i];
-        const T *e = reinterpret_cast<const T *>(u);
+        for (int i = 0; i < (int)sizeof(Z) / 2; ++i) u[i] = reinterpret_cast<const uint4 *>(z)[i];
+        const Z *e = reinterpret_cast<const Z *>(u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope<PL == 3>(ElemOf<T>::to(e[i]));
+        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope<PL == 3>(ElemOf<Z>::to(e[i]));
       }
       if constexpr (PL == 1) {
         uint32_t w[4];

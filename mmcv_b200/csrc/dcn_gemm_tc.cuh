@@ -373,6 +373,9 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   constexpr int RB = kChunkRow<TO, BN>, kChunkBytes = 32 * RB;
   constexpr int CW = RB / (int)sizeof(TO);             // columns of a staging chunk
   constexpr int kWarpCols = BN / kGroups > CW ? BN / kGroups : CW;   // columns of an epilogue warp
+  // Kept pre-activations of 16-bit tensors are fp16 whatever the tensors' type: eight times finer than bf16
+  // within +-65504, and gelu's derivative is 0 or 1 beyond +-40, an infinity's too.
+  using TZ = std::conditional_t<sizeof(TO) == 4, float, __half>;
 
   const GemmArgs &g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           for (int c1 = 0; c1 < CW; c1 += 32) {
             float v[32];
             sums(j0 + c1, ch * CW + c1, v);
-            stage_store<TO, RB>(chunk, lane, c1 * (int)sizeof(TO) / 16, v);
+            stage_store<TZ, RB>(chunk, lane, c1 * (int)sizeof(TZ) / 16, v);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
 #pragma unroll
             for (int k = 0; k < 32 / E; ++k) {
               float z[E];
-              unpack16<TO>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), z);
+              unpack16<TZ>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), z);
 #pragma unroll
               for (int j = 0; j < E; ++j) v[E * k + j] *= gelu_slope<PL == 3>(z[j]);
             }

@@ -100,7 +100,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor &x, const Tensor &w, const
   Tensor y = at::empty(shape, x.options()), saved;
   const Tensor b = has(bias) ? bias->contiguous() : Tensor();
   if (save && act == DCN_ACT_RELU) saved = at::empty({xr.rows, (cout + 31) / 32}, x.options().dtype(at::kInt));
-  if (save && act == DCN_ACT_GELU) saved = at::empty({xr.rows, (cout + 7) / 8 * 8}, x.options());
+  if (save && act == DCN_ACT_GELU) saved = at::empty({xr.rows, (cout + 7) / 8 * 8}, x.options().dtype(code == DCN_DTYPE_F32 ? at::kFloat : at::kHalf));
   const int64_t align = (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p | ((xr.ld | wr.ld) * es);
   size_t bytes = 0;
   check(dcn_linear_workspace_bytes(code, xr.rows, cin, cout, align, &bytes));

@@ -190,6 +190,26 @@ def test_linear_infinities(dtype):
     assert torch.equal(y, torch.zeros_like(y))      # gelu(-inf)
 
 
+def test_gelu_gradient_keeps_fine_and_huge_pre_activations():
+    """One element per row with a weight of one: gz alone is tested, through gx.  Its pre-activation is
+    kept in fp16 for bf16 tensors: half a step of 2^-11 of |z| (slope's slope at most 0.8), then the two
+    roundings of gz and gx to bf16; beyond fp16's range the derivative is 0 or 1 exactly."""
+    z = torch.cat([torch.linspace(-6, 6, 400), torch.tensor([1e5, -1e5, 3e38, -3e38, 70.0, -70.0])])
+    x = torch.zeros(z.numel(), 8)
+    x[:, 0] = z
+    x = x.bfloat16().cuda().requires_grad_(True)
+    w = torch.zeros(8, 8)
+    w[0, 0] = 1
+    w = w.bfloat16().cuda()
+    y = ops.fused_linear(x, w, activation='gelu')
+    gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    v = x.detach()[:, 0].double()
+    slope = plain.activation(v, 'gelu')[1]
+    bound = 0.8 * v.abs().clamp(max=40) * 2.0 ** -11 + slope.abs() * (2 * 2.0 ** -8 + 2.0 ** -16) + 2.0 ** -19
+    assert ((gx[:, 0].double() - slope).abs() <= bound).all()
+    assert gx[-6:, 0].tolist() == [1, 0, 1, 0, 1, 0]
+
+
 def test_linear_gradient_against_differences():
     """The directional derivative of sum(y * gy) along random directions, by central differences of
     the 64-bit form; the gradients are fp32: relative error of a sum of n products, and the
