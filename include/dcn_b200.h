@@ -375,14 +375,16 @@ int dcn_msda_backward(const void *value, const int64_t *spatial_shapes, const in
  * dcn_linear_backward, from gy = dL/dy [rows, cout] (row stride ldgy) and gz = gy * act'(z):
  *     gx = (gz weight) * in_act'(in_saved) + gx_add      [rows, cin] dense
  *     gw = gz^T x   [cout, cin] dense,     gb = sum_r gz [cout]
- * gx, gw and gb may be NULL (not wanted); x may be NULL when gw is, weight when gx is.  in_act /
+ * gx_sum [cin]: column sums of gx before its rounding, the bias gradient of the layer before; only with
+ * gx and in_act and without gx_add.
+ * gx, gx_sum, gw and gb may be NULL (not wanted); x may be NULL when gw is, weight when gx is.  in_act /
  * in_saved apply the derivative of the activation that produced x (its own `saved` tensor), for a
  * caller that runs two products back to back; DCN_ACT_NONE leaves it out.  gx_add [rows, cin]
  * dense, or NULL.  The result does not depend on the order in which blocks run.
  *
  * The workspace is scratch, 256-byte aligned, of the size the two *_workspace_bytes functions
  * report for the same arguments (alignment: the bitwise OR of the operands' addresses and of their
- * row strides in bytes; only its low four bits count).  Asynchronous on `stream`, no allocation.
+ * row strides in bytes; only its low four bits count; want_gx: 2 for gx_sum as well).  Asynchronous on `stream`, no allocation.
  * rows may be 0: y is empty, gw and gb are zero.  One-time work per device (kernel attributes) is
  * done by the first call on it, also inside a stream capture.
  */
@@ -397,7 +399,7 @@ int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows
                                         size_t *bytes);
 int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
                         int64_t ldw, const void *saved, const void *in_saved, const void *gx_add, void *gx,
-                        void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
+                        void *gx_sum, void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
                         int64_t cin, int64_t cout, int32_t device, void *workspace, size_t workspace_bytes,
                         void *stream);
 

@@ -124,7 +124,7 @@ def load():
         [vp, i64, vp, i64, vp, vp, i64, vp, vp, i32, i32, i64, i64, i64, i32, vp, sz, vp])
     lib.dcn_linear_backward_workspace_bytes.argtypes = [i32, i32] + [i64] * 4 + [i32, i32, i32, P(sz)]
     lib.dcn_linear_backward.argtypes = (
-        [vp, i64, vp, i64, vp, i64] + [vp] * 6 + [i32] * 3 + [i64] * 3 + [i32, vp, sz, vp])
+        [vp, i64, vp, i64, vp, i64] + [vp] * 7 + [i32] * 3 + [i64] * 3 + [i32, vp, sz, vp])
     lib.dcn_linear_read_status.argtypes = [i32, vp, P(i32)]
     lib.dcn_layer_norm_forward.argtypes = (
         [vp, i64, vp, vp, vp, vp, i32, i32, i64, i64, f32, i32, vp])

@@ -45,8 +45,10 @@ __global__ void __launch_bounds__(1024) dcn_column_reduce(const float *__restric
   float v = 0.f;
   pdl_wait();
   pdl_launch();
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int p = ty; p < parts; p += 32) v += part[p * cols + c];
+  }
   sm[ty][tx] = v;
   __syncthreads();
   for (int d = 16; d > 0; d >>= 1) {

@@ -343,6 +343,20 @@ __device__ __forceinline__ void chunk_out(uint8_t *chunk, TO *dst, long long ld,
     for (int c = 0; c < P; ++c)
       if (j0 + c * 32 + lane < n) dst[r * ld + c * 32 + lane] = *chunk_at<TO, RB>(chunk, r, c * 32 + lane);
 }
+// The sum over the lanes of v[j], in lane j: 31 exchanges, each lane giving away the half that the other
+// keeps.  v is used up.
+__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int j = 0; j < d; ++j) {
+      const float give = up ? v[j] : v[j + d], keep = up ? v[j + d] : v[j];
+      v[j] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+    }
+  }
+  return v[0];
+}
 // v[0..31] += a lane's own row of the residual, for the rare epilogue whose chunk is taken
 template <typename TO>
 __device__ __forceinline__ void add_row(const TO *src, int j1, int n, float (&v)[32]) {
@@ -602,6 +616,16 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           }
           if (EPI == kEpiRelu && sizeof(TO) == 2 && !g.res) stage_store<TO, RB, EPI == kEpiRelu>(chunk, lane, q0, v);
           else stage_store<TO, RB>(chunk, lane, q0, v);
+          if constexpr (EPI == kEpiSlopeRelu || EPI == kEpiSlopeGelu) {
+            if (g.col_part) {   // no residual then: v is the gradient itself
+              if (row >= m) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.f;
+              }
+              const float s = column_sums(v, lane);
+              if (i0 < m && j1 + lane < n) g.col_part[(long long)(i0 >> 5) * n + j1 + lane] = s;
+            }
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();

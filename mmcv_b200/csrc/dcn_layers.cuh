@@ -35,6 +35,9 @@ struct GemmArgs {
   void *out;       // element type of the operands, row stride n
   // row sums of A over k, [m] (the bias gradient, when A is the transposed output gradient)
   void *row_sum;
+  // with slope_act: fp32 column sums of v (before the residual and the rounding) over every 32 rows,
+  // [ceil(m / 32)][n]
+  float *col_part;
 };
 
 template <typename T> struct ElemOf;

@@ -4,6 +4,8 @@
 //   backward  gz = gy * act'(z)                            element-wise, only with an activation
 //             gx = gz W  (times the derivative of the activation before, plus gx_add)
 //             gW = gz^T x,  gb = column sums of gz
+// Column sums of gx on its way through that derivative (the bias gradient of the layer before) are taken
+// from the epilogue's fp32 values: gx itself is rounded to the tensors' type.
 // 16-bit operands whose rows start on 16 bytes are read where they lie; others are first copied to
 // rows that do, and fp32 operands are split into three bf16 planes (dcn_gemm_stage, both).
 #include "dcn_gemm.cuh"
@@ -22,7 +24,7 @@ size_t plane_bytes(int dtype, long long rows, long long cols) {
 
 // Byte offsets of a pass's scratch tensors; total in `bytes`.
 struct Layout {
-  size_t gz = 0, x = 0, w = 0, part = 0, row_part = 0, sums = 0, bytes = 0;
+  size_t gz = 0, x = 0, w = 0, part = 0, row_part = 0, sums = 0, gx_sums = 0, bytes = 0;
   bool stage_gz = false, stage_x = false, stage_w = false;
   GemmPlan gx_plan = {}, gw_plan = {};
 };
@@ -44,7 +46,7 @@ Layout forward_layout(int dtype, long long rows, long long cin, long long cout, 
 }
 
 Layout backward_layout(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment,
-                       bool want_gx, bool want_gw, bool want_gb) {
+                       bool want_gx, bool want_gw, bool want_gb, bool want_gx_sum) {
   Layout l;
   const bool stage = needs_stage(dtype, alignment);
   l.stage_gz = stage || act != DCN_ACT_NONE || (want_gb && !want_gw);   // the last: for its column sums
@@ -60,6 +62,7 @@ Layout backward_layout(int dtype, int act, long long rows, long long cin, long l
     l.row_part = take(&l, l.gw_plan.row_part_bytes);
   }
   if (l.stage_gz) l.sums = take(&l, (size_t)stage_slabs(rows, cout) * cout * 4);
+  if (want_gx_sum) l.gx_sums = take(&l, (size_t)((rows + 31) / 32) * cin * 4);
   return l;
 }
 
@@ -142,13 +145,14 @@ int dcn_linear_backward_workspace_bytes(int32_t dtype, int32_t act, int64_t rows
   if (!bytes) return set_error(DCN_ERR_ARG, "linear: bytes is NULL");
   int rc = check_sizes(dtype, act, rows, cin, cout);
   if (rc) return rc;
-  *bytes = rows ? backward_layout(dtype, act, rows, cin, cout, alignment, want_gx != 0, want_gw != 0, want_gb != 0).bytes : 0;
+  *bytes = rows ? backward_layout(dtype, act, rows, cin, cout, alignment, want_gx != 0, want_gw != 0, want_gb != 0,
+                                  want_gx == 2).bytes : 0;
   return DCN_OK;
 }
 
 int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx, const void *weight,
                         int64_t ldw, const void *saved, const void *in_saved, const void *gx_add, void *gx,
-                        void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
+                        void *gx_sum, void *gw, void *gb, int32_t dtype, int32_t act, int32_t in_act, int64_t rows,
                         int64_t cin, int64_t cout, int32_t device, void *workspace, size_t workspace_bytes,
                         void *stream) {
   int rc = check_sizes(dtype, act, rows, cin, cout);
@@ -161,11 +165,14 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
   if (rows == 0) {
     if (gw) e = cudaMemsetAsync(gw, 0, (size_t)cin * cout * esize(dtype), s);
     if (e == cudaSuccess && gb) e = cudaMemsetAsync(gb, 0, (size_t)cout * esize(dtype), s);
+    if (e == cudaSuccess && gx_sum) e = cudaMemsetAsync(gx_sum, 0, (size_t)cin * esize(dtype), s);
     return e == cudaSuccess ? DCN_OK : cuda_error(e);
   }
   if (!gy || (gx && !weight) || (gw && !x) || (act != DCN_ACT_NONE && !saved) ||
       (gx && in_act != DCN_ACT_NONE && !in_saved))
     return set_error(DCN_ERR_ARG, "linear backward: a needed pointer is NULL");
+  if (gx_sum && (!gx || gx_add || in_act == DCN_ACT_NONE))
+    return set_error(DCN_ERR_ARG, "linear backward: gx_sum goes with gx and in_act, without gx_add");
   if (ldgy < cout || (gw && ldx < cin) || (gx && ldw < cin))
     return set_error(DCN_ERR_ARG, "linear backward: a row stride is smaller than the row");
   if ((act == DCN_ACT_GELU && !aligned16(saved)) || (in_act == DCN_ACT_GELU && !aligned16(in_saved)))
@@ -175,7 +182,8 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
   if (rows == 1) { ldgy = pitch_of(cout); ldx = pitch_of(cin); }   // a single row has no stride
   const int64_t alignment = (int64_t)(uintptr_t)gy | (gw ? (int64_t)(uintptr_t)x | ldx * es : 0) |
                             (gx ? (int64_t)(uintptr_t)weight | ldw * es : 0) | ldgy * es;
-  const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr, gb != nullptr);
+  const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr, gb != nullptr,
+                                   gx_sum != nullptr);
   if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
     return set_error(DCN_ERR_WORKSPACE, "linear backward: workspace missing, too small or misaligned");
   uint8_t *ws = (uint8_t *)workspace;
@@ -200,7 +208,9 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
     g.a = gz; g.lda = ldgz; g.b = wt; g.ldb = ldwt; g.b_mn = true;
     g.m = rows; g.n = cin; g.kk = cout;
     g.slope = in_saved; g.slope_act = in_act; g.res = gx_add; g.ldr = cin; g.out = gx;
+    g.col_part = gx_sum ? (float *)(ws + l.gx_sums) : nullptr;
     e = launch_gemm_tc(g, l.gx_plan, dtype, nullptr, nullptr, s);
+    if (e == cudaSuccess && gx_sum) e = launch_column_reduce(g.col_part, (int)((rows + 31) / 32), cin, dtype, gx_sum, s);
     if (e != cudaSuccess) return cuda_error(e);
   }
   if (gw) {

@@ -4,6 +4,9 @@
 // host time than its kernels run (a layer norm's training step on 300 rows: 121 us of host time with
 // Python nodes).  mmcv_b200/_layers.py loads it; mmcv_b200.ops documents the operators.
 #include <atomic>
+#include <initializer_list>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -11,8 +14,11 @@
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 
@@ -22,7 +28,7 @@ namespace {
 
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 std::atomic<bool> g_check_status{false};
@@ -111,11 +117,12 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor &x, const Tensor &w, const
   return {y, saved};
 }
 
-struct Want { bool x, w, b; };
+struct Want { bool x, w, b, x_sum; };
+struct LinearGrads { Tensor x, w, b, x_sum; };
 
 // The gradients of linear_forward that `want` asks for.  in_saved / in_act: the gradient of x is taken on
-// through the activation that made x; gx_add is added to it.
-std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor &gy, const Tensor &x, const Tensor &w, int64_t cin,
+// through the activation that made x; gx_add is added to it; x_sum: its column sums.
+LinearGrads linear_backward(const Tensor &gy, const Tensor &x, const Tensor &w, int64_t cin,
                                                    const std::vector<int64_t> &x_shape, const Tensor &saved, int act,
                                                    Want want, const Tensor &in_saved, int in_act,
                                                    const Tensor &gx_add) {
@@ -125,21 +132,23 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor &gy, const Tenso
   const int dev = gy.device().index();
   void *stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   const Rows gr(gy, cout), xr = want.w ? Rows(x, cin) : Rows(), wr = want.x ? Rows(w, cin) : Rows();
-  Tensor gx, gw, gb;
-  if (want.x) gx = at::empty(x_shape, gy.options());
-  if (want.w) gw = at::empty({cout, cin}, gy.options());
-  if (want.b) gb = at::empty({cout}, gy.options());
+  LinearGrads g;
+  if (want.x) g.x = at::empty(x_shape, gy.options());
+  if (want.w) g.w = at::empty({cout, cin}, gy.options());
+  if (want.b) g.b = at::empty({cout}, gy.options());
+  if (want.x_sum) g.x_sum = at::empty({cin}, gy.options());
   const Tensor add = gx_add.defined() ? gx_add.contiguous() : Tensor();
   const int64_t align = (int64_t)(uintptr_t)gr.p | (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p |
                         ((gr.ld | xr.ld | wr.ld) * es);
   size_t bytes = 0;
-  check(dcn_linear_backward_workspace_bytes(code, act, gr.rows, cin, cout, align, want.x, want.w, want.b, &bytes));
+  check(dcn_linear_backward_workspace_bytes(code, act, gr.rows, cin, cout, align, want.x ? want.x_sum ? 2 : 1 : 0,
+                                            want.w, want.b, &bytes));
   const Tensor ws = workspace(gy, bytes);
   check(dcn_linear_backward(gr.p, gr.ld, xr.p, xr.ld, wr.p, wr.ld, out_ptr(saved), out_ptr(in_saved), out_ptr(add),
-                            out_ptr(gx), out_ptr(gw), out_ptr(gb), code, act, in_act, gr.rows, cin, cout, dev,
+                            out_ptr(g.x), out_ptr(g.x_sum), out_ptr(g.w), out_ptr(g.b), code, act, in_act, gr.rows, cin, cout, dev,
                             out_ptr(ws), bytes, stream));
   after(dev, stream);
-  return {gx, gw, gb};
+  return g;
 }
 
 // The kernels' gradients are values, not functions of the inputs: a second derivative is an error, not zero.
@@ -160,30 +169,54 @@ variable_list once(const char *op, variable_list grads) {
 bool needs(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool needs(const OptTensor &t) { return has(t) && t->requires_grad(); }
 
-struct LinearNode : torch::autograd::Function<LinearNode> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias,
-                        const OptTensor &res, int64_t act) {
-    const bool nx = needs(x), nw = needs(w), nb = needs(bias);
-    auto [y, saved] = linear_forward(x, w, bias, res, (int)act, nx || nw || nb);
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["cin"] = w.size(1);
-    ctx->saved_data["bias"] = has(bias);
-    ctx->saved_data["res"] = has(res);
-    ctx->save_for_backward({nw ? x : Tensor(), nx ? w : Tensor(), saved});
-    return y;
+// A tangent of forward-mode differentiation would be lost without a word.
+void refuse_tangents(const char *op, std::initializer_list<const Tensor *> tensors) {
+  for (const Tensor *t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "dcn_b200: ", op,
+                ": forward-mode differentiation is not supported");
+}
+
+const Tensor &get(const OptTensor &t) {
+  static const Tensor none;
+  return t.has_value() ? *t : none;
+}
+
+// Nodes are written against the engine's own interface: the convenience class for custom functions keeps
+// its values in a dictionary of boxed ones, 6 us more for a forward call and a backward pass.
+template <typename N, typename... T>
+std::shared_ptr<N> make_node(const T &...inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
+}
+
+struct LinearNode final : torch::autograd::Node {
+  SavedVariable x, w, saved;
+  std::vector<int64_t> shape;
+  int64_t cin = 0;
+  int act = 0;
+  std::string name() const override { return "FusedLinearBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    w.reset_data();
+    saved.reset_data();
   }
-  static variable_list backward(AutogradContext *ctx, variable_list gys) {
-    const variable_list s = ctx->get_saved_variables();
-    const bool bias = ctx->saved_data["bias"].toBool(), res = ctx->saved_data["res"].toBool();
-    const Want want{ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias && ctx->needs_input_grad(2)};
-    variable_list out(5);
+  variable_list apply(variable_list &&gys) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(4);
     if (!gys[0].defined()) return out;
-    if (want.x || want.w || want.b)
-      std::tie(out[0], out[1], out[2]) =
-          linear_backward(gys[0], s[0], s[1], ctx->saved_data["cin"].toInt(), ctx->saved_data["shape"].toIntVector(),
-                          s[2], (int)ctx->saved_data["act"].toInt(), want, Tensor(), DCN_ACT_NONE, Tensor());
-    if (res && ctx->needs_input_grad(2 + (bias ? 1 : 0))) out[3] = gys[0];
+    const Want want{task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2), false};
+    if (want.x || want.w || want.b) {
+      LinearGrads g;
+      {
+        const c10::AutoGradMode off(false);
+        g = linear_backward(gys[0], x.unpack(), w.unpack(), cin, shape, saved.unpack(), act, want, Tensor(),
+                            DCN_ACT_NONE, Tensor());
+      }
+      out = {g.x, g.w, g.b, Tensor()};
+    }
+    if (task_should_compute_output(3)) out[3] = gys[0];
     return once("fused_linear", std::move(out));
   }
 };
@@ -220,54 +253,70 @@ Tensor fused_linear(const Tensor &input, const Tensor &weight, const OptTensor &
   check_weight("fused_linear", "weight", input, input.size(-1), weight);
   check_bias("fused_linear", "bias", input, bias, weight.size(0));
   const OptTensor res = check_residual("fused_linear", input, residual, weight.size(0));
-  if (at::GradMode::is_enabled() && (needs(input) || needs(weight) || needs(bias) || needs(res)))
-    return LinearNode::apply(input, weight, bias, res, act);
-  return linear_forward(input, weight, bias, res, (int)act, false).first;
+  refuse_tangents("fused_linear", {&input, &weight, &get(bias), &get(res)});
+  const bool grad = at::GradMode::is_enabled(), nx = grad && needs(input), nw = grad && needs(weight),
+             nb = grad && needs(bias), nr = grad && needs(res);
+  std::pair<Tensor, Tensor> made;
+  {
+    const c10::AutoGradMode off(false);
+    made = linear_forward(input, weight, bias, res, (int)act, nx || nw || nb);
+  }
+  if (nx || nw || nb || nr) {
+    auto node = make_node<LinearNode>(input, weight, get(bias), get(res));
+    if (nw) node->x = SavedVariable(input, false);
+    if (nx) node->w = SavedVariable(weight, false);
+    if (made.second.defined()) node->saved = SavedVariable(made.second, false);
+    node->shape = input.sizes().vec();
+    node->cin = weight.size(1);
+    node->act = (int)act;
+    torch::autograd::set_history(made.first, node);
+  }
+  return made.first;
 }
 
 // ---- two products back to back ----------------------------------------------------------------
 
-struct FeedForwardNode : torch::autograd::Function<FeedForwardNode> {
-  // identity: the residual is the input itself (res is empty then)
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w1, const OptTensor &b1,
-                        const Tensor &w2, const OptTensor &b2, const OptTensor &res, int64_t act, bool identity) {
-    const bool inner = needs(x) || needs(w1) || needs(b1), keep_h = needs(w2);
-    auto [h, saved] = linear_forward(x, w1, b1, std::nullopt, (int)act, inner);
-    Tensor y = linear_forward(h, w2, b2, identity ? OptTensor(x) : res, DCN_ACT_NONE, false).first;
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["identity"] = identity;
-    ctx->saved_data["b1"] = has(b1);
-    ctx->saved_data["b2"] = has(b2);
-    ctx->saved_data["res"] = has(res);
-    ctx->save_for_backward({x, w1, w2, keep_h ? h : Tensor(), saved});
-    return y;
+struct FeedForwardNode final : torch::autograd::Node {
+  SavedVariable x, w1, w2, h, saved;
+  std::vector<int64_t> shape;
+  int64_t cin = 0, hidden = 0;
+  int act = 0;
+  bool identity = false;   // the residual is the input itself
+  std::string name() const override { return "FeedForwardBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable *v : {&x, &w1, &w2, &h, &saved}) v->reset_data();
   }
-  static variable_list backward(AutogradContext *ctx, variable_list gys) {
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w1 = s[1], &w2 = s[2];
-    const bool hb1 = ctx->saved_data["b1"].toBool(), hb2 = ctx->saved_data["b2"].toBool();
-    size_t edge = 0;   // edges exist for the tensors that were given
-    const bool nx = ctx->needs_input_grad(edge++), nw1 = ctx->needs_input_grad(edge++);
-    const bool nb1 = hb1 && ctx->needs_input_grad(edge++);
-    const bool nw2 = ctx->needs_input_grad(edge++);
-    const bool nb2 = hb2 && ctx->needs_input_grad(edge++);
-    const bool nres = ctx->saved_data["res"].toBool() && ctx->needs_input_grad(edge);
-    const bool inner = nx || nw1 || nb1;
-    variable_list out(8);
-    if (!gys[0].defined()) return out;
-    const int64_t hidden = w1.size(0);
-    auto h_shape = x.sizes().vec();
-    h_shape.back() = hidden;
-    Tensor gz;
-    if (inner || nw2 || nb2)
-      std::tie(gz, out[3], out[4]) =
-          linear_backward(gys[0], s[3], w2, hidden, h_shape, Tensor(), DCN_ACT_NONE, Want{inner, nw2, nb2}, s[4],
-                          (int)ctx->saved_data["act"].toInt(), Tensor());
-    if (inner)
-      std::tie(out[0], out[1], out[2]) =
-          linear_backward(gz, x, w1, x.size(-1), x.sizes().vec(), Tensor(), DCN_ACT_NONE, Want{nx, nw1, nb1}, Tensor(),
-                          DCN_ACT_NONE, nx && ctx->saved_data["identity"].toBool() ? gys[0] : Tensor());
-    if (nres) out[5] = gys[0];
+  variable_list apply(variable_list &&gys) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(6);
+    const Tensor &gy = gys[0];
+    if (!gy.defined()) return out;
+    const bool nx = task_should_compute_output(0), nw1 = task_should_compute_output(1),
+               nb1 = task_should_compute_output(2), nw2 = task_should_compute_output(3),
+               nb2 = task_should_compute_output(4), inner = nx || nw1 || nb1;
+    {
+      const c10::AutoGradMode off(false);
+      Tensor gz;
+      if (inner || nw2 || nb2) {
+        auto h_shape = shape;
+        h_shape.back() = hidden;
+        LinearGrads g = linear_backward(gy, h.unpack(), w2.unpack(), hidden, h_shape, Tensor(), DCN_ACT_NONE,
+                                        Want{inner, nw2, nb2, nb1}, saved.unpack(), act, Tensor());
+        gz = g.x;
+        out[2] = g.x_sum;
+        out[3] = g.w;
+        out[4] = g.b;
+      }
+      if (nx || nw1) {
+        LinearGrads g = linear_backward(gz, x.unpack(), w1.unpack(), cin, shape, Tensor(), DCN_ACT_NONE,
+                                        Want{nx, nw1, false, false}, Tensor(), DCN_ACT_NONE,
+                                        nx && identity ? gy : Tensor());
+        out[0] = g.x;
+        out[1] = g.w;
+      }
+    }
+    if (task_should_compute_output(5)) out[5] = gy;
     return once("feed_forward", std::move(out));
   }
 };
@@ -282,11 +331,32 @@ Tensor feed_forward(const Tensor &input, const Tensor &w1, const OptTensor &b1, 
   check_bias(op, "bias2", input, b2, w2.size(0));
   const bool identity = has(residual) && residual->is_same(input) && w2.size(0) == input.size(-1);
   const OptTensor res = identity ? OptTensor() : check_residual(op, input, residual, w2.size(0));
-  if (at::GradMode::is_enabled() &&
-      (needs(input) || needs(w1) || needs(b1) || needs(w2) || needs(b2) || needs(res)))
-    return FeedForwardNode::apply(input, w1, b1, w2, b2, res, act, identity);
-  const Tensor h = linear_forward(input, w1, b1, std::nullopt, (int)act, false).first;
-  return linear_forward(h, w2, b2, identity ? OptTensor(input) : res, DCN_ACT_NONE, false).first;
+  refuse_tangents(op, {&input, &w1, &get(b1), &w2, &get(b2), &get(res)});
+  const bool grad = at::GradMode::is_enabled(), nx = grad && needs(input), nw1 = grad && needs(w1),
+             nb1 = grad && needs(b1), nw2 = grad && needs(w2), nb2 = grad && needs(b2), nr = grad && needs(res);
+  const bool inner = nx || nw1 || nb1;
+  std::pair<Tensor, Tensor> first;
+  Tensor y;
+  {
+    const c10::AutoGradMode off(false);
+    first = linear_forward(input, w1, b1, std::nullopt, (int)act, inner);
+    y = linear_forward(first.first, w2, b2, identity ? OptTensor(input) : res, DCN_ACT_NONE, false).first;
+  }
+  if (inner || nw2 || nb2 || nr) {
+    auto node = make_node<FeedForwardNode>(input, w1, get(b1), w2, get(b2), get(res));
+    if (nw1) node->x = SavedVariable(input, false);
+    if (nx) node->w1 = SavedVariable(w1, false);
+    if (inner) node->w2 = SavedVariable(w2, false);
+    if (nw2) node->h = SavedVariable(first.first, false);
+    if (first.second.defined()) node->saved = SavedVariable(first.second, false);
+    node->shape = input.sizes().vec();
+    node->cin = input.size(-1);
+    node->hidden = w1.size(0);
+    node->act = (int)act;
+    node->identity = identity;
+    torch::autograd::set_history(y, node);
+  }
+  return y;
 }
 
 // ---- layer norm -------------------------------------------------------------------------------
@@ -305,43 +375,41 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor &x, const OptTensor &w, cons
   return {y, stats};
 }
 
-struct NormNode : torch::autograd::Function<NormNode> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const OptTensor &w, const OptTensor &b, int64_t cols,
-                        double eps) {
-    auto [y, stats] = norm_forward(x, w, b, cols, eps, true);
-    ctx->saved_data["cols"] = cols;
-    ctx->saved_data["w"] = has(w);
-    ctx->saved_data["b"] = has(b);
-    const Tensor &p = has(w) ? *w : has(b) ? *b : x;
-    ctx->saved_data["type"] = (int64_t)p.scalar_type();
-    ctx->saved_data["shape"] = p.sizes().vec();
-    ctx->save_for_backward({x, has(w) ? *w : Tensor(), stats});
-    return y;
+struct NormNode final : torch::autograd::Node {
+  SavedVariable x, w, stats;
+  int64_t cols = 0;
+  std::vector<int64_t> shape;        // of weight and bias
+  at::ScalarType type = at::kFloat;  // of weight and bias
+  std::string name() const override { return "LayerNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    w.reset_data();
+    stats.reset_data();
   }
-  static variable_list backward(AutogradContext *ctx, variable_list gys) {
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0];
-    const int64_t cols = ctx->saved_data["cols"].toInt();
-    const bool hw = ctx->saved_data["w"].toBool(), hb = ctx->saved_data["b"].toBool();
-    variable_list out(5);
+  variable_list apply(variable_list &&gys) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(3);
     if (!gys[0].defined()) return out;
-    const c10::cuda::CUDAGuard guard(x.device());
-    const int dev = x.device().index();
-    const at::ScalarType type = (at::ScalarType)ctx->saved_data["type"].toInt();
-    const auto shape = ctx->saved_data["shape"].toIntVector();
-    const auto options = x.options().dtype(type);
-    if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options());
-    if (hw && ctx->needs_input_grad(1)) out[1] = at::empty(shape, options);
-    if (hb && ctx->needs_input_grad(hw ? 2 : 1)) out[2] = at::empty(shape, options);
-    const Rows gr(gys[0], cols), xr(x, cols);
-    size_t bytes = 0;
-    if (out[1].defined() || out[2].defined()) check(dcn_layer_norm_workspace_bytes(xr.rows, cols, &bytes));
-    const Tensor ws = workspace(x, bytes);
-    check(dcn_layer_norm_backward(gr.p, gr.ld, xr.p, xr.ld, s[1].defined() ? s[1].const_data_ptr() : nullptr,
-                                  (const float *)s[2].const_data_ptr(), out_ptr(out[0]), out_ptr(out[1]),
-                                  out_ptr(out[2]), dtype_code("layer_norm", x.scalar_type()),
-                                  dtype_code("layer_norm", type), xr.rows, cols, dev, out_ptr(ws), bytes,
-                                  c10::cuda::getCurrentCUDAStream(dev).stream()));
+    {
+      const c10::AutoGradMode off(false);
+      const Tensor in = x.unpack(), weight = w.unpack(), st = stats.unpack();
+      const c10::cuda::CUDAGuard guard(in.device());
+      const int dev = in.device().index();
+      const auto options = in.options().dtype(type);
+      if (task_should_compute_output(0)) out[0] = at::empty(in.sizes(), in.options());
+      if (task_should_compute_output(1)) out[1] = at::empty(shape, options);
+      if (task_should_compute_output(2)) out[2] = at::empty(shape, options);
+      const Rows gr(gys[0], cols), xr(in, cols);
+      size_t bytes = 0;
+      if (out[1].defined() || out[2].defined()) check(dcn_layer_norm_workspace_bytes(xr.rows, cols, &bytes));
+      const Tensor ws = workspace(in, bytes);
+      check(dcn_layer_norm_backward(gr.p, gr.ld, xr.p, xr.ld, weight.defined() ? weight.const_data_ptr() : nullptr,
+                                    (const float *)st.const_data_ptr(), out_ptr(out[0]), out_ptr(out[1]),
+                                    out_ptr(out[2]), dtype_code("layer_norm", in.scalar_type()),
+                                    dtype_code("layer_norm", type), xr.rows, cols, dev, out_ptr(ws), bytes,
+                                    c10::cuda::getCurrentCUDAStream(dev).stream()));
+    }
     return once("layer_norm", std::move(out));
   }
 };
@@ -370,9 +438,25 @@ Tensor layer_norm(const Tensor &input, const std::vector<int64_t> &shape, const 
               ": weight and bias have different dtypes");
   const OptTensor w = has(weight) ? OptTensor(weight->contiguous()) : OptTensor();
   const OptTensor b = has(bias) ? OptTensor(bias->contiguous()) : OptTensor();
-  if (at::GradMode::is_enabled() && (needs(input) || needs(w) || needs(b)))
-    return NormNode::apply(input, w, b, cols, eps);
-  return norm_forward(input, w, b, cols, eps, false).first;
+  refuse_tangents(op, {&input, &get(w), &get(b)});
+  const bool grad = at::GradMode::is_enabled() && (needs(input) || needs(w) || needs(b));
+  std::pair<Tensor, Tensor> made;
+  {
+    const c10::AutoGradMode off(false);
+    made = norm_forward(input, w, b, cols, eps, grad);
+  }
+  if (grad) {
+    auto node = make_node<NormNode>(input, get(w), get(b));
+    node->x = SavedVariable(input, false);
+    if (has(w)) node->w = SavedVariable(*w, false);
+    node->stats = SavedVariable(made.second, false);
+    node->cols = cols;
+    const Tensor &p = has(w) ? *w : has(b) ? *b : input;
+    node->shape = p.sizes().vec();
+    node->type = p.scalar_type();
+    torch::autograd::set_history(made.first, node);
+  }
+  return made.first;
 }
 
 }  // namespace

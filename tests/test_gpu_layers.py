@@ -253,6 +253,62 @@ def test_feed_forward(rows, cin, hidden, dtype):
         hold({'y': y.detach(), 'gx': g}, {'y': both['y'], 'gx': gx.rounded(dtype)})
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,hidden', [(1, 16, 32), (31, 24, 70), (333, 40, 48), (2500, 64, 520)])
+def test_feed_forward_bias_gradient_is_summed_before_rounding(rows, cin, hidden, dtype):
+    """bias1's gradient within one rounding of the sum of the unrounded gradients, which the hidden
+    gradient's own rounding would exceed."""
+    for act in ('relu', 'gelu'):
+        x, gy = tensors(1, dtype, (rows, cin), (rows, cin))
+        w1, w2 = tensors(2, dtype, (hidden, cin), (cin, hidden), scale=(cin + hidden) ** -0.5)
+        b1, b2 = tensors(3, dtype, (hidden,), (cin,), scale=0.1)
+        z = plain.add(plain.product(plain.Value(x), plain.Value(w1)), b1.double())
+        gz = plain.through(plain.product(plain.Value(gy), plain.Value(w2).t()), z, act,
+                           kept=torch.float32 if dtype == torch.float32 else torch.float16)
+        want = plain.column_sum(gz).rounded(dtype)
+        leaf = b1.detach().requires_grad_(True)
+        g, = torch.autograd.grad(ops.feed_forward(x, w1, leaf, w2, b2, None, act), leaf, gy)
+        hold({'gb1': g}, {'gb1': want})
+        # the same bits beside the other gradients
+        leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2)]
+        grads = torch.autograd.grad(ops.feed_forward(*leaves, None, act), leaves, gy)
+        assert torch.equal(grads[2], g)
+
+
+def test_graphs_are_used_once_unless_retained():
+    x, w, b, r, gy = linear_case(20, 24, 32, torch.bfloat16, 'gelu')
+    w2, = tensors(5, torch.bfloat16, (24, 32))
+    for f in (lambda t: ops.fused_linear(t, w, b, activation='gelu'), lambda t: ops.layer_norm(t, (24,), t[0], None),
+              lambda t: ops.feed_forward(t, w, b, w2, None, t)):
+        leaf = x.detach().requires_grad_(True)
+        y = f(leaf)
+        one, = torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+        two, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        assert torch.equal(one, two)
+        with pytest.raises(RuntimeError, match='second time'):
+            torch.autograd.grad(y, leaf, torch.ones_like(y))
+    leaf, wl = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    y = ops.fused_linear(leaf, wl)
+    with torch.no_grad():
+        leaf.add_(1)           # what the backward pass needs has changed
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x, w, b, _, _ = linear_case(20, 24, 32, torch.bfloat16, None)
+    w2, = tensors(5, torch.bfloat16, (24, 32))
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda t: ops.fused_linear(t, w, b), lambda t: ops.layer_norm(t, (24,)),
+                  lambda t: ops.feed_forward(t, w, b, w2, None)):
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                f(dual)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            ops.fused_linear(x, w, fwd.make_dual(b, torch.ones_like(b)))
+
+
 NORM_SIZES = [(1, 1), (1, 256), (3, 8), (300, 256), (77, 100), (9, 1024), (5, 1537), (40, 2048), (3, 8192), (2, 8200),
               (3, 9001), (5000, 64), (1203, 384), (700, 4096)]
 
