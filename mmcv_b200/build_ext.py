@@ -60,7 +60,7 @@ def build_binding(force=False):
     for i in include:
         cmd += ['-isystem', i]
     cmd += [BINDING_SRC, '-o', BINDING, '-L', LIB_DIR, '-l:libdcn_b200.so', '-L', torch_lib, '-lc10', '-lc10_cuda',
-            '-ltorch_cpu', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
+            '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f'{CXX} failed on {BINDING_SRC}:\n{r.stdout}{r.stderr}')

@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "dcn_b200.h"
 
@@ -80,8 +81,13 @@ struct Rows {
 const void *ptr(const OptTensor &t) { return has(t) ? t->const_data_ptr() : nullptr; }
 void *out_ptr(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
+// A dense tensor on `like`'s device, straight from the allocator.
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 Tensor workspace(const Tensor &like, size_t bytes) {
-  return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+  return bytes ? make({(int64_t)bytes}, at::kByte, like) : Tensor();
 }
 
 void after(int device, void *stream) {
@@ -103,10 +109,10 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor &x, const Tensor &w, const
   const Rows xr(x, cin), wr(w, cin), rr = has(res) ? Rows(*res, cout) : Rows();
   auto shape = x.sizes().vec();
   shape.back() = cout;
-  Tensor y = at::empty(shape, x.options()), saved;
+  Tensor y = make(shape, x.scalar_type(), x), saved;
   const Tensor b = has(bias) ? bias->contiguous() : Tensor();
-  if (save && act == DCN_ACT_RELU) saved = at::empty({xr.rows, (cout + 31) / 32}, x.options().dtype(at::kInt));
-  if (save && act == DCN_ACT_GELU) saved = at::empty({xr.rows, (cout + 7) / 8 * 8}, x.options().dtype(code == DCN_DTYPE_F32 ? at::kFloat : at::kHalf));
+  if (save && act == DCN_ACT_RELU) saved = make({xr.rows, (cout + 31) / 32}, at::kInt, x);
+  if (save && act == DCN_ACT_GELU) saved = make({xr.rows, (cout + 7) / 8 * 8}, code == DCN_DTYPE_F32 ? at::kFloat : at::kHalf, x);
   const int64_t align = (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p | ((xr.ld | wr.ld) * es);
   size_t bytes = 0;
   check(dcn_linear_workspace_bytes(code, xr.rows, cin, cout, align, &bytes));
@@ -133,10 +139,11 @@ LinearGrads linear_backward(const Tensor &gy, const Tensor &x, const Tensor &w, 
   void *stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   const Rows gr(gy, cout), xr = want.w ? Rows(x, cin) : Rows(), wr = want.x ? Rows(w, cin) : Rows();
   LinearGrads g;
-  if (want.x) g.x = at::empty(x_shape, gy.options());
-  if (want.w) g.w = at::empty({cout, cin}, gy.options());
-  if (want.b) g.b = at::empty({cout}, gy.options());
-  if (want.x_sum) g.x_sum = at::empty({cin}, gy.options());
+  const at::ScalarType type = gy.scalar_type();
+  if (want.x) g.x = make(x_shape, type, gy);
+  if (want.w) g.w = make({cout, cin}, type, gy);
+  if (want.b) g.b = make({cout}, type, gy);
+  if (want.x_sum) g.x_sum = make({cin}, type, gy);
   const Tensor add = gx_add.defined() ? gx_add.contiguous() : Tensor();
   const int64_t align = (int64_t)(uintptr_t)gr.p | (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p |
                         ((gr.ld | xr.ld | wr.ld) * es);
@@ -367,8 +374,8 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor &x, const OptTensor &w, cons
   const c10::cuda::CUDAGuard guard(x.device());
   const int dev = x.device().index();
   const Rows xr(x, cols);
-  Tensor y = at::empty(x.sizes(), x.options()), stats;
-  if (save) stats = at::empty({3, xr.rows}, x.options().dtype(at::kFloat));
+  Tensor y = make(x.sizes(), x.scalar_type(), x), stats;
+  if (save) stats = make({3, xr.rows}, at::kFloat, x);
   const int wcode = has(w) ? dtype_code("layer_norm", w->scalar_type()) : has(b) ? dtype_code("layer_norm", b->scalar_type()) : code;
   check(dcn_layer_norm_forward(xr.p, xr.ld, ptr(w), ptr(b), out_ptr(y), (float *)out_ptr(stats), code, wcode, xr.rows,
                                cols, (float)eps, dev, c10::cuda::getCurrentCUDAStream(dev).stream()));
@@ -396,10 +403,9 @@ struct NormNode final : torch::autograd::Node {
       const Tensor in = x.unpack(), weight = w.unpack(), st = stats.unpack();
       const c10::cuda::CUDAGuard guard(in.device());
       const int dev = in.device().index();
-      const auto options = in.options().dtype(type);
-      if (task_should_compute_output(0)) out[0] = at::empty(in.sizes(), in.options());
-      if (task_should_compute_output(1)) out[1] = at::empty(shape, options);
-      if (task_should_compute_output(2)) out[2] = at::empty(shape, options);
+      if (task_should_compute_output(0)) out[0] = make(in.sizes(), in.scalar_type(), in);
+      if (task_should_compute_output(1)) out[1] = make(shape, type, in);
+      if (task_should_compute_output(2)) out[2] = make(shape, type, in);
       const Rows gr(gys[0], cols), xr(in, cols);
       size_t bytes = 0;
       if (out[1].defined() || out[2].defined()) check(dcn_layer_norm_workspace_bytes(xr.rows, cols, &bytes));
