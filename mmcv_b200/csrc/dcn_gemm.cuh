@@ -46,12 +46,43 @@ cudaError_t read_gemm_status_f32(cudaStream_t s, int *status);
 cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, float *part, float *row_part,
                            cudaStream_t s);
 
+// The forward product for m <= 8 (g.a, g.b in the tensors' own type, k contiguous, any row stride).
+cudaError_t launch_linear_rows(const GemmArgs &g, int dtype, cudaStream_t s);
+
+// Up to two products in one launch, operands in the tensors' own type as they lie (dcn_gemm_simt.cu).
+// a_saved / a_act: A is multiplied by that derivative, [rows of the tensor][its columns], as it is loaded.
+// g.row_sum without g.out: the row sums alone.
+struct SimtJob {
+  GemmArgs g;
+  const void *a_saved;
+  int a_act;
+  int tiles_n, tiles;
+};
+struct SimtJobs {
+  SimtJob job[2];   // no tiles: nothing to do
+};
+SimtJob simt_job(const GemmArgs &g, const void *a_saved, int a_act);
+cudaError_t launch_gemm_simt(const SimtJobs &jobs, int dtype, cudaStream_t s);
+
 // Element-wise pass in front of a product: v = src * act'(saved), written as the planes that the
-// product reads ([planes][rows][pitch], pitch a multiple of 8).  With `sums`, [slabs][cols] fp32
-// column sums of v as well; returns the number of slabs through *slabs.
-cudaError_t launch_gemm_stage(const void *src, long long ld, const void *saved, int act, long long rows,
-                              long long cols, int dtype, void *planes, long long pitch, float *sums, int *slabs,
-                              cudaStream_t s);
+// product reads ([planes][rows][pitch], pitch: cols rounded up to 8).  With `sums`, [stage_slabs][cols] fp32
+// column sums of v as well.
+struct StageJob {
+  const void *src, *saved;
+  void *dst;
+  float *sums;
+  long long ld, rows, cols, pitch;
+  int act;
+  int vec_src;                // rows start on 16 bytes
+  int log_tx, gx, gy, first;  // threads along a row, blocks along a row, slabs of rows, the first block
+};
+struct StageJobs {
+  StageJob job[3];
+  int count, blocks;
+};
+void add_stage(StageJobs *jobs, const void *src, long long ld, const void *saved, int act, long long rows, long long cols,
+               int dtype, void *planes, float *sums);
+cudaError_t launch_gemm_stage(StageJobs &jobs, int dtype, cudaStream_t s);
 int stage_slabs(long long rows, long long cols);
 // out[c] = sum over `parts` rows of part [parts][cols]
 cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s);

@@ -70,26 +70,22 @@ __device__ __forceinline__ void split3(float x, uint32_t (&b)[3]) {
   if (x != x) b[0] |= 0x00400000u;
 }
 
-struct StageArgs {
-  const void *src, *saved;
-  void *dst;
-  float *sums;
-  long long ld, rows, cols, pitch;
-  int act;
-  int vec_src;   // rows start on 16 bytes
-};
-
-// blockDim.x threads of 8 columns each, blockDim.y rows at a time; blockIdx.y: a slab of rows
+// The operands of a pass in one launch, a range of blocks each.  In a block, a power of two of threads of
+// 8 columns each, the rest side by side on rows; a slab of blocks takes every gy-th group of rows.
 template <typename T, int PL>
-__global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
+__global__ void __launch_bounds__(256) dcn_gemm_stage(const StageJobs jobs) {
   __shared__ float red[256 * 8];
-  const long long c = (blockIdx.x * (long long)blockDim.x + threadIdx.x) * 8;
+  const int which = (int)blockIdx.x < jobs.job[1].first ? 0 : (int)blockIdx.x < jobs.job[2].first ? 1 : 2;
+  const StageJob &a = jobs.job[which];
+  const int block = (int)blockIdx.x - a.first, slab = block / a.gx, tx = threadIdx.x & ((1 << a.log_tx) - 1),
+            ty = threadIdx.x >> a.log_tx, rows_at_once = 256 >> a.log_tx;
+  const long long c = ((long long)((block - slab * a.gx) << a.log_tx) + tx) * 8;
   const long long words = (a.cols + 31) / 32;
   pdl_wait();
   pdl_launch();
   float sum[8] = {};
   if (c < a.pitch) {
-    for (long long r = blockIdx.y * (long long)blockDim.y + threadIdx.y; r < a.rows; r += (long long)gridDim.y * blockDim.y) {
+    for (long long r = (long long)slab * rows_at_once + ty; r < a.rows; r += (long long)a.gy * rows_at_once) {
       float v[8];
       const T *src = (const T *)a.src + r * a.ld + c;
       if (a.vec_src && c + 8 <= a.cols) {
@@ -150,31 +146,30 @@ __global__ void __launch_bounds__(256) dcn_gemm_stage(const StageArgs a) {
   }
   if (!a.sums) return;
   // the block's rows in order, one row of threads after another
-  for (int y = 0; y < (int)blockDim.y; ++y) {
-    if ((int)threadIdx.y == y)
+  for (int y = 0; y < rows_at_once; ++y) {
+    if (ty == y)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float *s = red + threadIdx.x * 8 + i;
+        float *s = red + tx * 8 + i;
         *s = y ? *s + sum[i] : sum[i];
       }
     __syncthreads();
   }
-  if (threadIdx.y == 0)
+  if (ty == 0)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < a.cols) a.sums[blockIdx.y * a.cols + c + i] = red[threadIdx.x * 8 + i];
+      if (c + i < a.cols) a.sums[(long long)slab * a.cols + c + i] = red[tx * 8 + i];
 }
 
-void stage_shape(long long rows, long long pitch, int *tx, int *ty, int *gx, int *gy) {
-  int x = 1;
-  while (x < 32 && x * 8 < pitch) x *= 2;
-  *tx = x;
-  *ty = 256 / x;
-  *gx = (int)((pitch + x * 8 - 1) / (x * 8));
-  const long long want = (rows + *ty - 1) / *ty;
-  long long most = 148 * 8 / *gx;
+void stage_shape(long long rows, long long pitch, StageJob *j) {
+  j->log_tx = 0;
+  while (j->log_tx < 5 && (8LL << j->log_tx) < pitch) ++j->log_tx;
+  const long long x = 1LL << j->log_tx, y = 256 / x;
+  j->gx = (int)((pitch + x * 8 - 1) / (x * 8));
+  const long long want = (rows + y - 1) / y;
+  long long most = 148 * 8 / j->gx;
   if (most < 1) most = 1;
-  *gy = (int)(want < 1 ? 1 : want < most ? want : most);
+  j->gy = (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -313,26 +308,28 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
 }
 
 int stage_slabs(long long rows, long long cols) {
-  int tx, ty, gx, gy;
-  stage_shape(rows, (cols + 7) / 8 * 8, &tx, &ty, &gx, &gy);
-  return gy;
+  StageJob j;
+  stage_shape(rows, (cols + 7) / 8 * 8, &j);
+  return j.gy;
 }
 
-cudaError_t launch_gemm_stage(const void *src, long long ld, const void *saved, int act, long long rows,
-                              long long cols, int dtype, void *planes, long long pitch, float *sums, int *slabs,
-                              cudaStream_t s) {
-  StageArgs a = {};
-  a.src = src; a.saved = saved; a.dst = planes; a.sums = sums;
-  a.ld = ld; a.rows = rows; a.cols = cols; a.pitch = pitch; a.act = act;
-  const int esize = dtype == DCN_DTYPE_F32 ? 4 : 2;
-  a.vec_src = aligned16(src) && ld * esize % 16 == 0;
-  int tx, ty, gx, gy;
-  stage_shape(rows, pitch, &tx, &ty, &gx, &gy);
-  if (slabs) *slabs = gy;
-  const dim3 grid(gx, gy), block(tx, ty);
-  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_gemm_stage<float, 3>, grid, block, 0, s, 1, a);
-  if (dtype == DCN_DTYPE_BF16) return launch_pdl(dcn_gemm_stage<__nv_bfloat16, 1>, grid, block, 0, s, 1, a);
-  return launch_pdl(dcn_gemm_stage<__half, 1>, grid, block, 0, s, 1, a);
+void add_stage(StageJobs *jobs, const void *src, long long ld, const void *saved, int act, long long rows, long long cols,
+               int dtype, void *planes, float *sums) {
+  StageJob &j = jobs->job[jobs->count++];
+  j.src = src; j.saved = saved; j.dst = planes; j.sums = sums;
+  j.ld = ld; j.rows = rows; j.cols = cols; j.pitch = (cols + 7) / 8 * 8; j.act = act;
+  j.vec_src = aligned16(src) && ld * (dtype == DCN_DTYPE_F32 ? 4 : 2) % 16 == 0;
+  stage_shape(rows, j.pitch, &j);
+  j.first = jobs->blocks;
+  jobs->blocks += j.gx * j.gy;
+}
+
+cudaError_t launch_gemm_stage(StageJobs &jobs, int dtype, cudaStream_t s) {
+  if (!jobs.count) return cudaSuccess;
+  for (int i = jobs.count; i < 3; ++i) jobs.job[i].first = jobs.blocks;
+  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_gemm_stage<float, 3>, jobs.blocks, 256, 0, s, 1, jobs);
+  if (dtype == DCN_DTYPE_BF16) return launch_pdl(dcn_gemm_stage<__nv_bfloat16, 1>, jobs.blocks, 256, 0, s, 1, jobs);
+  return launch_pdl(dcn_gemm_stage<__half, 1>, jobs.blocks, 256, 0, s, 1, jobs);
 }
 
 cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s) {

@@ -26,6 +26,7 @@ size_t plane_bytes(int dtype, long long rows, long long cols) {
 struct Layout {
   size_t gz = 0, x = 0, w = 0, part = 0, row_part = 0, sums = 0, gx_sums = 0, bytes = 0;
   bool stage_gz = false, stage_x = false, stage_w = false;
+  bool rows = false, simt = false;   // nothing staged: dcn_linear_rows, dcn_gemm_simt
   GemmPlan gx_plan = {}, gw_plan = {};
 };
 size_t take(Layout *l, size_t n) {
@@ -35,8 +36,39 @@ size_t take(Layout *l, size_t n) {
 }
 bool needs_stage(int dtype, int64_t alignment) { return dtype == DCN_DTYPE_F32 || (alignment & 15) != 0; }
 
+// Which kernel a pass runs on; depends on sizes, type and alignment only, so that the workspace query and
+// the call agree and a call that keeps something for the backward pass gives the same bits as one that
+// does not.
+//
+// Times in us of one call among others, here / tensor cores with their staging pass:
+//   dcn_linear_rows   1 x 256 x 1024 bf16 2.0 / 4.5, fp32 2.2 / 10.1; 4 x 1024 x 1024 bf16 6.1 / 8.0, fp32
+//                     8.6 / 22; 4 x 4096 x 4096 bf16 20 / 23; 8 rows bf16 10.6 / 8.0, fp32 16 / 22
+//   dcn_gemm_simt     forward, fp32: 300 x 256 x 256 7.9 / 10.8, 600 x 256 x 256 11.2 / 10.9; backward, fp32:
+//                     300 x 256 x 256 9.1 / 25, 600 x 256 x 256 19 / 27, with gelu 100 x 256 x 256 21 / 23
+// and its one launch takes the place of two to six.  16-bit operands that need no staging stay on the tensor
+// cores (32 x 256 x 256 bf16 backward: 10.7 / 9.7).
+bool forward_rows(int dtype, long long rows, int64_t alignment) {
+  return rows <= (needs_stage(dtype, alignment) ? 8 : 4);
+}
+// rows as whole tiles
+double products(long long rows, long long cin, long long cout) {
+  return (double)((rows + 31) / 32 * 32) * (double)cin * (double)cout;
+}
+bool forward_simt(int dtype, long long rows, long long cin, long long cout) {
+  return dtype == DCN_DTYPE_F32 && cin <= 1024 && products(rows, cin, cout) <= 1 << 25;
+}
+// a block walks all of cout (for gx) or of the rows (for gw): long walks are slow; gelu's derivative is computed
+// again for every 32 columns of a product
+bool backward_simt(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment) {
+  return needs_stage(dtype, alignment) && rows <= 640 && cout <= 640 &&
+         products(rows, cin, cout) <= (act == DCN_ACT_GELU ? 1 << 23 : 1 << 25);
+}
+
 Layout forward_layout(int dtype, long long rows, long long cin, long long cout, int64_t alignment) {
   Layout l;
+  l.rows = forward_rows(dtype, rows, alignment);
+  l.simt = !l.rows && forward_simt(dtype, rows, cin, cout);
+  if (l.rows || l.simt) return l;
   l.stage_x = l.stage_w = needs_stage(dtype, alignment);
   if (l.stage_x) {
     l.x = take(&l, plane_bytes(dtype, rows, cin));
@@ -48,6 +80,9 @@ Layout forward_layout(int dtype, long long rows, long long cin, long long cout, 
 Layout backward_layout(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment,
                        bool want_gx, bool want_gw, bool want_gb, bool want_gx_sum) {
   Layout l;
+  if (want_gx_sum) l.gx_sums = take(&l, (size_t)((rows + 31) / 32) * cin * 4);
+  l.simt = backward_simt(dtype, act, rows, cin, cout, alignment);
+  if (l.simt) return l;
   const bool stage = needs_stage(dtype, alignment);
   l.stage_gz = stage || act != DCN_ACT_NONE || (want_gb && !want_gw);   // the last: for its column sums
   l.stage_x = stage && want_gw;
@@ -62,7 +97,6 @@ Layout backward_layout(int dtype, int act, long long rows, long long cin, long l
     l.row_part = take(&l, l.gw_plan.row_part_bytes);
   }
   if (l.stage_gz) l.sums = take(&l, (size_t)stage_slabs(rows, cout) * cout * 4);
-  if (want_gx_sum) l.gx_sums = take(&l, (size_t)((rows + 31) / 32) * cin * 4);
   return l;
 }
 
@@ -77,13 +111,6 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int64_t cin, int64_t c
   if (rows > most || cin > (1 << 20) || cout > (1 << 20))
     return set_error(DCN_ERR_UNSUPPORTED, "linear: at most 2^31 rows and 2^20 channels");
   return DCN_OK;
-}
-
-cudaError_t stage_operand(const void *src, long long ld, long long rows, long long cols, int dtype, void *dst,
-                          cudaStream_t s, const void **at, long long *pitch) {
-  *at = dst;
-  *pitch = pitch_of(cols);
-  return launch_gemm_stage(src, ld, nullptr, DCN_ACT_NONE, rows, cols, dtype, dst, *pitch, nullptr, nullptr, s);
 }
 
 int cuda_error(cudaError_t e) { return set_error(DCN_ERR_CUDA, cudaGetErrorString(e)); }
@@ -119,7 +146,6 @@ int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t l
   if (scope.err != cudaSuccess) return cuda_error(scope.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t es = (int64_t)esize(dtype);
-  if (rows == 1) ldx = pitch_of(cin);   // a single row has no stride
   const int64_t alignment = (int64_t)(uintptr_t)x | (int64_t)(uintptr_t)weight | ((ldx | ldw) * es);
   const Layout l = forward_layout(dtype, rows, cin, cout, alignment);
   if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
@@ -130,10 +156,21 @@ int dcn_linear_forward(const void *x, int64_t ldx, const void *weight, int64_t l
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = ldw;
   g.m = rows; g.n = cout; g.kk = cin;
   g.bias = bias; g.act = act; g.saved = saved; g.res = residual; g.ldr = ldr; g.out = y;
+  if (l.rows || l.simt) {
+    SimtJobs jobs = {};
+    if (l.simt) jobs.job[0] = simt_job(g, nullptr, DCN_ACT_NONE);
+    e = l.simt ? launch_gemm_simt(jobs, dtype, s) : launch_linear_rows(g, dtype, s);
+    return e == cudaSuccess ? DCN_OK : cuda_error(e);
+  }
   if (l.stage_x) {
-    e = stage_operand(x, ldx, rows, cin, dtype, ws + l.x, s, &g.a, &g.lda);
-    if (e == cudaSuccess) e = stage_operand(weight, ldw, cout, cin, dtype, ws + l.w, s, &g.b, &g.ldb);
+    StageJobs jobs = {};
+    add_stage(&jobs, x, ldx, nullptr, DCN_ACT_NONE, rows, cin, dtype, ws + l.x, nullptr);
+    add_stage(&jobs, weight, ldw, nullptr, DCN_ACT_NONE, cout, cin, dtype, ws + l.w, nullptr);
+    e = launch_gemm_stage(jobs, dtype, s);
     if (e != cudaSuccess) return cuda_error(e);
+    g.a = ws + l.x;
+    g.b = ws + l.w;
+    g.lda = g.ldb = pitch_of(cin);
   }
   e = launch_gemm_tc(g, plan_gemm(planes_of(dtype), rows, cout, cin, false), dtype, nullptr, nullptr, s);
   return e == cudaSuccess ? DCN_OK : cuda_error(e);
@@ -179,7 +216,6 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
     return set_error(DCN_ERR_ARG, "linear backward: saved and in_saved must be 16-byte aligned");
   if (!gx && !gw && !gb) return DCN_OK;
   const int64_t es = (int64_t)esize(dtype);
-  if (rows == 1) { ldgy = pitch_of(cout); ldx = pitch_of(cin); }   // a single row has no stride
   const int64_t alignment = (int64_t)(uintptr_t)gy | (gw ? (int64_t)(uintptr_t)x | ldx * es : 0) |
                             (gx ? (int64_t)(uintptr_t)weight | ldw * es : 0) | ldgy * es;
   const Layout l = backward_layout(dtype, act, rows, cin, cout, alignment, gx != nullptr, gw != nullptr, gb != nullptr,
@@ -187,21 +223,51 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
   if (l.bytes && (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)))
     return set_error(DCN_ERR_WORKSPACE, "linear backward: workspace missing, too small or misaligned");
   uint8_t *ws = (uint8_t *)workspace;
+  if (l.simt) {
+    SimtJobs jobs = {};
+    float *gx_part = gx_sum ? (float *)(ws + l.gx_sums) : nullptr;
+    if (gx) {
+      GemmArgs g = {};
+      g.a = gy; g.lda = ldgy; g.b = weight; g.ldb = ldw; g.b_mn = true;
+      g.m = rows; g.n = cin; g.kk = cout;
+      g.slope = in_saved; g.slope_act = in_act; g.res = gx_add; g.ldr = cin; g.out = gx; g.col_part = gx_part;
+      jobs.job[0] = simt_job(g, saved, act);
+    }
+    if (gw || gb) {
+      GemmArgs g = {};
+      g.a = gy; g.lda = ldgy; g.a_mn = true; g.b = x; g.ldb = ldx; g.b_mn = true;
+      g.m = cout; g.n = cin; g.kk = rows;
+      g.out = gw; g.row_sum = gb;
+      jobs.job[1] = simt_job(g, saved, act);
+    }
+    e = launch_gemm_simt(jobs, dtype, s);
+    if (e == cudaSuccess && gx_sum) e = launch_column_reduce(gx_part, (int)((rows + 31) / 32), cin, dtype, gx_sum, s);
+    return e == cudaSuccess ? DCN_OK : cuda_error(e);
+  }
   const void *gz = gy, *xs = x, *wt = weight;
   long long ldgz = ldgy, ldxs = ldx, ldwt = ldw;
   // the bias gradient: column sums of the staging pass, taken before gz is rounded, where there is one,
   // else row sums of the weight gradient's A operand
   const bool sums = gb && l.stage_gz;
+  StageJobs jobs = {};
   if (l.stage_gz) {
-    int slabs = 0;
-    ldgz = pitch_of(cout);
-    e = launch_gemm_stage(gy, ldgy, saved, act, rows, cout, dtype, ws + l.gz, ldgz,
-                          sums ? (float *)(ws + l.sums) : nullptr, &slabs, s);
-    if (e == cudaSuccess && sums) e = launch_column_reduce((const float *)(ws + l.sums), slabs, cout, dtype, gb, s);
+    add_stage(&jobs, gy, ldgy, saved, act, rows, cout, dtype, ws + l.gz, sums ? (float *)(ws + l.sums) : nullptr);
     gz = ws + l.gz;
+    ldgz = pitch_of(cout);
   }
-  if (e == cudaSuccess && l.stage_x) e = stage_operand(x, ldx, rows, cin, dtype, ws + l.x, s, &xs, &ldxs);
-  if (e == cudaSuccess && l.stage_w) e = stage_operand(weight, ldw, cout, cin, dtype, ws + l.w, s, &wt, &ldwt);
+  if (l.stage_x) {
+    add_stage(&jobs, x, ldx, nullptr, DCN_ACT_NONE, rows, cin, dtype, ws + l.x, nullptr);
+    xs = ws + l.x;
+    ldxs = pitch_of(cin);
+  }
+  if (l.stage_w) {
+    add_stage(&jobs, weight, ldw, nullptr, DCN_ACT_NONE, cout, cin, dtype, ws + l.w, nullptr);
+    wt = ws + l.w;
+    ldwt = pitch_of(cin);
+  }
+  e = launch_gemm_stage(jobs, dtype, s);
+  if (e == cudaSuccess && sums)
+    e = launch_column_reduce((const float *)(ws + l.sums), stage_slabs(rows, cout), cout, dtype, gb, s);
   if (e != cudaSuccess) return cuda_error(e);
   if (gx) {
     GemmArgs g = {};
