@@ -11,7 +11,8 @@ namespace dcn {
 struct GemmPlan {
   int bn;          // columns of an output tile
   int cg;          // blocks that share a tile: 1 (128 rows) or a cluster of 2 (256 rows)
-  int splits;      // ranges of k, each with fp32 parts of its own
+  int ks;          // blocks of a cluster that share a tile's sum over k, joined in shared memory (cg = 1, bn = 64)
+  int splits;      // ranges of k, each with fp32 parts of its own in memory
   int kb_total, kb_split;   // 64-value blocks of k, in all and in a range
   long long ldp;   // row stride of the fp32 parts, elements
   size_t part_bytes, row_part_bytes;   // 0 without splits
@@ -25,6 +26,7 @@ struct alignas(64) GemmTc {
   int m, n;                        // of g
   int tiles_m, tiles_n, splits, kb_total, kb_split;
   int step_n, step_m, step_s;      // a block's stride through the items, in column tiles, row tiles and ranges
+  int ks;
   int stages;
   int out_tma, res_tma;            // 0: element by element
   int bias16;                      // the bias starts on 16 bytes

@@ -224,7 +224,7 @@ GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weigh
   auto tiles = [&](int rows, int bn) { return (m + rows - 1) / rows * ((n + bn - 1) / bn); };
   p.kb_total = (int)((k + 63) / 64);
   p.splits = 1;
-  p.cg = 1;
+  p.cg = p.ks = 1;
   if (weight_gradient) {
     p.bn = n > wide / 2 ? wide : n > 64 ? 128 : 64;
     if (m > 128 && p.bn == wide) p.cg = 2;
@@ -243,7 +243,18 @@ GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weigh
     } else {
       p.bn = n > wide / 2 && tiles(128, wide) >= 148 ? wide : n > 64 && tiles(128, 128) >= 148 ? 128 : 64;
     }
-    p.kb_split = p.kb_total;
+    if (p.bn == 64) {
+      // Few tiles and a long sum: a block takes in 24 KB (fp32: 72 KB) a step at 46 bytes a cycle, so that
+      // sharing the steps pays for the cluster's 2 us from some length on.  One block / two / four, us:
+      // bf16 600 x 1024 x 256 8.4 / 8.7 / 9.2, 600 x 2048 x 64 12.9 / 10.8 / 9.4, 32 x 4096 x 4096 22.3 / 16.7;
+      // fp32 (two at most: each has 32 KB of sums to send) 600 x 256 x 256 10.0 / 10.7, 600 x 512 x 256
+      // 13.4 / 12.6, 600 x 1024 x 256 21.3 / 16.8, 32 x 4096 x 4096 97 / 68.
+      const int most = planes == 1 ? 4 : 2;
+      if (p.kb_total >= (planes == 1 ? 20 : 8))
+        while (p.ks < most && tiles(128, 64) * p.ks * 2 <= 148) p.ks *= 2;
+    }
+    p.kb_split = (p.kb_total + p.ks - 1) / p.ks;
+    while ((p.ks - 1) * p.kb_split >= p.kb_total) --p.ks;   // a range each
   }
   p.ldp = (n + 3) / 4 * 4;
   if (p.splits > 1) {
@@ -267,6 +278,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   p.tiles_m = (int)((g.m + 128 * plan.cg - 1) / (128 * plan.cg));
   p.tiles_n = (int)((g.n + plan.bn - 1) / plan.bn);
   p.splits = plan.splits;
+  p.ks = plan.ks;
   p.kb_total = plan.kb_total;
   p.kb_split = plan.kb_split;
   p.row_part = row_part;

@@ -141,27 +141,36 @@ __device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t cols)
   else
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
-template <int CG>
-__device__ __forceinline__ void pair_sync() {
-  if constexpr (CG == 2) {
+__device__ __forceinline__ void cluster_sync(bool clustered) {
+  if (clustered) {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
-// The address of the first block's copy of a shared variable, and an arrival there.
-template <int CG>
-__device__ __forceinline__ uint32_t lead_addr(uint32_t addr) {
-  if constexpr (CG == 1) return addr;
+// To the first block of a cluster: where its copy of a shared address is, 16 bytes there, an arrival there.
+__device__ __forceinline__ uint32_t first_block(uint32_t addr) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
+}
+__device__ __forceinline__ void cluster_store16(uint32_t addr, const float *v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
+               : "memory");
+}
+__device__ __forceinline__ void cluster_arrive(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// The address of the first block's copy of a shared variable, and an arrival there.
+template <int CG>
+__device__ __forceinline__ uint32_t lead_addr(uint32_t addr) {
+  return CG == 1 ? addr : first_block(addr);
 }
 template <int CG>
 __device__ __forceinline__ void lead_arrive(uint32_t addr) {
   if constexpr (CG == 1)
     mbar_arrive(addr);
   else
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    cluster_arrive(addr);
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
@@ -396,12 +405,18 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   const int ST = p.stages;
   const uint32_t bar0 = smem_u32(smem);
   const uint32_t full = bar0, empty = full + 8 * ST, tmem_full = empty + 8 * ST, tmem_empty = tmem_full + 16,
-                 in_bar = tmem_empty + 16;             // one per epilogue warp
+                 in_bar = tmem_empty + 16, part_bar = in_bar + 8 * kEpiWarps;   // one each per epilogue warp
+  // p.ks blocks of a cluster each sum a range of k of one tile; the first adds the others' sums, in order, to
+  // its own.  There are as many clusters as tiles then.
+  constexpr bool kCanShare = CG == 1 && BN == 64 && !AMN;
+  static_assert(!kCanShare || kWarpCols == 32, "a warp's part: 32 x 32");
+  const int ks = kCanShare ? p.ks : 1, krank = kCanShare && ks > 1 ? (int)(blockIdx.x % (uint32_t)ks) : 0;
   uint32_t *tmem_slot = (uint32_t *)(smem + 896);
   volatile int *abort_s = (volatile int *)(smem + 904);
   uint8_t *ring = smem + 1024;
   uint8_t *staging = ring + (size_t)ST * kStage;
   uint8_t *ones = staging + (size_t)kEpiWarps * kChunkBytes;
+  uint8_t *parts = ones;   // (nobody has both) [ks - 1][active epilogue warps][8][32 lanes] x 16 bytes
   const unsigned long long limit = p.wait_limit_ns;
 
   if (threadIdx.x == 0) {
@@ -413,7 +428,10 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
       mbar_init(tmem_full + 8 * i, 1);
       mbar_init(tmem_empty + 8 * i, CG * kEpiWarps);
     }
-    for (int i = 0; i < kEpiWarps; ++i) mbar_init(in_bar + 8 * i, 1);
+    for (int i = 0; i < kEpiWarps; ++i) {
+      mbar_init(in_bar + 8 * i, 1);
+      if (ks > 1) mbar_init(part_bar + 8 * i, ks - 1);
+    }
     *abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -427,14 +445,15 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  pair_sync<CG>();
+  cluster_sync(CG == 2 || ks > 1);
   tc_fence_after();
   pdl_wait();
   pdl_launch();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t items = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
   const int rank = CG == 1 ? 0 : (int)(blockIdx.x & 1);   // a cluster is two neighbouring blocks
-  const uint32_t first_item = blockIdx.x / CG, item_step = gridDim.x / CG;
+  const uint32_t first_item = ks > 1 ? blockIdx.x / (uint32_t)ks : blockIdx.x / CG,
+                 item_step = ks > 1 ? items : gridDim.x / CG;
   const uint32_t lead_empty = lead_addr<CG>(tmem_empty), lead_full = lead_addr<CG>(full);
 
   if (warp < kEpiWarps) {
@@ -454,7 +473,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
     for (uint32_t item = first_item; item < items && ok; item += item_step, walk.next(p)) {
       const int i0 = (walk.tm * CG + rank) * 128 + q * 32, row = i0 + lane;
       const int jw = walk.tn * BN + cg * kWarpCols;   // this warp's first column
-      const int kb0 = walk.sp * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
+      const int kb0 = (ks > 1 ? krank : walk.sp) * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
       const int chunks = cg * kWarpCols < BN && jw < n ? (min(n - jw, kWarpCols) + CW - 1) / CW : 0;
       // the store that read the chunk last is done with it
       auto chunk_free = [&] {
@@ -476,7 +495,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
         }
       };
       const bool takes = load_in || res_staged;
-      if (takes && chunks) fetch(jw);
+      if (takes && chunks && krank == 0) fetch(jw);
       float facc[PL == 3 ? kWarpCols : 1];
       const int units = PL == 3 ? (kb1 - kb0 + kUnitBlocks - 1) / kUnitBlocks : 1;
       int buf = 0;
@@ -519,6 +538,38 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           else ((TI *)g.row_sum)[row] = ElemOf<TI>::from(v);
         }
       }
+      if constexpr (kCanShare) {
+        if (ks > 1) {
+          const uint32_t mine = smem_u32(parts) + (uint32_t)warp * 4096u + (uint32_t)lane * 16u;
+          constexpr uint32_t kPart = BN / 32 * 4 * 4096u;   // of a block
+          if (krank) {
+            if (chunks) {
+              float v[32];
+              if constexpr (PL == 3) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = facc[j];
+              } else {
+                uint32_t r[32];
+                tmem_ld32(lane_base + (uint32_t)(cg * kWarpCols), r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+              }
+              const uint32_t to = first_block(mine + (uint32_t)(krank - 1) * kPart);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) cluster_store16(to + j * 512, v + 4 * j);
+              __syncwarp();
+              if (lane == 0) cluster_arrive(first_block(part_bar + 8 * warp));
+            }
+            break;   // the first block has the rest
+          }
+          if (chunks) {
+            ok = __all_sync(0xffffffffu, g_wait(part_bar + 8 * warp, 0, abort_s, 9, 2 * limit, 0));
+            if (!ok) break;
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          }
+        }
+      }
       // the 32 sums of a group of columns, with the bias
       auto sums = [&](int j1, int c, float (&v)[32]) {
         if constexpr (PL == 3) {
@@ -533,6 +584,16 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        }
+        if constexpr (kCanShare) {
+          for (int k = 1; k < ks; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = *reinterpret_cast<const float4 *>(
+                  parts + (size_t)(k - 1) * (BN / 32 * 4 * 4096) + warp * 4096 + j * 512 + lane * 16);
+              add2(v[4 * j], v[4 * j + 1], f.x, f.y);
+              add2(v[4 * j + 2], v[4 * j + 3], f.z, f.w);
+            }
         }
         if (g.bias) add_bias<TO>((const TO *)g.bias, j1, n, p.bias16 != 0, v);
       };
@@ -659,7 +720,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
     bool ok = rank == 0;   // the first block of a pair issues for both
     Walk walk(first_item, p);
     for (uint32_t item = first_item; item < items && ok; item += item_step, walk.next(p)) {
-      const int kb0 = walk.sp * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
+      const int kb0 = (ks > 1 ? krank : walk.sp) * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
       const bool sums = kRowSum && g.row_sum && walk.tn == 0;
       uint32_t d = 0;
       int buf = 0;
@@ -715,7 +776,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
       bool ok = true;
       Walk walk(first_item, p);
       for (uint32_t item = first_item; item < items && ok; item += item_step, walk.next(p)) {
-        const int kb0 = walk.sp * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
+        const int kb0 = (ks > 1 ? krank : walk.sp) * p.kb_split, kb1 = min(p.kb_total, kb0 + p.kb_split);
         const int m0 = (walk.tm * CG + rank) * 128, nb = walk.tn * BN + rank * (BN / CG);
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = g_wait(empty + 8 * st, ph ^ 1u, abort_s, 7, 2 * limit, 32);
@@ -753,7 +814,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  pair_sync<CG>();   // no block leaves while the other may still reach into it
+  cluster_sync(CG == 2 || ks > 1);   // no block leaves while the other may still reach into it
   if (warp == kEpiWarps) {
     tc_fence_after();
     pair_tmem_dealloc<CG>(tmem_base, kAlloc);
@@ -778,15 +839,17 @@ cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
   }
   constexpr size_t stage = (size_t)PL * (16384 + BN / CG * 128);
   constexpr size_t fixed = 1024 + 1024 + (size_t)kEpi<PL> * 32 * kChunkRow<TO, BN> + (AMN && PL == 1 ? 2048 : 0);
-  constexpr int stages = (kMost - fixed) / stage > 8 ? 8 : (int)((kMost - fixed) / stage);
-  static_assert(stages >= 2, "a ring");
+  const size_t parts = (size_t)(p.ks - 1) * (BN / 32 * 4 * 4096);
+  const int fit = (int)((kMost - fixed - parts) / stage), stages = fit > 8 ? 8 : fit;
+  static_assert((kMost - fixed) / stage >= 2, "a ring");
+  if (stages < 2 || (p.ks > 1 && (CG == 2 || BN != 64 || AMN))) return cudaErrorInvalidValue;
   p.stages = stages;
   const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
-  const int grid = CG * (int)(items < 148 / CG ? items : 148 / CG), step = grid / CG;
+  const int grid = p.ks > 1 ? (int)items * p.ks : CG * (int)(items < 148 / CG ? items : 148 / CG), step = grid / CG;
   p.step_n = step % p.tiles_n;
   p.step_m = step / p.tiles_n % p.tiles_m;
   p.step_s = step / p.tiles_n / p.tiles_m;
-  return launch_pdl(kern, grid, kThreadsOf<PL>, fixed + stages * stage, s, CG, p);
+  return launch_pdl(kern, grid, kThreadsOf<PL>, fixed + parts + stages * stage, s, p.ks > 1 ? p.ks : CG, p);
 }
 
 template <typename TI, typename TO, int PL, bool AMN, bool BMN, int EPI>

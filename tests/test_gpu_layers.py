@@ -59,6 +59,48 @@ def test_linear_forward_and_gradients(rows, cin, cout, dtype):
             assert torch.equal(ops.fused_linear(x, w, b, r, act), got['y'])
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,cout', [(9, 2048, 64), (300, 1024, 256), (130, 576, 40), (257, 1600, 100), (33, 4104, 72),
+                                           (20, 1030, 130), (140, 513, 90)])
+def test_linear_long_sums_of_few_tiles(rows, cin, cout, dtype):
+    """Sums over k that several blocks of a cluster share, forward and (with the sides swapped) backward,
+    ranges of uneven length among them."""
+    for act, res in ((None, True), ('relu', False), ('gelu', True)):
+        x, w, b, r, gy = linear_case(rows, cin, cout, dtype, act, True, res)
+        got = run_linear(x, w, b, r, gy, act)
+        hold(got, plain.linear(x, w, b, r, act, gy))
+        with torch.no_grad():
+            assert torch.equal(ops.fused_linear(x, w, b, r, act), got['y'])
+        x, w, b, r, gy = linear_case(rows, cout, cin, dtype, act, False, res)
+        got = run_linear(x, w, b, r, gy, act)
+        want = plain.linear(x, w, b, r, act, gy)
+        want.pop('gb')
+        hold(got, want)
+        again = run_linear(x, w, b, r, gy, act)
+        assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_linear_few_rows_and_small_problems(dtype):
+    """One to eight rows, with everything an epilogue has; weights and inputs off 16 bytes; rows that leave
+    the kernels for few of them and for small problems."""
+    big, = tensors(7, dtype, (700, 300))
+    for rows in (1, 2, 3, 4, 5, 8, 9, 33, 640):
+        for cin, cout in ((1, 33), (96, 200), (257, 31), (264, 4801 if rows == 3 else 64)):
+            x, w, b, r, gy = linear_case(rows, cin, cout, dtype, None, True, True, seed=rows)
+            for act in (None, 'relu', 'gelu'):
+                got = run_linear(x, w, b, r, gy, act)
+                hold(got, plain.linear(x, w, b, r, act, gy))
+                with torch.no_grad():
+                    assert torch.equal(ops.fused_linear(x, w, b, r, act), got['y'])
+            if cin == 257:
+                x = big[:rows, 3:3 + cin]
+                hold(run_linear(x, w, b, r, gy, 'gelu'), plain.linear(x, w, b, r, 'gelu', gy))
+                x = big[:rows, 8:8 + cin]      # rows on 16 bytes whose length is odd
+                hold(run_linear(x, w, None, r, gy, 'relu'),
+                     {k: v for k, v in plain.linear(x, w, None, r, 'relu', gy).items() if k != 'gb'})
+
+
 def test_first_call_of_a_thread():
     """A new thread has no CUDA context bound to it; a call that allocates nothing binds none before the
     tensor maps are encoded."""
