@@ -85,25 +85,32 @@ __device__ __forceinline__ void load_param(const void *p, bool f32, long long at
   }
 }
 
-// Sums of N values over the G threads of a group; every thread gets them.
+// Sums of N values over the G threads of a group; every thread gets them.  A group of several warps meets on
+// a barrier of its own.
+template <int G>
+__device__ __forceinline__ void group_barrier() {
+  if constexpr (G >= kThreads) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / G), "n"(G) : "memory");
+}
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float *smem) {
+  static_assert(N <= 2, "a warp's place in smem");
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
+  for (int d = (G < 32 ? G : 32) / 2; d > 0; d >>= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
   if constexpr (G > 32) {
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();   // the values of an earlier call have been read
+    const int warp = threadIdx.x >> 5, first = (int)threadIdx.x / G * (G / 32);
+    group_barrier<G>();   // the values of an earlier call have been read
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) smem[warp * N + i] = v[i];
-    __syncthreads();
+      for (int i = 0; i < N; ++i) smem[warp * 2 + i] = v[i];   // a warp's place is the same for every N: groups do not wait for one another
+    group_barrier<G>();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < G / 32; ++w) v[i] += smem[w * N + i];
+      for (int w = 0; w < G / 32; ++w) v[i] += smem[(first + w) * 2 + i];
     }
   }
 }
@@ -119,15 +126,38 @@ struct NormArgs {
   float eps;
 };
 
+// A thread's part of a row as it lies in memory.
+template <typename T, int V, int NV>
+struct Loads {
+  uint4 q[V == 1 ? 1 : NV];
+  T e[V == 1 ? NV : 1];
+  template <int G>
+  __device__ __forceinline__ void get(const T *p, int t, int cols) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + t) * V;
+      if (c < cols) {
+        if constexpr (V == 1) e[i] = p[c];
+        else q[i] = *reinterpret_cast<const uint4 *>(p + c);
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(int i, float (&o)[V]) const {
+    if constexpr (V == 1) o[0] = ElemOf<T>::to(e[i]);
+    else load_vec<T, V>(reinterpret_cast<const T *>(&q[i]), o);
+  }
+};
+
 template <typename T, int V, int E, int G>
 __global__ void __launch_bounds__(kThreads) norm_forward(const NormArgs a) {
   constexpr int NV = E / V;
-  __shared__ float red[(G > 32 ? G / 32 : 1) * 2];
+  __shared__ float red[kThreads / 32 * 2];
   const int t = threadIdx.x % G;
-  const long long row = blockIdx.x * (long long)(kThreads / G) + threadIdx.x / G;
+  long long row = blockIdx.x * (long long)(kThreads / G) + threadIdx.x / G;
   pdl_wait();
   pdl_launch();
-  if (row >= a.rows) return;   // whole groups leave together
+  const bool live = row < a.rows;   // a warp may hold several rows: all lanes go through the sums
+  if (!live) row = a.rows - 1;
   const T *x = (const T *)a.x + row * a.ldx;
   float v[NV][V];
   float s[1] = {0.f};
@@ -158,6 +188,7 @@ __global__ void __launch_bounds__(kThreads) norm_forward(const NormArgs a) {
   const float corr = q[0] * inv;
   const float rstd = 1.f / sqrtf(fmaxf(q[1] * inv - corr * corr, 0.f) + a.eps);
   // fmaxf drops a NaN; m carries it into every element of the row all the same
+  if (!live) return;
   T *y = (T *)a.y + row * a.cols;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -178,28 +209,41 @@ __global__ void __launch_bounds__(kThreads) norm_forward(const NormArgs a) {
   }
 }
 
+// Blocks that share an SM: a thread holds 4 E sums and values and the loads of its next row.
+template <int V, int E>
+constexpr int kResident = E <= 8 ? 3 : V > 1 && E <= 16 ? 2 : 1;
+
 template <typename T, int V, int E, int G, bool kParams>
-__global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kResident<V, E>) norm_backward(const NormArgs a) {
   constexpr int NV = E / V, RPB = kThreads / G;
-  __shared__ float red[(G > 32 ? G / 32 : 1) * 2];
-  __shared__ float cols_s[G > 32 ? 1 : 2 * G * E];
+  constexpr bool kAhead = V > 1 && E <= 16;   // the next row's loads run under this row's sums
+  __shared__ float red[kThreads / 32 * 2];
+  __shared__ float cols_s[kParams && RPB > 1 ? RPB * 2 * G * E : 1];
   const int t = threadIdx.x % G;
   const float inv = 1.f / (float)a.cols;
   float gw[kParams ? NV : 1][V] = {}, gb[kParams ? NV : 1][V] = {};
   pdl_wait();
   pdl_launch();
-  for (long long row = blockIdx.x * (long long)RPB + threadIdx.x / G; row < a.rows; row += (long long)gridDim.x * RPB) {
-    const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * a.ldgy;
+  const T *xs = (const T *)a.x, *gys = (const T *)a.gy;
+  const long long step = (long long)gridDim.x * RPB;
+  Loads<T, V, NV> nx, ng;
+  auto get = [&](long long r) {
+    nx.template get<G>(xs + r * a.ldx, t, a.cols);
+    ng.template get<G>(gys + r * a.ldgy, t, a.cols);
+  };
+  long long row = blockIdx.x * (long long)RPB + threadIdx.x / G;
+  if (kAhead && row < a.rows) get(row);
+  for (; row < a.rows; row += step) {
+    if (!kAhead) get(row);
+    const float m = a.stats[row], corr = a.stats[a.rows + row], rstd = a.stats[2 * a.rows + row];
     float n[NV][V], g[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + t) * V;
-      if (c < a.cols) {
-        load_vec<T, V>(x + c, n[i]);
-        load_vec<T, V>(gy + c, g[i]);
+    for (int i = 0; i < NV; ++i)
+      if ((i * G + t) * V < a.cols) {
+        nx.unpack(i, n[i]);
+        ng.unpack(i, g[i]);
       }
-    }
-    const float m = a.stats[row], corr = a.stats[a.rows + row], rstd = a.stats[2 * a.rows + row];
+    if (kAhead && row + step < a.rows) get(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -220,9 +264,9 @@ __global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
         }
       }
     }
-    group_sum<G>(s, red);
-    const float mg = s[0] * inv, mgn = s[1] * inv;
     if (a.y) {
+      group_sum<G>(s, red);
+      const float mg = s[0] * inv, mgn = s[1] * inv;
       T *gx = (T *)a.y + row * a.cols;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -235,9 +279,10 @@ __global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
       }
     }
   }
+  static_assert(G >= 32, "whole warps leave the loop together");
   if constexpr (kParams) {
     float *out = a.part + (long long)blockIdx.x * 2 * a.cols;
-    if constexpr (G > 32) {
+    if constexpr (RPB == 1) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * G + t) * V;
@@ -249,21 +294,24 @@ __global__ void __launch_bounds__(kThreads) norm_backward(const NormArgs a) {
           }
       }
     } else {
-      for (int w = 0; w < RPB; ++w) {   // the warps in order
-        if (threadIdx.x / G == w)
+      float *mine = cols_s + threadIdx.x / G * (2 * G * E);
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const int at = (i * G + t) * V + e;
-              cols_s[at] = gw[i][e] + (w ? cols_s[at] : 0.f);
-              cols_s[G * E + at] = gb[i][e] + (w ? cols_s[G * E + at] : 0.f);
-            }
-        __syncthreads();
-      }
+        for (int e = 0; e < V; ++e) {
+          mine[(i * G + t) * V + e] = gw[i][e];
+          mine[G * E + (i * G + t) * V + e] = gb[i][e];
+        }
+      __syncthreads();
       for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-        out[c] = cols_s[c];
-        out[a.cols + c] = cols_s[G * E + c];
+        float sw = 0.f, sb = 0.f;
+#pragma unroll
+        for (int q = 0; q < RPB; ++q) {   // the groups in order
+          sw += cols_s[q * 2 * G * E + c];
+          sb += cols_s[q * 2 * G * E + G * E + c];
+        }
+        out[c] = sw;
+        out[a.cols + c] = sb;
       }
     }
   }
@@ -361,8 +409,10 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
   pdl_launch();
   if (!out) return;
   float v = 0.f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int p = ty; p < parts; p += 32) v += part[((long long)p * 2 + blockIdx.y) * cols + c];
+  }
   s[ty][tx] = v;
   __syncthreads();
   for (int d = 16; d > 0; d >>= 1) {
@@ -373,28 +423,60 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
 }
 
 template <typename T, int V, int E, int G>
-cudaError_t run_one(const NormArgs &a, bool backward, bool params, int grid, cudaStream_t s) {
-  if (!backward) return launch_pdl(norm_forward<T, V, E, G>, grid, kThreads, 0, s, 1, a);
-  if (params) return launch_pdl(norm_backward<T, V, E, G, true>, grid, kThreads, 0, s, 1, a);
-  return launch_pdl(norm_backward<T, V, E, G, false>, grid, kThreads, 0, s, 1, a);
+cudaError_t run_forward(const NormArgs &a, cudaStream_t s) {
+  constexpr int rpb = kThreads / G;
+  return launch_pdl(norm_forward<T, V, E, G>, (unsigned)((a.rows + rpb - 1) / rpb), kThreads, 0, s, 1, a);
+}
+template <typename T, int V, int E, int G>
+cudaError_t run_backward(const NormArgs &a, bool params, int *parts, cudaStream_t s) {
+  constexpr int rpb = kThreads / G, most = 148 * kResident<V, E>;
+  static_assert(most <= kMaxPartials, "the workspace");
+  const long long blocks = (a.rows + rpb - 1) / rpb;
+  *parts = (int)(blocks < most ? blocks : most);
+  if (params) return launch_pdl(norm_backward<T, V, E, G, true>, *parts, kThreads, 0, s, 1, a);
+  return launch_pdl(norm_backward<T, V, E, G, false>, *parts, kThreads, 0, s, 1, a);
 }
 
-// E: the fewest elements to a thread that hold the row; G: a warp while that is at most 32.
+// Elements to a thread and threads to a row.
+//
+// Forward: two loads of 16 bytes while that keeps a row within a warp (35642 x 64 bf16: 3.9 us against 11.3 us
+// with a warp to each row; 35642 x 256 bf16: 9.5 us, with one load 11.5, with four 10.6), 32 elements beyond
+// (20000 x 768 bf16 16.8 us, with two loads 20.3; 5000 x 1536 10.0 us, with one load 13.8).  Keeping the
+// parameters in registers over several rows, with the next row's loads ahead, was slower everywhere
+// (35642 x 256 fp32 25 us against 11.6).  One element at a time: a warp's lanes side by side, for the sake of
+// whole sectors.
+//
+// Backward: 8 elements and a fixed set of blocks, so that the sums for gw and gb leave room for several rows
+// at once on an SM (20000 x 768 bf16 41 us, with 32 elements 78); the same without those sums, so that gx
+// does not depend on what else is wanted.
 template <typename T, int V>
 cudaError_t run_rows(const NormArgs &a, bool backward, bool params, int *parts, cudaStream_t s) {
-  const int G = a.cols <= 1024 ? 32 : 256, E = (a.cols + G - 1) / G;
-  const long long rpb = kThreads / G;
-  long long grid = (a.rows + rpb - 1) / rpb;
-  if (backward && grid > kMaxPartials) grid = kMaxPartials;
-  *parts = (int)grid;
-  if (G == 32) {
-    if (E <= 8) return run_one<T, V, 8, 32>(a, backward, params, (int)grid, s);
-    if (E <= 16) return run_one<T, V, 16, 32>(a, backward, params, (int)grid, s);
-    return run_one<T, V, 32, 32>(a, backward, params, (int)grid, s);
+  const int cols = a.cols;
+  if (backward) {
+    if (cols <= 256) return run_backward<T, V, 8, 32>(a, params, parts, s);
+    if (cols <= 512) return run_backward<T, V, 8, 64>(a, params, parts, s);
+    if (cols <= 1024) return run_backward<T, V, 8, 128>(a, params, parts, s);
+    if (cols <= 2048) return run_backward<T, V, 8, 256>(a, params, parts, s);
+    if (cols <= 4096) return run_backward<T, V, 16, 256>(a, params, parts, s);
+    return run_backward<T, V, 32, 256>(a, params, parts, s);
   }
-  if (E <= 8) return run_one<T, V, 8, 256>(a, backward, params, (int)grid, s);
-  if (E <= 16) return run_one<T, V, 16, 256>(a, backward, params, (int)grid, s);
-  return run_one<T, V, 32, 256>(a, backward, params, (int)grid, s);
+  if constexpr (V > 1) {
+    constexpr int E = 2 * V;
+    if (cols <= 4 * E) return run_forward<T, V, E, 4>(a, s);
+    if (cols <= 8 * E) return run_forward<T, V, E, 8>(a, s);
+    if (cols <= 16 * E) return run_forward<T, V, E, 16>(a, s);
+    if (cols <= 32 * E) return run_forward<T, V, E, 32>(a, s);
+    if (cols <= 1024) return run_forward<T, V, 32, 32>(a, s);
+    if (cols <= 2048) return run_forward<T, V, 32, 64>(a, s);
+    if (cols <= 4096) return run_forward<T, V, 32, 128>(a, s);
+  } else {
+    if (cols <= 256) return run_forward<T, V, 8, 32>(a, s);
+    if (cols <= 512) return run_forward<T, V, 16, 32>(a, s);
+    if (cols <= 1024) return run_forward<T, V, 32, 32>(a, s);
+    if (cols <= 2048) return run_forward<T, V, 8, 256>(a, s);
+    if (cols <= 4096) return run_forward<T, V, 16, 256>(a, s);
+  }
+  return run_forward<T, V, 32, 256>(a, s);
 }
 
 template <typename T>
