@@ -368,8 +368,8 @@ int dcn_msda_backward(const void *value, const int64_t *spatial_shapes, const in
  * saved (may be NULL): what the activation's derivative needs, for dcn_linear_backward.
  *   RELU  uint32 words [rows][(cout + 31) / 32]; bit j % 32 of word j / 32 is set where the
  *         pre-activation is not <= 0;
- *   GELU  the pre-activation, [rows][(cout + 7) / 8 * 8], 16-byte aligned: fp32 for fp32 tensors, fp16
- *         for both 16-bit types (finer than bf16; the derivative is 0 or 1 where fp16 overflows);
+ *   GELU  the derivative Phi(z) + z phi(z), [rows][(cout + 7) / 8 * 8], 16-byte aligned: fp32 for fp32
+ *         tensors, for 16-bit ones uint16 codes (derivative * 2^15 + 2^13 rounded, 65535: NaN);
  *   NONE  not written.
  *
  * dcn_linear_backward, from gy = dL/dy [rows, cout] (row stride ldgy) and gz = gy * act'(z):

@@ -19,6 +19,27 @@ struct GemmPlan {
 };
 GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weight_gradient);
 
+// 16 bytes of kept derivatives (of tensors of type T) as floats
+template <typename T>
+__device__ __forceinline__ void unpack_slopes(const uint4 &u, float *v) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(w[i]);
+    } else {
+      v[2 * i] = slope_of_low(w[i]);
+      v[2 * i + 1] = slope_of_high(w[i]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void keep_slope(void *saved, long long at, float slope) {
+  if constexpr (sizeof(T) == 4) ((float *)saved)[at] = slope;
+  else ((uint16_t *)saved)[at] = (uint16_t)slope_code(slope);
+}
+
 // One launch of the tensor-core kernel.
 struct alignas(64) GemmTc {
   CUtensorMap a, b, out, res, aux;
@@ -30,7 +51,7 @@ struct alignas(64) GemmTc {
   int stages;
   int out_tma, res_tma;            // 0: element by element
   int bias16;                      // the bias starts on 16 bytes
-  long long ldz;                   // row stride of kept pre-activations: a multiple of 8
+  long long ldz;                   // row stride of kept derivatives: a multiple of 8
   float *row_part;                 // [splits][m], with splits > 1
   unsigned long long wait_limit_ns;
 };

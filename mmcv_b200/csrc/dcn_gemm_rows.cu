@@ -6,8 +6,6 @@
 // each lane gives away the half that its partner keeps.  A block has 32 columns, so that it owns whole
 // words of relu's kept bits.  Bound: memory (the weight), or the launch.
 // Measured against the tensor-core kernel (its tiles are 128 rows): see run_rows.
-#include <type_traits>
-
 #include "dcn_gemm.cuh"
 
 namespace dcn {
@@ -96,16 +94,15 @@ __global__ void __launch_bounds__(1024 / NC) dcn_linear_rows(const GemmArgs g) {
   }
   const int idx = lane / (32 / N), c = idx / R, r = idx % R, j = j0 + c;
   if (lane % (32 / N) == 0 && j < n && r < m) {
-    constexpr bool kExact = sizeof(T) == 4;
-    using Z = std::conditional_t<sizeof(T) == 4, float, __half>;
+    constexpr bool kFine = sizeof(T) == 4;
     float v = acc[0];
     if (g.bias) v += ElemOf<T>::to(((const T *)g.bias)[j]);
     if (g.act == DCN_ACT_RELU) {
       if (keep_bits && relu_bit(v)) atomicOr(&bits[r], 1u << (j & 31));
       v = relu_value(v);
     } else if (g.act == DCN_ACT_GELU) {
-      if (g.saved) ((Z *)g.saved)[r * ((g.n + 7) / 8 * 8) + j] = ElemOf<Z>::from(v);
-      v = gelu_value<kExact>(v);
+      if (g.saved) keep_slope<T>(g.saved, r * ((g.n + 7) / 8 * 8) + j, gelu_slope<kFine>(v));
+      v = gelu_value<kFine>(v);
     }
     if (g.res) v += ElemOf<T>::to(((const T *)g.res)[r * g.ldr + j]);
     ((T *)g.out)[r * g.n + j] = ElemOf<T>::from(v);

@@ -10,8 +10,6 @@
 // take 16 of them each, 4 x 4 results to a thread, and are added in order at the end.  The next 64 values
 // are in registers while these are multiplied.  Bound: the shared-memory reads and FMAs of the 4 x 4 step;
 // with few tiles, the chain of loads.
-#include <type_traits>
-
 #include "dcn_gemm.cuh"
 
 namespace dcn {
@@ -19,15 +17,14 @@ namespace {
 
 constexpr int kTile = 32, kStep = 64, kPitch = kTile + 4;   // (k + i) pitch: 16-byte rows, no bank conflicts
 
-template <typename T>
-using Kept = std::conditional_t<sizeof(T) == 4, float, __half>;   // gelu's pre-activations
-
 // act'(z) from what the forward pass kept at [r, c] of [rows, cols]
 template <typename T>
 __device__ __forceinline__ float slope_at(const void *saved, int act, long long r, long long c, long long cols) {
   if (act == DCN_ACT_RELU)
     return (((const uint32_t *)saved)[r * ((cols + 31) / 32) + (c >> 5)] >> (c & 31)) & 1u ? 1.f : 0.f;
-  return gelu_slope<sizeof(T) == 4>(ElemOf<Kept<T>>::to(((const Kept<T> *)saved)[r * ((cols + 7) / 8 * 8) + c]));
+  const long long at = r * ((cols + 7) / 8 * 8) + c;
+  if constexpr (sizeof(T) == 4) return ((const float *)saved)[at];
+  else return slope_of_low(((const uint16_t *)saved)[at]);
 }
 // g * act'(z); relu drops g where the bit is off, whatever g is
 template <typename T>
@@ -149,7 +146,7 @@ __device__ void tile_product(const SimtJob &p, int tile, float *smem) {
       }
       v = relu_value(v);
     } else if (g.act == DCN_ACT_GELU) {
-      if (g.saved && in) ((Kept<T> *)g.saved)[i * ((g.n + 7) / 8 * 8) + j] = ElemOf<Kept<T>>::from(v);
+      if (g.saved && in) keep_slope<T>(g.saved, i * ((g.n + 7) / 8 * 8) + j, gelu_slope<sizeof(T) == 4>(v));
       v = gelu_value<sizeof(T) == 4>(v);
     }
     if (!in) continue;
@@ -172,7 +169,7 @@ __device__ void tile_product(const SimtJob &p, int tile, float *smem) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dcn_gemm_simt(const SimtJobs jobs) {
+__global__ void __launch_bounds__(256) dcn_gemm_simt(const __grid_constant__ SimtJobs jobs) {
   __shared__ __align__(16) float smem[2 * kStep * kPitch];
   static_assert(2 * kStep * kPitch >= 4 * kTile * kTile, "the groups' results");
   pdl_wait();

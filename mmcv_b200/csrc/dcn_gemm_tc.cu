@@ -2,7 +2,6 @@
 // element-wise pass that writes operand planes, and the ordered sums of split results.
 #include <atomic>
 #include <cstring>
-#include <type_traits>
 
 #include <cuda.h>
 
@@ -12,21 +11,33 @@ namespace dcn {
 
 namespace {
 
-// out[i, j] = sum over the ranges of part [splits][m][ldp], in order; four columns a thread
+// out[i, j] = sum over the ranges of part [splits][m][ldp]: a thread has four columns and, in a block cut into
+// `groups`, every groups-th range; the groups are joined in order
 template <typename T>
 __global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__ part, int splits, long long m,
-                                                       long long n, long long ldp, T *__restrict__ out) {
-  const long long per_row = ldp / 4, idx = blockIdx.x * 256LL + threadIdx.x;
+                                                       long long n, long long ldp, int groups, T *__restrict__ out) {
+  __shared__ float4 join[256];
+  const int across = 256 / groups, group = threadIdx.x / across;
+  const long long per_row = ldp / 4, idx = blockIdx.x * (long long)across + (threadIdx.x - group * across);
+  const bool live = idx < m * per_row;
   pdl_wait();
   pdl_launch();
-  if (idx >= m * per_row) return;
   const long long i = idx / per_row, j = (idx - i * per_row) * 4;
-  const float4 *p = reinterpret_cast<const float4 *>(part + i * ldp + j);
-  const long long step = m * ldp / 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    const float4 *p = reinterpret_cast<const float4 *>(part + i * ldp + j);
+    const long long step = m * ldp / 4;
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float4 a = p[s * step];
+    for (int s = group; s < splits; s += groups) {
+      const float4 a = p[s * step];
+      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+    }
+  }
+  join[threadIdx.x] = v;
+  __syncthreads();
+  if (group || !live) return;
+  for (int k = 1; k < groups; ++k) {
+    const float4 a = join[k * across + threadIdx.x];
     v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
   }
   T *o = out + i * n + j;
@@ -70,10 +81,12 @@ __device__ __forceinline__ void split3(float x, uint32_t (&b)[3]) {
   if (x != x) b[0] |= 0x00400000u;
 }
 
+constexpr int kStageResident = 3;   // blocks that share an SM: two rows a thread in flight take 80 registers
+
 // The operands of a pass in one launch, a range of blocks each.  In a block, a power of two of threads of
 // 8 columns each, the rest side by side on rows; a slab of blocks takes every gy-th group of rows.
 template <typename T, int PL>
-__global__ void __launch_bounds__(256) dcn_gemm_stage(const StageJobs jobs) {
+__global__ void __launch_bounds__(256, kStageResident) dcn_gemm_stage(const __grid_constant__ StageJobs jobs) {
   __shared__ float red[256 * 8];
   const int which = (int)blockIdx.x < jobs.job[1].first ? 0 : (int)blockIdx.x < jobs.job[2].first ? 1 : 2;
   const StageJob &a = jobs.job[which];
@@ -84,64 +97,78 @@ __global__ void __launch_bounds__(256) dcn_gemm_stage(const StageJobs jobs) {
   pdl_wait();
   pdl_launch();
   float sum[8] = {};
-  if (c < a.pitch) {
-    for (long long r = (long long)slab * rows_at_once + ty; r < a.rows; r += (long long)a.gy * rows_at_once) {
-      float v[8];
-      const T *src = (const T *)a.src + r * a.ld + c;
-      if (a.vec_src && c + 8 <= a.cols) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 4);
-          v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-          v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4 *>(src);
-          const T *e = reinterpret_cast<const T *>(&u);
+  constexpr int Q = (int)sizeof(T) / 2;   // 16-byte pieces of 8 elements, and of 8 kept derivatives
+  struct Piece {
+    uint4 v[Q], z[Q];
+    uint32_t bits;
+  };
+  auto load = [&](long long r, Piece &p) {
+    const T *src = (const T *)a.src + r * a.ld + c;
+    if (a.vec_src && c + 8 <= a.cols) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = ElemOf<T>::to(e[i]);
-        }
-      } else {
+      for (int i = 0; i < Q; ++i) p.v[i] = reinterpret_cast<const uint4 *>(src)[i];
+    } else {
+      T *e = reinterpret_cast<T *>(p.v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < a.cols ? ElemOf<T>::to(src[i]) : 0.f;
+      for (int i = 0; i < 8; ++i) e[i] = c + i < a.cols ? src[i] : ElemOf<T>::from(0.f);
+    }
+    if (a.act == DCN_ACT_RELU) {
+      p.bits = c < a.cols ? ((const uint32_t *)a.saved)[r * words + (c >> 5)] >> (c & 31) : 0u;
+    } else if (a.act == DCN_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) p.z[i] = reinterpret_cast<const uint4 *>((const uint8_t *)a.saved + (r * a.pitch + c) * sizeof(T))[i];
+    }
+  };
+  auto finish = [&](long long r, const Piece &p) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ElemOf<T>::to(reinterpret_cast<const T *>(p.v)[i]);
+    if (a.act == DCN_ACT_RELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (p.bits >> i) & 1u ? v[i] : 0.f;
+    } else if (a.act == DCN_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        float z[8 / Q];
+        unpack_slopes<T>(p.z[i], z);
+#pragma unroll
+        for (int k = 0; k < 8 / Q; ++k) v[i * (8 / Q) + k] *= z[k];
       }
-      if (a.act == DCN_ACT_RELU) {
-        const uint32_t bits = c < a.cols ? ((const uint32_t *)a.saved)[r * words + (c >> 5)] >> (c & 31) : 0u;
+    }
+    if constexpr (PL == 1) {
+      uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (bits >> i) & 1u ? v[i] : 0.f;
-      } else if (a.act == DCN_ACT_GELU) {
-        using Z = std::conditional_t<sizeof(T) == 4, float, __half>;
-        const Z *z = (const Z *)a.saved + r * a.pitch + c;   // kept with the same pitch
-        uint4 u[sizeof(Z) / 2];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(Z) / 2; ++i) u[i] = reinterpret_cast<const uint4 *>(z)[i];
-        const Z *e = reinterpret_cast<const Z *>(u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= gelu_slope<PL == 3>(ElemOf<Z>::to(e[i]));
+      for (int i = 0; i < 4; ++i) {
+        T lo = ElemOf<T>::from(v[2 * i]), hi = ElemOf<T>::from(v[2 * i + 1]);
+        w[i] = (uint32_t)*reinterpret_cast<uint16_t *>(&lo) | ((uint32_t)*reinterpret_cast<uint16_t *>(&hi) << 16);
       }
-      if constexpr (PL == 1) {
-        uint32_t w[4];
+      *reinterpret_cast<uint4 *>((T *)a.dst + r * a.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      uint32_t w[3][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          T lo = ElemOf<T>::from(v[2 * i]), hi = ElemOf<T>::from(v[2 * i + 1]);
-          w[i] = (uint32_t)*reinterpret_cast<uint16_t *>(&lo) | ((uint32_t)*reinterpret_cast<uint16_t *>(&hi) << 16);
-        }
-        *reinterpret_cast<uint4 *>((T *)a.dst + r * a.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-        uint32_t w[3][4];
+      for (int i = 0; i < 4; ++i) {
+        uint32_t lo[3], hi[3];
+        split3(v[2 * i], lo);
+        split3(v[2 * i + 1], hi);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t lo[3], hi[3];
-          split3(v[2 * i], lo);
-          split3(v[2 * i + 1], hi);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) w[k][i] = (lo[k] >> 16) | hi[k];
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          *reinterpret_cast<uint4 *>((uint16_t *)a.dst + (k * a.rows + r) * a.pitch + c) =
-              make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        for (int k = 0; k < 3; ++k) w[k][i] = (lo[k] >> 16) | hi[k];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += v[i];
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint4 *>((uint16_t *)a.dst + (k * a.rows + r) * a.pitch + c) =
+            make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += v[i];
+  };
+  if (c < a.pitch) {   // two rows in flight
+    const long long step = (long long)a.gy * rows_at_once;
+    for (long long r = (long long)slab * rows_at_once + ty; r < a.rows; r += 2 * step) {
+      Piece p0, p1;
+      load(r, p0);
+      if (r + step < a.rows) load(r + step, p1);
+      finish(r, p0);
+      if (r + step < a.rows) finish(r + step, p1);
     }
   }
   if (!a.sums) return;
@@ -167,7 +194,7 @@ void stage_shape(long long rows, long long pitch, StageJob *j) {
   const long long x = 1LL << j->log_tx, y = 256 / x;
   j->gx = (int)((pitch + x * 8 - 1) / (x * 8));
   const long long want = (rows + y - 1) / y;
-  long long most = 148 * 8 / j->gx;
+  long long most = 148 * kStageResident / j->gx;
   if (most < 1) most = 1;
   j->gy = (int)(want < 1 ? 1 : want < most ? want : most);
 }
@@ -210,8 +237,12 @@ bool encode3(CUtensorMap *map, CUtensorMapDataType type, int esize, const void *
 template <typename T>
 cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &g, cudaStream_t s) {
   const long long n = g.m * (plan.ldp / 4);
-  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + 255) / 256), 256, 0, s, 1, part, plan.splits, g.m, g.n, plan.ldp,
-                    (T *)g.out);
+  // as many groups as fill the SMs (74 parts of 256 x 256: 5 us, with one group 19)
+  int groups = 1;
+  while (groups < 8 && plan.splits >= 4 * groups && n * groups < 148LL * 4 * 256) groups *= 2;
+  const int across = 256 / groups;
+  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + across - 1) / across), 256, 0, s, 1, part, plan.splits, g.m, g.n,
+                    plan.ldp, groups, (T *)g.out);
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }

@@ -17,7 +17,7 @@
 // into fp32 accumulators in tensor memory, double-buffered so that the epilogue of a tile runs under
 // the main loop of the next; eight warps run the epilogue: tcgen05.ld, bias, activation, derivative,
 // residual, one rounding, a 32-row chunk in shared memory, a tensor store.  The residual arrives by
-// tensor load in the chunk that the result leaves from, as do the kept pre-activations of a derivative.
+// tensor load in the chunk that the result leaves from, as do the kept derivatives of gelu.
 // Sixteen epilogue warps (eight with fp32 tensors) and not four: a warp's share of a tile is a chain of waits (tensor memory,
 // loads, the store of its last chunk), and the products around an embedding of 256 have main loops of
 // four steps only (35642 x 256 x 1024 bf16 with relu: 42 us with eight warps).  Every wait is bounded.
@@ -294,6 +294,20 @@ __device__ __forceinline__ void stage_store(uint8_t *chunk, int row, int q0, con
   }
 }
 
+// the same of gelu's derivatives, as they are kept
+template <typename TO, int RB>
+__device__ __forceinline__ void stage_slopes(uint8_t *chunk, int row, int q0, const float (&v)[32]) {
+  if constexpr (sizeof(TO) == 4) {
+    stage_store<TO, RB>(chunk, row, q0, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4 *>(chunk + chunk_piece<RB>(row, q0 + q)) =
+          make_uint4(slope_codes(v[8 * q], v[8 * q + 1]), slope_codes(v[8 * q + 2], v[8 * q + 3]),
+                     slope_codes(v[8 * q + 4], v[8 * q + 5]), slope_codes(v[8 * q + 6], v[8 * q + 7]));
+  }
+}
+
 // v[0..31] += bias[j1 ..]; whole groups of a bias that starts on 16 bytes by 16-byte loads (the same
 // address in every lane)
 template <typename TO>
@@ -396,9 +410,6 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   constexpr int RB = kChunkRow<TO, BN>, kChunkBytes = 32 * RB;
   constexpr int CW = RB / (int)sizeof(TO);             // columns of a staging chunk
   constexpr int kWarpCols = BN / kGroups > CW ? BN / kGroups : CW;   // columns of an epilogue warp
-  // Kept pre-activations of 16-bit tensors are fp16 whatever the tensors' type: eight times finer than bf16
-  // within +-65504, and gelu's derivative is 0 or 1 beyond +-40, an infinity's too.
-  using TZ = std::conditional_t<sizeof(TO) == 4, float, __half>;
 
   const GemmArgs &g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -598,17 +609,68 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
         if (g.bias) add_bias<TO>((const TO *)g.bias, j1, n, p.bias16 != 0, v);
       };
       static_assert(PL == 1 || kWarpCols <= 64, "two groups");
+      // all read: the next tile may have the accumulator
+      auto accumulator_free = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
+      };
+      auto chunk_leaves = [&](int j0) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (!p.out_tma) {
+          chunk_out<TO, RB>(chunk, (TO *)g.out, n, i0, m, j0, n, lane);
+          __syncwarp();
+        } else if (lane == 0) {
+          tma_store_3d(&p.out, chunk_u, j0, i0, walk.sp);
+          bulk_commit();
+        }
+      };
 #pragma unroll 1
       for (int ch = 0; ch < chunks; ++ch) {
         const int j0 = jw + ch * CW;
         if (takes && ch) fetch(j0);
-        if (aux_out) {   // the pre-activations leave first, through the same chunk
+        if constexpr (EPI == kEpiGelu && PL == 1) {
+          if (aux_out && !g.res) {   // derivatives and values at once; the values wait in registers
+            uint32_t keep[CW / 32][16];
+            chunk_free();
+#pragma unroll
+            for (int c1 = 0; c1 < CW; c1 += 32) {
+              float v[32], slope[32];
+              sums(j0 + c1, ch * CW + c1, v);
+              if (ch == chunks - 1 && c1 == CW - 32) accumulator_free();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                gelu_both<false>(v[j], v[j + 1], slope[j], slope[j + 1]);
+                keep[c1 / 32][j / 2] = pack2<TO, false>(v[j], v[j + 1]);
+              }
+              stage_slopes<TO, RB>(chunk, lane, c1 * (int)sizeof(TO) / 16, slope);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&p.aux, chunk_u, j0, i0, 0);
+              bulk_commit();
+            }
+            chunk_free();
+#pragma unroll
+            for (int q = 0; q < CW / 8; ++q)
+              *reinterpret_cast<uint4 *>(chunk + chunk_piece<RB>(lane, q)) =
+                  make_uint4(keep[q / 4][q % 4 * 4], keep[q / 4][q % 4 * 4 + 1], keep[q / 4][q % 4 * 4 + 2],
+                             keep[q / 4][q % 4 * 4 + 3]);
+            chunk_leaves(j0);
+            continue;
+          }
+        }
+        if (aux_out) {   // the derivatives leave first, through the same chunk
           chunk_free();
 #pragma unroll 1
           for (int c1 = 0; c1 < CW; c1 += 32) {
             float v[32];
             sums(j0 + c1, ch * CW + c1, v);
-            stage_store<TZ, RB>(chunk, lane, c1 * (int)sizeof(TZ) / 16, v);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) gelu_slopes<PL == 3>(v[j], v[j + 1]);
+            stage_slopes<TO, RB>(chunk, lane, c1 * (int)sizeof(TO) / 16, v);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -628,11 +690,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           float v[32];
           sums(j1, ch * CW + c1, v);
           if constexpr (PL == 1) {
-            if (ch == chunks - 1 && c1 == CW - 32) {   // all read: the next tile may have the accumulator
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
-            }
+            if (ch == chunks - 1 && c1 == CW - 32) accumulator_free();
           }
           if (c1 == 0 && !takes) chunk_free();
           constexpr int E = 16 / (int)sizeof(TO);
@@ -649,7 +707,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
             }
           } else if constexpr (EPI == kEpiGelu) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = gelu_value<PL == 3>(v[j]);
+            for (int j = 0; j < 32; j += 2) gelu_values<PL == 3>(v[j], v[j + 1]);
           } else if constexpr (EPI == kEpiSlopeRelu) {
             const uint32_t bits =
                 row < m && j1 < n ? __ldg((const uint32_t *)g.slope + (long long)row * words + (j1 >> 5)) : 0u;
@@ -659,9 +717,9 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
 #pragma unroll
             for (int k = 0; k < 32 / E; ++k) {
               float z[E];
-              unpack16<TZ>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), z);
+              unpack_slopes<TO>(*reinterpret_cast<const uint4 *>(chunk + chunk_piece<RB>(lane, q0 + k)), z);
 #pragma unroll
-              for (int j = 0; j < E; ++j) v[E * k + j] *= gelu_slope<PL == 3>(z[j]);
+              for (int j = 0; j < E; ++j) v[E * k + j] *= z[j];
             }
           }
           if (res_staged) {
@@ -688,22 +746,10 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
             }
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (!p.out_tma) {
-          chunk_out<TO, RB>(chunk, (TO *)g.out, n, i0, m, j0, n, lane);
-          __syncwarp();
-        } else if (lane == 0) {
-          tma_store_3d(&p.out, chunk_u, j0, i0, walk.sp);
-          bulk_commit();
-        }
+        chunk_leaves(j0);
       }
       if constexpr (PL == 1) {
-        if (!chunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) lead_arrive<CG>(lead_empty + 8 * buf);
-        }
+        if (!chunks) accumulator_free();
       }
     }
     if (lane == 0) bulk_wait_all();

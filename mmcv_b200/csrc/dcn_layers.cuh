@@ -54,44 +54,131 @@ template <> struct ElemOf<__half> {
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
 };
 
-// Phi(z) = 0.5 * (1 + erf(z / sqrt 2)) and phi(z), the normal distribution function and density.
+// Phi and phi: the normal distribution function and density.  gelu(z) = z Phi(z), its derivative
+// Phi(z) + z phi(z).
 //
-// kExact (fp32 tensors): through erfcf, so that the lower tail keeps its relative accuracy.
-// Otherwise (16-bit tensors): erfc(x) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2),
-// t = 1 / (1 + p x), x >= 0 (Abramowitz and Stegun 7.1.26, absolute error below 1.5e-7, a fiftieth of
-// half a step of fp16 at 1).  It takes two special-function instructions and a dozen others, and
-// the exponential is the density's too; with erfcf the epilogue of a 128 x 256 tile took longer than
-// 16 steps of its main loop (4096 x 1024 x 2048 fp16 forward: 57 us).
-template <bool kExact>
-__device__ __forceinline__ void normal(float z, float *cdf, float *density) {
-  if constexpr (kExact) {
-    *cdf = 0.5f * erfcf(-0.70710678118654752f * z);
-    *density = 0.39894228040143268f * expf(-0.5f * z * z);
-  } else {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float e = __expf(-x * x);
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                             0.254829592f);
-    const float tail = 0.5f * q * e;   // Phi(-|z|)
-    *cdf = z < 0.f ? tail : 1.f - tail;
-    *density = 0.39894228040143268f * e;
+// fp32 tensors (kFine): Phi(-a) = e^(-a^2 / 2) q(s), s = 1 / (1 + 0.23 a), q a polynomial of degree 8, fitted
+// here (iteratively reweighted least squares on 0 <= a <= 14) for relative error: 5e-8, with fp32's roundings
+// 5e-7, and 7e-8 absolute in a Phi(-a).  With erfcf and expf the epilogue took longer than the product
+// (35642 x 256 x 1024: 245 us, without gelu 108).
+//
+// 16-bit tensors: Phi(-a) = 2^p(a), a = |z|, p a polynomial of degree 7, fitted here (iteratively reweighted
+// least squares on [0, 6]) so that the error of a Phi(-a) is a fixed share of half a step of fp16: at most
+// 0.0073 of it, 9.3e-7 absolute; beyond 6 p falls to -274 at 20, where a is cut off.  Then
+// gelu(z) = max(z, 0) - a Phi(-a): one special-function instruction and, two elements at a time, four and a
+// half multiply-adds an element, no branch and no cancellation.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (x0, x1) * (y0, y1) + (z, z), each rounded to nearest
+__device__ __forceinline__ void fma2(float &x0, float &x1, float y0, float y1, float z) {
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "mov.b64 c, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y0), "f"(y1), "f"(z));
+}
+// Phi(-a0), Phi(-a1), 0 <= a <= 20
+template <bool kFine>
+__device__ __forceinline__ void tails(float a0, float a1, float &t0, float &t1) {
+  if constexpr (kFine) {
+    constexpr float c[9] = {-2.7761721867136657e-05f, 0.09237844496965408f, 0.08576300740242004f, 0.11951372772455215f,
+                            -0.032919447869062424f, 0.3014717698097229f, -0.2781260907649994f, 0.2904137372970581f,
+                            -0.07846737653017044f};
+    float s0, s1;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(fmaf(a0, 0.23f, 1.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(fmaf(a1, 0.23f, 1.f)));
+    t0 = t1 = c[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) fma2(t0, t1, s0, s1, c[i]);
+    t0 *= exp2_approx(-0.72134752044448170f * (a0 * a0));
+    t1 *= exp2_approx(-0.72134752044448170f * (a1 * a1));
+    return;
   }
+  constexpr float c[8] = {-0.9999973773956299f, -1.151201844215393f, -0.4586567282676697f, -0.053682103753089905f,
+                          0.008319714106619358f, -0.0008661015890538692f, 5.079910988570191e-05f,
+                          -1.131071940108086e-06f};
+  t0 = t1 = c[7];
+#pragma unroll
+  for (int i = 6; i >= 0; --i) fma2(t0, t1, a0, a1, c[i]);
+  t0 = exp2_approx(t0);
+  t1 = exp2_approx(t1);
 }
-template <bool kExact>
+__device__ __forceinline__ float relu_value(float z);
+// z clipped to +-20, a NaN kept
+__device__ __forceinline__ float clip20(float z) {
+  float v;
+  asm("min.NaN.f32 %0, %1, 0f41A00000;\n\tmax.NaN.f32 %0, %0, 0fC1A00000;" : "=f"(v) : "f"(z));
+  return v;
+}
+__device__ __forceinline__ float slope_from(float clipped, float tail) {
+  const float density = 0.39894228040143268f * exp2_approx(-0.72134752044448170f * clipped * clipped);
+  return fmaf(clipped, density, clipped > 0.f ? 1.f - tail : tail);
+}
+
+// Two values of gelu; two derivatives; both (s: the derivatives).
+template <bool kFine>
+__device__ __forceinline__ void gelu_values(float &v0, float &v1) {
+  const float a0 = fminf(fabsf(v0), 20.f), a1 = fminf(fabsf(v1), 20.f);
+  float t0, t1;
+  tails<kFine>(a0, a1, t0, t1);
+  v0 = fmaf(-a0, t0, relu_value(v0));
+  v1 = fmaf(-a1, t1, relu_value(v1));
+}
+template <bool kFine>
+__device__ __forceinline__ void gelu_both(float &v0, float &v1, float &s0, float &s1) {
+  const float c0 = clip20(v0), c1 = clip20(v1);
+  float t0, t1;
+  tails<kFine>(fabsf(c0), fabsf(c1), t0, t1);
+  v0 = fmaf(-fabsf(c0), t0, relu_value(v0));
+  v1 = fmaf(-fabsf(c1), t1, relu_value(v1));
+  s0 = slope_from(c0, t0);
+  s1 = slope_from(c1, t1);
+}
+template <bool kFine>
+__device__ __forceinline__ void gelu_slopes(float &v0, float &v1) {
+  const float c0 = clip20(v0), c1 = clip20(v1);
+  float t0, t1;
+  tails<kFine>(fabsf(c0), fabsf(c1), t0, t1);
+  v0 = slope_from(c0, t0);
+  v1 = slope_from(c1, t1);
+}
+template <bool kFine>
 __device__ __forceinline__ float gelu_value(float z) {
-  float cdf, density;
-  normal<kExact>(z, &cdf, &density);
-  // far out z * Phi(z) is -inf * 0; below -40 nothing is left of it in any type
-  return z < -40.f ? -0.f : z * cdf;
+  float other = z;
+  gelu_values<kFine>(z, other);
+  return z;
 }
-// d gelu / dz = Phi(z) + z phi(z)
-template <bool kExact>
+template <bool kFine>
 __device__ __forceinline__ float gelu_slope(float z) {
-  float cdf, density;
-  normal<kExact>(z, &cdf, &density);
-  return fabsf(z) > 40.f ? (z > 0.f ? 1.f : 0.f) : fmaf(z, density, cdf);
+  float other = z;
+  gelu_slopes<kFine>(z, other);
+  return z;
 }
+
+// What is kept of gelu for the backward pass: the derivative.  fp32 tensors keep it as it is.  For 16-bit ones
+// it is a fixed-point number of 16 bits, 2^-15 a step from -0.25 (it lies in -0.13 .. 1.13; 0 and 1 are exact):
+// within 1.6e-5, an eighth of half a step of fp16 at 1, for one instruction each way instead of the
+// derivative's twenty in the backward pass.  65535 stands for NaN.
+//
+// 1.5 * 2^23 + q has q in the low bits of its pattern; a NaN comes out of the multiply-add as 0x7fffffff.
+__device__ __forceinline__ uint32_t slope_code(float slope) {
+  return __float_as_uint(fmaf(slope, 32768.f, 12582912.f + 8192.f));   // the code: the low 16 bits
+}
+__device__ __forceinline__ uint32_t slope_codes(float lo, float hi) {
+  return __byte_perm(slope_code(lo), slope_code(hi), 0x5410);
+}
+__device__ __forceinline__ float slope_of(uint32_t pattern) {
+  const float v = fmaf(__uint_as_float(pattern), 1.f / 32768.f, -384.25f);   // exact
+  return v > 1.5f ? __uint_as_float(0x7fffffffu) : v;
+}
+__device__ __forceinline__ float slope_of_low(uint32_t codes) { return slope_of(__byte_perm(codes, 0x4B400000u, 0x7610)); }
+__device__ __forceinline__ float slope_of_high(uint32_t codes) { return slope_of(__byte_perm(codes, 0x4B400000u, 0x7632)); }
 // A NaN stays a NaN.
 __device__ __forceinline__ float relu_value(float z) {
   float v;

@@ -44,7 +44,7 @@ bool needs_stage(int dtype, int64_t alignment) { return dtype == DCN_DTYPE_F32 |
 //   dcn_linear_rows   1 x 256 x 1024 bf16 2.0 / 4.5, fp32 2.2 / 10.1; 4 x 1024 x 1024 bf16 6.1 / 8.0, fp32
 //                     8.6 / 22; 4 x 4096 x 4096 bf16 20 / 23; 8 rows bf16 10.6 / 8.0, fp32 16 / 22
 //   dcn_gemm_simt     forward, fp32: 300 x 256 x 256 7.9 / 10.8, 600 x 256 x 256 11.2 / 10.9; backward, fp32:
-//                     300 x 256 x 256 9.1 / 25, 600 x 256 x 256 19 / 27, with gelu 100 x 256 x 256 21 / 23
+//                     300 x 256 x 256 9.1 / 25, 600 x 256 x 256 19 / 27
 // and its one launch takes the place of two to six.  16-bit operands that need no staging stay on the tensor
 // cores (32 x 256 x 256 bf16 backward: 10.7 / 9.7).
 bool forward_rows(int dtype, long long rows, int64_t alignment) {
@@ -57,11 +57,9 @@ double products(long long rows, long long cin, long long cout) {
 bool forward_simt(int dtype, long long rows, long long cin, long long cout) {
   return dtype == DCN_DTYPE_F32 && cin <= 1024 && products(rows, cin, cout) <= 1 << 25;
 }
-// a block walks all of cout (for gx) or of the rows (for gw): long walks are slow; gelu's derivative is computed
-// again for every 32 columns of a product
-bool backward_simt(int dtype, int act, long long rows, long long cin, long long cout, int64_t alignment) {
-  return needs_stage(dtype, alignment) && rows <= 640 && cout <= 640 &&
-         products(rows, cin, cout) <= (act == DCN_ACT_GELU ? 1 << 23 : 1 << 25);
+// a block walks all of cout (for gx) or of the rows (for gw): long walks are slow
+bool backward_simt(int dtype, long long rows, long long cin, long long cout, int64_t alignment) {
+  return needs_stage(dtype, alignment) && rows <= 640 && cout <= 640 && products(rows, cin, cout) <= 1 << 25;
 }
 
 Layout forward_layout(int dtype, long long rows, long long cin, long long cout, int64_t alignment) {
@@ -81,7 +79,7 @@ Layout backward_layout(int dtype, int act, long long rows, long long cin, long l
                        bool want_gx, bool want_gw, bool want_gb, bool want_gx_sum) {
   Layout l;
   if (want_gx_sum) l.gx_sums = take(&l, (size_t)((rows + 31) / 32) * cin * 4);
-  l.simt = backward_simt(dtype, act, rows, cin, cout, alignment);
+  l.simt = backward_simt(dtype, rows, cin, cout, alignment);
   if (l.simt) return l;
   const bool stage = needs_stage(dtype, alignment);
   l.stage_gz = stage || act != DCN_ACT_NONE || (want_gb && !want_gw);   // the last: for its column sums

@@ -112,7 +112,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor &x, const Tensor &w, const
   Tensor y = make(shape, x.scalar_type(), x), saved;
   const Tensor b = has(bias) ? bias->contiguous() : Tensor();
   if (save && act == DCN_ACT_RELU) saved = make({xr.rows, (cout + 31) / 32}, at::kInt, x);
-  if (save && act == DCN_ACT_GELU) saved = make({xr.rows, (cout + 7) / 8 * 8}, code == DCN_DTYPE_F32 ? at::kFloat : at::kHalf, x);
+  if (save && act == DCN_ACT_GELU) saved = make({xr.rows, (cout + 7) / 8 * 8}, code == DCN_DTYPE_F32 ? at::kFloat : at::kShort, x);
   const int64_t align = (int64_t)(uintptr_t)xr.p | (int64_t)(uintptr_t)wr.p | ((xr.ld | wr.ld) * es);
   size_t bytes = 0;
   check(dcn_linear_workspace_bytes(code, xr.rows, cin, cout, align, &bytes));
