@@ -317,6 +317,26 @@ def test_feed_forward_bias_gradient_is_summed_before_rounding(rows, cin, hidden,
         assert torch.equal(grads[2], g)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,hidden', [(300, 48, 768), (70, 40, 1000)])
+def test_feed_forward_many_hidden_columns(rows, cin, hidden, dtype):
+    """bias1's gradient from the rounded hidden gradient, and each gradient wanted alone."""
+    x, gy = tensors(1, dtype, (rows, cin), (rows, cin))
+    w1, w2 = tensors(2, dtype, (hidden, cin), (cin, hidden), scale=(cin + hidden) ** -0.5)
+    b1, b2 = tensors(3, dtype, (hidden,), (cin,), scale=0.1)
+    for act in ('relu', 'gelu'):
+        want = plain.feed_forward(x, w1, b1, w2, b2, x, act, gy)
+        leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2)]
+        y = ops.feed_forward(*leaves, leaves[0], act)
+        grads = dict(zip(('gx', 'gw1', 'gb1', 'gw2', 'gb2'), torch.autograd.grad(y, leaves, gy)))
+        want['gx'] = plain.add(want['gx'], gy.double()).rounded(dtype)
+        hold({'y': y.detach(), **grads}, want)
+        for only in range(5):
+            parts = [t.detach().requires_grad_(i == only) for i, t in enumerate((x, w1, b1, w2, b2))]
+            g, = torch.autograd.grad(ops.feed_forward(*parts, parts[0], act), parts[only], gy)
+            hold({'g': g}, {'g': want[('gx', 'gw1', 'gb1', 'gw2', 'gb2')[only]]})
+
+
 def test_graphs_are_used_once_unless_retained():
     x, w, b, r, gy = linear_case(20, 24, 32, torch.bfloat16, 'gelu')
     w2, = tensors(5, torch.bfloat16, (24, 32))
