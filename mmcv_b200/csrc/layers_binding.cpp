@@ -70,7 +70,7 @@ struct Rows {
     if (t.is_contiguous()) {
       keep = t;
     } else {
-      keep = t.dim() == 2 ? t : t.reshape({rows, cols});
+      keep = t.dim() == 2 && t.size(1) == cols ? t : t.reshape({rows, cols});
       if ((keep.stride(1) != 1 && cols > 1) || (keep.stride(0) < cols && rows > 1)) keep = keep.contiguous();
       if (rows > 1) ld = keep.stride(0);
     }

@@ -458,6 +458,19 @@ def test_norm_strides_shapes_and_empty(dtype):
     hold({'gx': leaf.grad}, {'gx': plain.layer_norm(big[:, :256], w, b, 1e-5, one)['gx']})
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_over_all_dimensions_of_a_strided_matrix(dtype):
+    """One row made of a whole matrix whose own rows do not follow one another."""
+    big, w, b, gy = tensors(0, dtype, (16, 300), (16, 16), (16, 16), (16, 16))
+    for x in (big[:, :16], big[:, 3:19], big[:, :16].t(), big[::2, :32].reshape(16, 16)):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.layer_norm(leaves[0], (16, 16), leaves[1], leaves[2])
+        grads = torch.autograd.grad(y, leaves, gy.t())
+        flat = lambda t: t.reshape(1, 256)   # noqa: E731
+        want = plain.layer_norm(flat(x), w.flatten(), b.flatten(), 1e-5, flat(gy.t()))
+        hold({'y': flat(y.detach()), 'gx': flat(grads[0]), 'gw': grads[1].flatten(), 'gb': grads[2].flatten()}, want)
+
+
 def test_norm_gradient_against_differences():
     x, w, b, gy = norm_case(30, 40, torch.float32)
     got = run_norm(x, w, b, gy)
