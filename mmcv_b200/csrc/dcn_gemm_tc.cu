@@ -265,14 +265,35 @@ GemmPlan plan_gemm(int planes, long long m, long long n, long long k, bool weigh
     p.kb_split = (int)((p.kb_total + splits - 1) / splits);
     p.splits = (p.kb_total + p.kb_split - 1) / p.kb_split;
   } else {
-    // pairs halve the loads of B but tie two epilogues together: with few steps to a tile the epilogues are
-    // what counts (35642 x 256 x 1024 bf16: 27.8 us alone, 31.5 us in pairs; 35642 x 1024 x 256: 24.2 and
-    // 21.3 us; 8192 x 4096 x 4096: 239 and 173 us)
-    if (n > wide / 2 && tiles(256, wide) >= 74 && (planes == 3 || p.kb_total > 6)) {
-      p.bn = wide;
-      p.cg = 2;
-    } else {
-      p.bn = n > wide / 2 && tiles(128, wide) >= 148 ? wide : n > 64 && tiles(128, 128) >= 148 ? 128 : 64;
+    // The shape of least time by what was measured, in clocks: a block takes operands in at 46 bytes a clock
+    // (fp32: its six products are as slow), its epilogue works under the next tile's steps, and tiles come in
+    // rounds of as many as there are blocks or pairs.  us, chosen / next best / 128 x 128 tiles:
+    //   bf16 8192 x 4096 x 4096 173 / 214 / 352, 4096 x 2048 x 1024 18.4 / 19.5 / 27.0, 3000 x 2048 x 512 15.7 /
+    //   16.6, 600 x 1024 x 256 8.7 / 9.0; fp32 3000 x 2048 x 512 50.0 / 54.1, 4096 x 1024 x 2048 83 / 94 / 120
+    struct Shape {
+      int bn, cg;
+      long long step, epilogue;   // of 64 values of k; of a tile
+    };
+    const Shape shapes16[] = {{256, 2, 711, 7000}, {256, 1, 1050, 6000}, {128, 1, 711, 3000}, {64, 1, 520, 1600}};
+    const Shape shapes32[] = {{128, 2, 1600, 4000}, {128, 1, 2140, 4000}, {64, 1, 1600, 2000}};
+    const Shape *shapes = planes == 1 ? shapes16 : shapes32;
+    long long best = 0;
+    for (int i = 0; i < (planes == 1 ? 4 : 3); ++i) {
+      const Shape &c = shapes[i];
+      const long long rounds = (tiles(128 * c.cg, c.bn) * c.cg + 147) / 148, steps = p.kb_total * c.step;
+      const long long time = rounds * (steps > c.epilogue ? steps : c.epilogue) + (steps > c.epilogue ? c.epilogue : steps);
+      if (i == 0 || time < best) {
+        best = time;
+        p.bn = c.bn;
+        p.cg = c.cg;
+      }
+    }
+    // 16-bit tiles of few steps are bound by their stores and epilogues, which that does not tell apart: the
+    // widest tile that fills the SMs, no pairs (35642 x 256 x 1024 27.6 us, in pairs 31.6, 128 wide 31.7;
+    // 35642 x 256 x 256 10.1, 11.8, 11.2)
+    if (planes == 1 && p.kb_total <= 6) {
+      p.cg = 1;
+      p.bn = n > 128 && tiles(128, 256) >= 148 ? 256 : n > 64 && tiles(128, 128) >= 148 ? 128 : 64;
     }
     if (p.bn == 64) {
       // Few tiles and a long sum: a block takes in 24 KB (fp32: 72 KB) a step at 46 bytes a cycle, so that
