@@ -341,7 +341,7 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   ok = ok && (g.b_mn ? encode3(&p.b, t16, 2, g.b, g.n, g.kk, planes, g.ldb, 64, 64)
                      : encode3(&p.b, t16, 2, g.b, g.kk, g.n, planes, g.ldb, 64, plan.bn / plan.cg));
   const bool rows16 = g.n * esize % 16 == 0;
-  const unsigned cw = esize == 4 || plan.bn < 256 ? 32 : 64;   // kChunkRow
+  const unsigned cw = esize == 4 || plan.bn < 256 || plan.cg == 2 ? 32 : 64;   // kChunkRow
   if (parts) {
     p.out_tma = 1;
     ok = ok && encode3(&p.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, g.n, g.m, plan.splits, plan.ldp, 32, 32);

@@ -6,24 +6,28 @@
 // output index contiguous.  Tensor maps and tcgen05 descriptors take either order, so nothing is
 // transposed in memory.
 //
-// Where there are enough tiles, two blocks of a cluster work on one tile of 256 rows (CG = 2): each loads
-// its own 128 rows of A and half of the rows of B, and one tcgen05.mma.cta_group::2 multiplies what
-// lies in both.  A step of a 256-column tile then brings 32 KB into an SM instead of 48: what bounds
-// the products with few steps or few output columns is the rate at which tiles come in (about 35
-// bytes a cycle and SM measured, from L2 or memory).
+// Two blocks of a cluster may work on one tile of 256 rows (CG = 2): each loads its own 128 rows of A and
+// half of the rows of B, and one tcgen05.mma.cta_group::2 multiplies what lies in both.  A step of a
+// 256-column tile then brings 32 KB into an SM instead of 48, and what bounds the long products is the rate
+// at which tiles come in (46 bytes a clock and SM with five stages in flight, 40 with three).  plan_gemm
+// chooses; where tiles are few and sums long, two to four blocks of a cluster share a tile's sum instead.
 //
 // One persistent block per SM: a loader lane fills a ring of stages (64 values of k of a 128-row A
 // tile and a BN-row B tile, 128-byte swizzle) with cp.async.bulk.tensor; one warp issues tcgen05.mma
 // into fp32 accumulators in tensor memory, double-buffered so that the epilogue of a tile runs under
-// the main loop of the next; eight warps run the epilogue: tcgen05.ld, bias, activation, derivative,
+// the main loop of the next; epilogue warps do the rest: tcgen05.ld, bias, activation, derivative,
 // residual, one rounding, a 32-row chunk in shared memory, a tensor store.  The residual arrives by
 // tensor load in the chunk that the result leaves from, as do the kept derivatives of gelu.
-// Sixteen epilogue warps (eight with fp32 tensors) and not four: a warp's share of a tile is a chain of waits (tensor memory,
-// loads, the store of its last chunk), and the products around an embedding of 256 have main loops of
-// four steps only (35642 x 256 x 1024 bf16 with relu: 42 us with eight warps).  Every wait is bounded.
+// Sixteen epilogue warps (eight with fp32 tensors) and not four: a warp's share of a tile is a chain of waits
+// (tensor memory, loads, the store of its last chunk), and the products around an embedding of 256 have main
+// loops of four steps only (35642 x 256 x 1024 bf16 with relu: 42 us with eight warps, 28 with sixteen).
+// Every wait is bounded.
+//
+// Measured: 8192 x 4096 x 4096 bf16 171 us, 1.61 PFLOP/s, the tensor pipe 88 % busy; 35642 x 256 x 1024 28 us
+// (its bytes 14 us at the copy rate), bound by the epilogue's chain.
 //
 // 16-bit tensors: one plane (PL = 1).  fp32 tensors: every operand is the exact sum of three bf16
-// planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_split writes them), and the product is
+// planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_stage writes them), and the product is
 //   x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1);
 // what is left out is below 2^-24 of |x||y|.  A tensor core truncates where it adds to its
 // accumulator, so long fp32 sums would drift by 2^-24 a step: the leading product and the five small
@@ -31,8 +35,8 @@
 // into registers, where the additions round to nearest.
 //
 // The weight gradient's sum over the rows is cut into `splits` ranges when its tiles alone do not
-// fill the SMs; the fp32 parts are added in order by dcn_gemm_reduce.  Its bias gradient (row sums
-// of A) costs one more 128x16 instruction a step: a product with a tile of ones.
+// fill the SMs; the fp32 parts are added in order by dcn_gemm_reduce.  With 16-bit tensors its bias gradient
+// (row sums of A) costs one more instruction a step: a product with a tile of ones.
 #pragma once
 
 #include <atomic>
@@ -56,10 +60,11 @@ constexpr int kEpi = PL == 3 ? 8 : 16;
 template <int PL>
 constexpr int kThreadsOf = (kEpi<PL> + 2) * 32;
 
-// Bytes of a row of an epilogue warp's staging chunk (32 rows): with 16-bit results a warp has 64
-// columns of a 256-column tile, else (at least) 32.
-template <typename TO, int BN>
-constexpr int kChunkRow = sizeof(TO) == 4 || BN == 256 ? 128 : 64;
+// Bytes of a row of an epilogue warp's staging chunk (32 rows).  128 where a warp of a 256-column tile has 64
+// columns of 16 bits: fewer, wider stores for tiles of few steps.  Pairs, which take the long sums, give the
+// memory to a sixth stage instead (8192 x 4096 x 4096: 176 -> 171 us).
+template <typename TO, int BN, int CG>
+constexpr int kChunkRow = sizeof(TO) == 4 || (BN == 256 && CG == 1) ? 128 : 64;
 constexpr int kUnitBlocks = 4;          // PL = 3: 64-value blocks between two drains of the accumulators
 
 __device__ int g_gemm_status;           // the first wait that ran out (0: none), until it is read
@@ -396,8 +401,7 @@ __device__ __forceinline__ void add_row(const TO *src, int j1, int n, float (&v)
 // the instruction cache and its registers).
 template <typename TI, typename TO, int PL, int BN, bool AMN, bool BMN, int CG, int EPI>
 __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_constant__ GemmTc p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   constexpr uint32_t kABytes = PL * 16384u, kBBytes = PL * (BN / CG) * 128u, kStage = kABytes + kBBytes;
   constexpr int kEpiWarps = kEpi<PL>, kGemmThreads = kThreadsOf<PL>, kGroups = kEpiWarps / 4;
   constexpr bool kRowSum = AMN && PL == 1;             // only the weight gradient asks for row sums
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   constexpr int kCols = kBufs * kBufCols + (kRowSum ? kOnes * kBufs : 0);
   constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512, "tensor memory");
-  constexpr int RB = kChunkRow<TO, BN>, kChunkBytes = 32 * RB;
+  constexpr int RB = kChunkRow<TO, BN, CG>, kChunkBytes = 32 * RB;
   constexpr int CW = RB / (int)sizeof(TO);             // columns of a staging chunk
   constexpr int kWarpCols = BN / kGroups > CW ? BN / kGroups : CW;   // columns of an epilogue warp
 
@@ -430,6 +434,10 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
   uint8_t *parts = ones;   // (nobody has both) [ks - 1][active epilogue warps][8][32 lanes] x 16 bytes
   const unsigned long long limit = p.wait_limit_ns;
 
+  if (bar0 & 1023u) {   // the swizzles go by addresses; the declaration sees to this
+    if (threadIdx.x == 0) atomicCAS(&g_gemm_status, 0, 10);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(full + 8 * i, 1);
@@ -884,7 +892,7 @@ cudaError_t run_tc(GemmTc &p, cudaStream_t s) {
     done_mask.fetch_or(bit, std::memory_order_release);
   }
   constexpr size_t stage = (size_t)PL * (16384 + BN / CG * 128);
-  constexpr size_t fixed = 1024 + 1024 + (size_t)kEpi<PL> * 32 * kChunkRow<TO, BN> + (AMN && PL == 1 ? 2048 : 0);
+  constexpr size_t fixed = 1024 + (size_t)kEpi<PL> * 32 * kChunkRow<TO, BN, CG> + (AMN && PL == 1 ? 2048 : 0);
   const size_t parts = (size_t)(p.ks - 1) * (BN / 32 * 4 * 4096);
   const int fit = (int)((kMost - fixed - parts) / stage), stages = fit > 8 ? 8 : fit;
   static_assert((kMost - fixed) / stage >= 2, "a ring");
