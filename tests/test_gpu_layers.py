@@ -516,6 +516,69 @@ def test_another_stream_and_two_at_once():
         assert all(torch.equal(o, want[k]) for o in got[k])
 
 
+def test_threads_with_a_stream_each():
+    """Training steps of four threads at once, sizes that run on every kernel."""
+    import threading
+    sets = [block_inputs(dt, rows=rows, seed=10 * k)
+            for k, (dt, rows) in enumerate([(torch.bfloat16, 3000), (torch.float32, 70), (torch.float16, 3),
+                                            (torch.float32, 2500)])]
+
+    def step(x, gy, *params):
+        leaves = [t.detach().requires_grad_(True) for t in (x, *params)]
+        y = block(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got, failed = [None] * 4, []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[k] = step(*sets[k])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:   # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed
+    for k in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want[k]))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows of the result and of the gradients against a call on those rows."""
+    rows, cin, cout = 2_150_000, 16, 1024
+    x, w, b, _, _ = linear_case(rows, cin, cout, torch.bfloat16, None)
+    tail = slice(rows - 300, rows)
+    for act in ('relu', 'gelu'):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.fused_linear(*leaves, activation=act)
+        assert y.numel() > 2 ** 31
+        gy = torch.zeros_like(y)
+        gy[tail] = tensors(5, torch.bfloat16, (300, cout))[0]
+        got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(y, leaves, gy)))
+        want = plain.linear(x[tail], w, b, None, act, gy[tail])
+        hold({'y': y.detach()[tail], 'gx': got['gx'][tail], 'gw': got['gw'], 'gb': got['gb']}, want)
+        assert not got['gx'][:rows - 300].any()
+        del y, gy, got, leaves
+    del x
+    rows, cols = 530_000, 4104
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device='cuda').normal_(generator=torch.Generator('cuda').manual_seed(0))
+    w, b = tensors(1, torch.bfloat16, (cols,), (cols,))
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = ops.layer_norm(leaves[0], (cols,), leaves[1], leaves[2])
+    gy = torch.zeros_like(y)
+    gy[-200:] = tensors(5, torch.bfloat16, (200, cols))[0]
+    got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(y, leaves, gy)))
+    hold({'y': y.detach()[-200:], 'gx': got['gx'][-200:], 'gw': got['gw'], 'gb': got['gb']},
+         plain.layer_norm(x[-200:], w, b, 1e-5, gy[-200:]))
+    assert not got['gx'][:-200].any()
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_captured_training_step(dtype):
     """Forward and backward in a CUDA graph while an eager graph of the same leaves lives (made on a side
