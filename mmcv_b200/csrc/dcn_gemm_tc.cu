@@ -47,26 +47,14 @@ __global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__
   if (j + 3 < n) o[3] = ElemOf<T>::from(v.w);
 }
 
-// out[c] = sum over the parts, 32 of them side by side, joined in a tree
-template <typename T>
+// out[c] = sum over the parts
+template <typename T, int C>
 __global__ void __launch_bounds__(1024) dcn_column_reduce(const float *__restrict__ part, int parts, long long cols, T *out) {
-  __shared__ float sm[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long long c = blockIdx.x * 32LL + tx;
-  float v = 0.f;
+  const long long c = blockIdx.x * (long long)C + threadIdx.x % C;
   pdl_wait();
   pdl_launch();
-  if (c < cols) {
-#pragma unroll 8
-    for (int p = ty; p < parts; p += 32) v += part[p * cols + c];
-  }
-  sm[ty][tx] = v;
-  __syncthreads();
-  for (int d = 16; d > 0; d >>= 1) {
-    if (ty < d) sm[ty][tx] += sm[ty + d][tx];
-    __syncthreads();
-  }
-  if (ty == 0 && c < cols) out[c] = ElemOf<T>::from(sm[0][tx]);
+  const float v = column_join<C>(part + c, parts, cols, c < cols);
+  if (threadIdx.x < C && c < cols) out[c] = ElemOf<T>::from(v);
 }
 
 // x = x1 + x2 + x3, 8 bits each (truncated, so that nothing overflows); an infinity or NaN stays in x1
@@ -245,6 +233,14 @@ cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &
                     plan.ldp, groups, (T *)g.out);
 }
 
+template <typename T>
+cudaError_t run_columns(const float *part, int parts, long long cols, void *out, cudaStream_t s) {
+  const int c = join_columns(cols);
+  const unsigned grid = (unsigned)((cols + c - 1) / c);
+  if (c == 8) return launch_pdl(dcn_column_reduce<T, 8>, grid, 1024, 0, s, 1, part, parts, cols, (T *)out);
+  return launch_pdl(dcn_column_reduce<T, 32>, grid, 1024, 0, s, 1, part, parts, cols, (T *)out);
+}
+
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
@@ -397,11 +393,9 @@ cudaError_t launch_gemm_stage(StageJobs &jobs, int dtype, cudaStream_t s) {
 }
 
 cudaError_t launch_column_reduce(const float *part, int parts, long long cols, int dtype, void *out, cudaStream_t s) {
-  const unsigned grid = (unsigned)((cols + 31) / 32);
-  if (dtype == DCN_DTYPE_F32) return launch_pdl(dcn_column_reduce<float>, grid, 1024, 0, s, 1, part, parts, cols, (float *)out);
-  if (dtype == DCN_DTYPE_BF16)
-    return launch_pdl(dcn_column_reduce<__nv_bfloat16>, grid, 1024, 0, s, 1, part, parts, cols, (__nv_bfloat16 *)out);
-  return launch_pdl(dcn_column_reduce<__half>, grid, 1024, 0, s, 1, part, parts, cols, (__half *)out);
+  if (dtype == DCN_DTYPE_F32) return run_columns<float>(part, parts, cols, out, s);
+  if (dtype == DCN_DTYPE_BF16) return run_columns<__nv_bfloat16>(part, parts, cols, out, s);
+  return run_columns<__half>(part, parts, cols, out, s);
 }
 
 cudaError_t read_gemm_status(cudaStream_t s, int *status) {

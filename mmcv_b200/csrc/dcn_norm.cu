@@ -398,28 +398,24 @@ __global__ void __launch_bounds__(kThreads) norm_columns_wide(const NormArgs a) 
   a.part[((long long)blockIdx.y * 2 + 1) * a.cols + c] = gb;
 }
 
-// out[c] = sum over the partial rows, 32 of them side by side; blockIdx.y: 0 gw, 1 gb
-template <typename T>
+// out[c] = sum over the partial rows; blockIdx.y: 0 gw, 1 gb
+template <typename T, int C>
 __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ part, int parts, int cols, T *gw, T *gb) {
-  __shared__ float s[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + tx;
+  const int c = blockIdx.x * C + threadIdx.x % C;
   T *out = blockIdx.y ? gb : gw;
   pdl_wait();
   pdl_launch();
   if (!out) return;
-  float v = 0.f;
-  if (c < cols) {
-#pragma unroll 8
-    for (int p = ty; p < parts; p += 32) v += part[((long long)p * 2 + blockIdx.y) * cols + c];
-  }
-  s[ty][tx] = v;
-  __syncthreads();
-  for (int d = 16; d > 0; d >>= 1) {
-    if (ty < d) s[ty][tx] += s[ty + d][tx];
-    __syncthreads();
-  }
-  if (ty == 0 && c < cols) out[c] = ElemOf<T>::from(s[0][tx]);
+  const float v = column_join<C>(part + blockIdx.y * (long long)cols + c, parts, 2LL * cols, c < cols);
+  if (threadIdx.x < C && c < cols) out[c] = ElemOf<T>::from(v);
+}
+
+template <typename T>
+cudaError_t run_reduce(const NormArgs &a, int parts, void *gw, void *gb, cudaStream_t s) {
+  const int c = join_columns(a.cols);
+  const dim3 grid((unsigned)((a.cols + c - 1) / c), 2);
+  if (c == 8) return launch_pdl(norm_reduce<T, 8>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (T *)gw, (T *)gb);
+  return launch_pdl(norm_reduce<T, 32>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (T *)gw, (T *)gb);
 }
 
 template <typename T, int V, int E, int G>
@@ -582,14 +578,9 @@ int dcn_layer_norm_backward(const void *gy, int64_t ldgy, const void *x, int64_t
   int parts = 0;
   e = run_typed(a, dtype, true, params, &parts, s);
   if (e == cudaSuccess && params) {
-    const dim3 grid((unsigned)((cols + 31) / 32), 2);
-    if (wdtype == DCN_DTYPE_F32)
-      e = launch_pdl(norm_reduce<float>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (float *)gw, (float *)gb);
-    else if (wdtype == DCN_DTYPE_BF16)
-      e = launch_pdl(norm_reduce<__nv_bfloat16>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (__nv_bfloat16 *)gw,
-                     (__nv_bfloat16 *)gb);
-    else
-      e = launch_pdl(norm_reduce<__half>, grid, 1024, 0, s, 1, a.part, parts, a.cols, (__half *)gw, (__half *)gb);
+    if (wdtype == DCN_DTYPE_F32) e = run_reduce<float>(a, parts, gw, gb, s);
+    else if (wdtype == DCN_DTYPE_BF16) e = run_reduce<__nv_bfloat16>(a, parts, gw, gb, s);
+    else e = run_reduce<__half>(a, parts, gw, gb, s);
   }
   return e == cudaSuccess ? DCN_OK : set_error(DCN_ERR_CUDA, cudaGetErrorString(e));
 }
