@@ -233,17 +233,6 @@ struct Walk {
   }
 };
 
-// (x0, x1) += (y0, y1) in one instruction
-__device__ __forceinline__ void add2(float &x0, float &x1, float y0, float y1) {
-  asm("{\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%0, %1};\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "add.rn.f32x2 a, a, b;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(x0), "+f"(x1)
-      : "f"(y0), "f"(y1));
-}
-
 // A staging chunk: 32 rows of RB bytes, 16-byte pieces permuted within a row as the tensor maps'
 // swizzles of that width have them, so that the lanes of a warp, a row each, meet no bank conflicts.
 template <int RB>

@@ -72,6 +72,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (x0, x1) += (y0, y1) in one instruction
+__device__ __forceinline__ void add2(float &x0, float &x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y0), "f"(y1));
+}
+// (a0, a1) += (x0, x1) * (y0, y1)
+__device__ __forceinline__ void fma2_to(float &a0, float &a1, float x0, float x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%0, %1};\n\t"
+      "fma.rn.f32x2 c, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
 // (x0, x1) * (y0, y1) + (z, z), each rounded to nearest
 __device__ __forceinline__ void fma2(float &x0, float &x1, float y0, float y1, float z) {
   asm("{\n\t.reg .b64 a, b, c;\n\t"
