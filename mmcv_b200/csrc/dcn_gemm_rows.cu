@@ -1,11 +1,12 @@
 // The forward product for up to eight rows (a token, a few queries):
 //   y[r, n] = act(sum_k x[r, k] w[n, k] + b[n]) + res[r, n]
-// What counts is the weight's way through the chip once and the latency of a single wave of loads, so
-// nothing is staged and no tensor core is asked: a warp owns NC columns, its lanes lie along k, 16 bytes
-// of the weight each, and x comes from L1.  The NC * R sums of a warp are joined by exchanges in which
-// each lane gives away the half that its partner keeps.  A block has 32 columns, so that it owns whole
-// words of relu's kept bits.  Bound: memory (the weight), or the launch.
-// Measured against the tensor-core kernel (its tiles are 128 rows): see run_rows.
+// What counts is the weight's way through the chip once and the latency of few waves of loads, so nothing is
+// staged and no tensor core is asked: a warp owns a column, or a half or quarter of its k (KP = 2, 4: as many
+// times the blocks, and that part of the turns), its lanes lie along k, 16 bytes of the weight each and four
+// loads in flight, and x comes from L1.  The R sums of a warp are joined by exchanges in which each lane gives
+// away the half that its partner keeps, the warps of a column in order.  More columns to a warp were slower
+// (1 x 4096 x 4096 bf16: one 11.5 us, two 17.8, four 31.7).  Bound: memory (the weight), or the launch.
+// Measured against the other kernels: forward_rows in dcn_linear.cu.
 #include "dcn_gemm.cuh"
 
 namespace dcn {
@@ -29,15 +30,14 @@ __device__ __forceinline__ void floats(const uint4 &u, float (&o)[V]) {
   for (int i = 0; i < V; ++i) o[i] = ElemOf<T>::to(e[i]);
 }
 
-template <typename T, int V, int R, int NC>
-__global__ void __launch_bounds__(1024 / NC) dcn_linear_rows(const GemmArgs g) {
-  constexpr int U = 4 / NC;             // chunks of k in flight: four loads of the weight in all
-  constexpr int N = NC * R;
+template <typename T, int V, int R, int KP>
+__global__ void __launch_bounds__(1024) dcn_linear_rows(const GemmArgs g) {
+  constexpr int U = 4, CB = 32 / KP;    // chunks of k in flight; columns of a block
   __shared__ uint32_t bits[R];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float join[KP > 1 ? KP : 1][CB][R];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = warp % CB, part = warp / CB;
   const int m = (int)g.m, n = (int)g.n, kk = (int)g.kk;
-  const int j0 = blockIdx.x * 32 + warp * NC;
-  const T *w = (const T *)g.b, *x = (const T *)g.a;
+  const int j = blockIdx.x * CB + col;
   const bool keep_bits = g.act == DCN_ACT_RELU && g.saved;
   pdl_wait();
   pdl_launch();
@@ -45,39 +45,33 @@ __global__ void __launch_bounds__(1024 / NC) dcn_linear_rows(const GemmArgs g) {
     if (threadIdx.x < R) bits[threadIdx.x] = 0u;
     __syncthreads();
   }
-  float acc[N] = {};
-  if (j0 < n) {
-    for (int k0 = lane * V; k0 < kk; k0 += 32 * V * U) {
-      uint4 wu[U][NC];
+  const T *w = (const T *)g.b + (long long)min(j, n - 1) * g.ldb, *x = (const T *)g.a;
+  float acc[R] = {};
+  for (int k0 = (part * 32 + lane) * V; k0 < kk; k0 += 32 * V * KP * U) {
+    uint4 wu[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 32 * V * KP;
+      wu[u] = make_uint4(0, 0, 0, 0);
+      if (k < kk) wu[u] = load16<T, V>(w + k, kk - k);
+    }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int k = k0 + u * 32 * V;
-          wu[u][c] = make_uint4(0, 0, 0, 0);
-          if (k < kk) wu[u][c] = load16<T, V>(w + min(j0 + c, n - 1) * g.ldb + k, kk - k);
-        }
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 32 * V * KP;
+      if (k >= kk) break;
+      float wv[V];
+      floats<T, V>(wu[u], wv);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + u * 32 * V;
-        if (k >= kk) break;
-        float wv[NC][V];
+      for (int r = 0; r < R; ++r) {
+        float xv[V];
+        floats<T, V>(load16<T, V>(x + min(r, m - 1) * g.lda + k, kk - k), xv);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) floats<T, V>(wu[u][c], wv[c]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float xv[V];
-          floats<T, V>(load16<T, V>(x + min(r, m - 1) * g.lda + k, kk - k), xv);
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[c * R + r] = fmaf(xv[i], wv[c][i], acc[c * R + r]);
-        }
+        for (int i = 0; i < V; ++i) acc[r] = fmaf(xv[i], wv[i], acc[r]);
       }
     }
   }
-  // lane / (32 / N) ends up with the sum acc[lane / (32 / N)] over the warp
-  int have = N;
+  // lane / (32 / R) ends up with the sum acc[lane / (32 / R)] over the warp
+  int have = R;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     if (have > 1) {
@@ -92,13 +86,23 @@ __global__ void __launch_bounds__(1024 / NC) dcn_linear_rows(const GemmArgs g) {
       acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], d);
     }
   }
-  const int idx = lane / (32 / N), c = idx / R, r = idx % R, j = j0 + c;
-  if (lane % (32 / N) == 0 && j < n && r < m) {
+  const int r = lane / (32 / R);
+  const bool mine = lane % (32 / R) == 0;
+  float v = acc[0];
+  if constexpr (KP > 1) {
+    if (mine) join[part][col][r] = v;
+    __syncthreads();
+    if (part == 0) {
+      v = join[0][col][r];
+#pragma unroll
+      for (int q = 1; q < KP; ++q) v += join[q][col][r];
+    }
+  }
+  if (part == 0 && mine && j < n && r < m) {
     constexpr bool kFine = sizeof(T) == 4;
-    float v = acc[0];
     if (g.bias) v += ElemOf<T>::to(((const T *)g.bias)[j]);
     if (g.act == DCN_ACT_RELU) {
-      if (keep_bits && relu_bit(v)) atomicOr(&bits[r], 1u << (j & 31));
+      if (keep_bits && relu_bit(v)) atomicOr(&bits[r], 1u << col);
       v = relu_value(v);
     } else if (g.act == DCN_ACT_GELU) {
       if (g.saved) keep_slope<T>(g.saved, r * ((g.n + 7) / 8 * 8) + j, gelu_slope<kFine>(v));
@@ -107,18 +111,24 @@ __global__ void __launch_bounds__(1024 / NC) dcn_linear_rows(const GemmArgs g) {
     if (g.res) v += ElemOf<T>::to(((const T *)g.res)[r * g.ldr + j]);
     ((T *)g.out)[r * g.n + j] = ElemOf<T>::from(v);
   }
-  if (keep_bits) {
+  if (keep_bits) {   // a block's columns are a word of the bits, or a half or byte of one
     __syncthreads();
-    if ((int)threadIdx.x < m) ((uint32_t *)g.saved)[threadIdx.x * ((g.n + 31) / 32) + blockIdx.x] = bits[threadIdx.x];
+    if ((int)threadIdx.x < m) {
+      uint32_t *row = (uint32_t *)g.saved + threadIdx.x * ((g.n + 31) / 32);
+      if constexpr (CB == 32) row[blockIdx.x] = bits[threadIdx.x];
+      else if constexpr (CB == 16) ((uint16_t *)row)[blockIdx.x] = (uint16_t)bits[threadIdx.x];
+      else ((uint8_t *)row)[blockIdx.x] = (uint8_t)bits[threadIdx.x];
+    }
   }
 }
 
 template <typename T, int V, int R>
 cudaError_t run_rows(const GemmArgs &g, cudaStream_t s) {
-  const unsigned blocks = (unsigned)((g.n + 31) / 32);
-  // one column a warp while the blocks do not fill the SMs: a column's loads are then spread over more of them
-  if (blocks < 148) return launch_pdl(dcn_linear_rows<T, V, R, 1>, blocks, 1024, 0, s, 1, g);
-  return launch_pdl(dcn_linear_rows<T, V, R, 4>, blocks, 256, 0, s, 1, g);
+  // parts of k while the blocks that come of it have an SM each (1 x 4096 x 1024 bf16: quarters 3.6 us, whole
+  // columns 8.8; 1 x 1024 x 4096: 7.2, 3.4)
+  if (g.n <= 8 * 148) return launch_pdl(dcn_linear_rows<T, V, R, 4>, (unsigned)((g.n + 7) / 8), 1024, 0, s, 1, g);
+  if (g.n <= 16 * 148) return launch_pdl(dcn_linear_rows<T, V, R, 2>, (unsigned)((g.n + 15) / 16), 1024, 0, s, 1, g);
+  return launch_pdl(dcn_linear_rows<T, V, R, 1>, (unsigned)((g.n + 31) / 32), 1024, 0, s, 1, g);
 }
 template <typename T, int V>
 cudaError_t run_v(const GemmArgs &g, cudaStream_t s) {

@@ -41,14 +41,16 @@ bool needs_stage(int dtype, int64_t alignment) { return dtype == DCN_DTYPE_F32 |
 // does not.
 //
 // Times in us of one call among others, here / tensor cores with their staging pass:
-//   dcn_linear_rows   1 x 256 x 1024 bf16 2.0 / 4.5, fp32 2.2 / 10.1; 4 x 1024 x 1024 bf16 6.1 / 8.0, fp32
-//                     8.6 / 22; 4 x 4096 x 4096 bf16 20 / 23; 8 rows bf16 10.6 / 8.0, fp32 16 / 22
+//   dcn_linear_rows   1 x 256 x 1024 bf16 2.0 / 5.0, fp32 2.1 / 9.2; 8 x 1024 x 1024 bf16 4.7 / 8.5, fp32
+//                     5.5 / 16; 8 x 4096 x 1024 bf16 10.5 / 11.9, fp32 16 / 41; but 8 x 1024 x 4096 bf16
+//                     10.9 / 9.0, 4 x 4096 x 4096 21 / 21, 1 x 2048 x 16384 26 / 22 (fp32 32 / 108)
 //   dcn_gemm_simt     forward, fp32: 300 x 256 x 256 7.9 / 10.8, 600 x 256 x 256 11.2 / 10.9; backward, fp32:
 //                     300 x 256 x 256 9.1 / 25, 600 x 256 x 256 19 / 27
 // and its one launch takes the place of two to six.  16-bit operands that need no staging stay on the tensor
 // cores (32 x 256 x 256 bf16 backward: 10.7 / 9.7).
-bool forward_rows(int dtype, long long rows, int64_t alignment) {
-  return rows <= (needs_stage(dtype, alignment) ? 8 : 4);
+bool forward_rows(int dtype, long long rows, long long cout, int64_t alignment) {
+  if (needs_stage(dtype, alignment) || cout <= 8 * 148) return rows <= 8;
+  return rows <= 4 && cout <= 32 * 148;
 }
 // rows as whole tiles
 double products(long long rows, long long cin, long long cout) {
@@ -64,7 +66,7 @@ bool backward_simt(int dtype, long long rows, long long cin, long long cout, int
 
 Layout forward_layout(int dtype, long long rows, long long cin, long long cout, int64_t alignment) {
   Layout l;
-  l.rows = forward_rows(dtype, rows, alignment);
+  l.rows = forward_rows(dtype, rows, cout, alignment);
   l.simt = !l.rows && forward_simt(dtype, rows, cin, cout);
   if (l.rows || l.simt) return l;
   l.stage_x = l.stage_w = needs_stage(dtype, alignment);

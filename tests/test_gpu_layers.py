@@ -86,7 +86,7 @@ def test_linear_few_rows_and_small_problems(dtype):
     the kernels for few of them and for small problems."""
     big, = tensors(7, dtype, (700, 300))
     for rows in (1, 2, 3, 4, 5, 8, 9, 33, 640):
-        for cin, cout in ((1, 33), (96, 200), (257, 31), (264, 4801 if rows == 3 else 64)):
+        for cin, cout in ((1, 33), (96, 200), (257, 31), (2100, 40), (72, 1300), (264, 4801 if rows == 3 else 64)):
             x, w, b, r, gy = linear_case(rows, cin, cout, dtype, None, True, True, seed=rows)
             for act in (None, 'relu', 'gelu'):
                 got = run_linear(x, w, b, r, gy, act)
