@@ -6,8 +6,10 @@
 //             gW = gz^T x,  gb = column sums of gz
 // Column sums of gx on its way through that derivative (the bias gradient of the layer before) are taken
 // from the epilogue's fp32 values: gx itself is rounded to the tensors' type.
-// 16-bit operands whose rows start on 16 bytes are read where they lie; others are first copied to
-// rows that do, and fp32 operands are split into three bf16 planes (dcn_gemm_stage, both).
+// Few rows and small fp32 or unaligned problems have kernels of their own, which read everything where and as
+// it lies (dcn_linear_rows, dcn_gemm_simt).  For the tensor cores, 16-bit operands whose rows start on 16
+// bytes are read where they lie; others are first copied to rows that do, and fp32 operands are split into
+// three bf16 planes (dcn_gemm_stage, both).
 #include "dcn_gemm.cuh"
 
 namespace dcn {

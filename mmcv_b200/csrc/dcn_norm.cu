@@ -8,12 +8,14 @@
 // row whose mean is large against its spread keeps its digits: the variance is taken around m + c,
 // never as a difference of large squares.  The statistics kept for the backward pass are m, c, rstd.
 //
-// Both passes read each tensor once: a row lives in the registers of a group of G threads (a warp up
-// to 1024 columns, a block of 256 up to 8192), E elements to a thread, loaded 16 bytes at a time
-// (one element at a time where sizes or alignment forbid it).  Bound: memory.
-// The backward pass keeps gw and gb in registers over all rows that a block takes, adds the warps of
+// Both passes read each tensor once: a row (up to 8192 columns) lives in the registers of a group of G
+// threads, 4 to 256, E elements to a thread, loaded 16 bytes at a time (one element at a time where sizes or
+// alignment forbid it).  Bound: memory for fp32 (35642 x 256 forward 11.7 us, its bytes 11.1 at the copy rate),
+// instructions and the latency of short rows for 16 bits (bf16 8.8 us, bytes 5.6).
+// The backward pass keeps gw and gb in registers over all rows that a group takes, adds the groups of
 // a block in order, writes one partial row per block, and a second kernel adds those in order: the
-// result does not depend on when blocks run.
+// result does not depend on when blocks run (35642 x 256 bf16: 17.6 us with both kernels, 11.8 for gx alone,
+// bytes 8.3).
 #include <cstdint>
 #include <type_traits>
 

@@ -12,6 +12,7 @@
 #include <tuple>
 #include <vector>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -90,8 +91,11 @@ Tensor workspace(const Tensor &like, size_t bytes) {
   return bytes ? make({(int64_t)bytes}, at::kByte, like) : Tensor();
 }
 
+// The status word is read after the call where that was asked for (set_check_status).  A stream that is being
+// captured cannot be waited for: what a replay leaves in the word is found by the next call outside a capture.
 void after(int device, void *stream) {
   if (!g_check_status.load(std::memory_order_relaxed)) return;
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return;
   int32_t status = 0;
   check(dcn_linear_read_status(device, stream, &status));
   TORCH_CHECK(status == 0, "dcn_b200: device-side wait ", status, " timed out; the output is not valid");

@@ -612,6 +612,28 @@ def test_captured_training_step(dtype):
             assert torch.equal(a, b)
 
 
+def test_status_reading_and_capture():
+    """With the status word read after every call, a capture still works (it reads nothing), eager calls are
+    checked, and the results are those without."""
+    from mmcv_b200 import _ext
+    x, gy, *params = block_inputs(torch.bfloat16)
+    want = block(x, *params)
+    before = _ext._check_status
+    _ext.set_check_status(True)
+    try:
+        assert torch.equal(block(x, *params), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = block(x, *params)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+        leaf = x.detach().requires_grad_(True)
+        torch.autograd.grad(block(leaf, *params), leaf, gy)
+    finally:
+        _ext.set_check_status(before)
+
+
 def test_autocast_follows_torch():
     x, gy, w1, b1, w2, b2, g, b = block_inputs(torch.float32)
     leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1)]
