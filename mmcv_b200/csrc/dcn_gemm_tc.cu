@@ -12,16 +12,25 @@ namespace dcn {
 namespace {
 
 // out[i, j] = sum over the ranges of part [splits][m][ldp]: a thread has four columns and, in a block cut into
-// `groups`, every groups-th range; the groups are joined in order
+// `groups`, every groups-th range; the groups are joined in order.  Blocks from `blocks` on: a bias gradient's
+// partial rows, eight columns each, which saves a launch.
 template <typename T>
 __global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__ part, int splits, long long m,
-                                                       long long n, long long ldp, int groups, T *__restrict__ out) {
+                                                       long long n, long long ldp, int groups, T *__restrict__ out,
+                                                       unsigned blocks, const float *join_part, int join_parts,
+                                                       T *join_out) {
   __shared__ float4 join[256];
   const int across = 256 / groups, group = threadIdx.x / across;
   const long long per_row = ldp / 4, idx = blockIdx.x * (long long)across + (threadIdx.x - group * across);
   const bool live = idx < m * per_row;
   pdl_wait();
   pdl_launch();
+  if (blockIdx.x >= blocks) {
+    const long long c = (blockIdx.x - blocks) * 8LL + (threadIdx.x & 7);
+    const float v = column_join<256, 8>(join_part + c, join_parts, m, c < m);
+    if (threadIdx.x < 8 && c < m) join_out[c] = ElemOf<T>::from(v);
+    return;
+  }
   const long long i = idx / per_row, j = (idx - i * per_row) * 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
@@ -47,14 +56,14 @@ __global__ void __launch_bounds__(256) dcn_gemm_reduce(const float *__restrict__
   if (j + 3 < n) o[3] = ElemOf<T>::from(v.w);
 }
 
-// out[c] = sum over the parts
-template <typename T, int C>
-__global__ void __launch_bounds__(1024) dcn_column_reduce(const float *__restrict__ part, int parts, long long cols, T *out) {
-  const long long c = blockIdx.x * (long long)C + threadIdx.x % C;
+// out[c] = sum over the parts, in the order that dcn_gemm_reduce has: the same bits whichever does it
+template <typename T>
+__global__ void __launch_bounds__(256) dcn_column_reduce(const float *__restrict__ part, int parts, long long cols, T *out) {
+  const long long c = blockIdx.x * 8LL + (threadIdx.x & 7);
   pdl_wait();
   pdl_launch();
-  const float v = column_join<C>(part + c, parts, cols, c < cols);
-  if (threadIdx.x < C && c < cols) out[c] = ElemOf<T>::from(v);
+  const float v = column_join<256, 8>(part + c, parts, cols, c < cols);
+  if (threadIdx.x < 8 && c < cols) out[c] = ElemOf<T>::from(v);
 }
 
 // x = x1 + x2 + x3, 8 bits each (truncated, so that nothing overflows); an infinity or NaN stays in x1
@@ -229,16 +238,14 @@ cudaError_t run_reduce(const float *part, const GemmPlan &plan, const GemmArgs &
   int groups = 1;
   while (groups < 8 && plan.splits >= 4 * groups && n * groups < 148LL * 4 * 256) groups *= 2;
   const int across = 256 / groups;
-  return launch_pdl(dcn_gemm_reduce<T>, (unsigned)((n + across - 1) / across), 256, 0, s, 1, part, plan.splits, g.m, g.n,
-                    plan.ldp, groups, (T *)g.out);
+  const unsigned blocks = (unsigned)((n + across - 1) / across), more = g.join_out ? (unsigned)((g.m + 7) / 8) : 0u;
+  return launch_pdl(dcn_gemm_reduce<T>, blocks + more, 256, 0, s, 1, part, plan.splits, g.m, g.n, plan.ldp, groups,
+                    (T *)g.out, blocks, g.join_part, g.join_parts, (T *)g.join_out);
 }
 
 template <typename T>
 cudaError_t run_columns(const float *part, int parts, long long cols, void *out, cudaStream_t s) {
-  const int c = join_columns(cols);
-  const unsigned grid = (unsigned)((cols + c - 1) / c);
-  if (c == 8) return launch_pdl(dcn_column_reduce<T, 8>, grid, 1024, 0, s, 1, part, parts, cols, (T *)out);
-  return launch_pdl(dcn_column_reduce<T, 32>, grid, 1024, 0, s, 1, part, parts, cols, (T *)out);
+  return launch_pdl(dcn_column_reduce<T>, (unsigned)((cols + 7) / 8), 256, 0, s, 1, part, parts, cols, (T *)out);
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -360,11 +367,15 @@ cudaError_t launch_gemm_tc(const GemmArgs &g, const GemmPlan &plan, int dtype, f
   else if (dtype == DCN_DTYPE_BF16) e = run_gemm_bf16(p, plan.bn, plan.cg, parts, s);
   else e = run_gemm_f16(p, plan.bn, plan.cg, parts, s);
   if (e != cudaSuccess || !parts) return e;
-  if (dtype == DCN_DTYPE_F32) e = run_reduce<float>(part, plan, g, s);
-  else if (dtype == DCN_DTYPE_BF16) e = run_reduce<__nv_bfloat16>(part, plan, g, s);
-  else e = run_reduce<__half>(part, plan, g, s);
-  if (e == cudaSuccess && g.row_sum) e = launch_column_reduce(row_part, plan.splits, g.m, dtype, g.row_sum, s);
-  return e;
+  GemmArgs r = g;
+  if (g.row_sum) {
+    r.join_part = row_part;
+    r.join_parts = plan.splits;
+    r.join_out = g.row_sum;
+  }
+  if (dtype == DCN_DTYPE_F32) return run_reduce<float>(part, plan, r, s);
+  if (dtype == DCN_DTYPE_BF16) return run_reduce<__nv_bfloat16>(part, plan, r, s);
+  return run_reduce<__half>(part, plan, r, s);
 }
 
 int stage_slabs(long long rows, long long cols) {

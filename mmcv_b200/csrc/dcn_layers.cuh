@@ -35,6 +35,10 @@ struct GemmArgs {
   void *out;       // element type of the operands, row stride n
   // row sums of A over k, [m] (the bias gradient, when A is the transposed output gradient)
   void *row_sum;
+  // column sums of other partial rows [join_parts][m] to join on the way, with a product whose parts are joined
+  const float *join_part;
+  int join_parts;
+  void *join_out;
   // with slope_act: fp32 column sums of v (before the residual and the rounding) over every 32 rows,
   // [ceil(m / 32)][n]
   float *col_part;
@@ -209,19 +213,20 @@ __device__ __forceinline__ float relu_value(float z) {
 // The bit that relu's backward pass keeps of z: the gradient passes unless z <= 0.
 __device__ __forceinline__ bool relu_bit(float z) { return !(z <= 0.f); }
 
-// The sum of `parts` values `stride` apart, from p on, for each of C neighbouring columns: a block of 1024
-// threads, 1024 / C to a column (threadIdx.x % C), joined in an order that does not change.  The result is in
+// The sum of `parts` values `stride` apart, from p on, for each of C neighbouring columns: a block of NT
+// threads, NT / C to a column (threadIdx.x % C), joined in an order that does not change.  The result is in
 // the first C threads.  Eight columns while they are few: all that counts then is latency (444 rows of 512
 // columns 7.8 us with 32 columns to a block); with many the blocks are enough anyway.
-template <int C>
+template <int NT, int C>
 __device__ __forceinline__ float column_join(const float *p, int parts, long long stride, bool live) {
-  static_assert(C == 8 || C == 32, "whole warps");
-  __shared__ float s[32][C];
+  constexpr int W = NT / 32, L = 32 / C;   // warps; lanes of a warp to a column
+  static_assert((C == 8 || C == 32) && W % L == 0, "whole warps");
+  __shared__ float s[W][C];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float v = 0.f;
   if (live) {
-#pragma unroll 4
-    for (int q = threadIdx.x / C; q < parts; q += 1024 / C) v += p[q * stride];
+#pragma unroll 8
+    for (int q = threadIdx.x / C; q < parts; q += NT / C) v += p[q * stride];
   }
 #pragma unroll
   for (int d = C; d < 32; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -230,7 +235,7 @@ __device__ __forceinline__ float column_join(const float *p, int parts, long lon
   if (warp) return 0.f;
   v = 0.f;
 #pragma unroll
-  for (int q = 0; q < C; ++q) v += s[lane / C * C + q][lane % C];
+  for (int q = 0; q < W / L; ++q) v += s[lane / C * (W / L) + q][lane % C];
 #pragma unroll
   for (int d = C; d < 32; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;

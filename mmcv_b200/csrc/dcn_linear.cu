@@ -268,7 +268,8 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
     ldwt = pitch_of(cin);
   }
   e = launch_gemm_stage(jobs, dtype, s);
-  if (e == cudaSuccess && sums)
+  const bool joined = sums && gw && l.gw_plan.splits > 1;   // by the launch that joins the weight gradient's parts
+  if (e == cudaSuccess && sums && !joined)
     e = launch_column_reduce((const float *)(ws + l.sums), stage_slabs(rows, cout), cout, dtype, gb, s);
   if (e != cudaSuccess) return cuda_error(e);
   if (gx) {
@@ -286,6 +287,11 @@ int dcn_linear_backward(const void *gy, int64_t ldgy, const void *x, int64_t ldx
     g.a = gz; g.lda = ldgz; g.a_mn = true; g.b = xs; g.ldb = ldxs; g.b_mn = true;
     g.m = cout; g.n = cin; g.kk = rows;
     g.out = gw; g.row_sum = sums ? nullptr : gb;
+    if (joined) {
+      g.join_part = (const float *)(ws + l.sums);
+      g.join_parts = stage_slabs(rows, cout);
+      g.join_out = gb;
+    }
     e = launch_gemm_tc(g, l.gw_plan, dtype, (float *)(ws + l.part), (float *)(ws + l.row_part), s);
     if (e != cudaSuccess) return cuda_error(e);
   }

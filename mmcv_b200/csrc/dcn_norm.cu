@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(1024) norm_reduce(const float *__restrict__ pa
   pdl_wait();
   pdl_launch();
   if (!out) return;
-  const float v = column_join<C>(part + blockIdx.y * (long long)cols + c, parts, 2LL * cols, c < cols);
+  const float v = column_join<1024, C>(part + blockIdx.y * (long long)cols + c, parts, 2LL * cols, c < cols);
   if (threadIdx.x < C && c < cols) out[c] = ElemOf<T>::from(v);
 }
 
