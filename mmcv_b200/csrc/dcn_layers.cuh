@@ -219,13 +219,13 @@ __device__ __forceinline__ bool relu_bit(float z) { return !(z <= 0.f); }
 // columns 7.8 us with 32 columns to a block); with many the blocks are enough anyway.
 template <int NT, int C>
 __device__ __forceinline__ float column_join(const float *p, int parts, long long stride, bool live) {
-  constexpr int W = NT / 32, L = 32 / C;   // warps; lanes of a warp to a column
+  constexpr int W = NT / 32, L = 32 / C, kInFlight = NT == 1024 ? 4 : 8;   // warps; lanes of a warp to a column
   static_assert((C == 8 || C == 32) && W % L == 0, "whole warps");
   __shared__ float s[W][C];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float v = 0.f;
   if (live) {
-#pragma unroll 8
+#pragma unroll kInFlight
     for (int q = threadIdx.x / C; q < parts; q += NT / C) v += p[q * stride];
   }
 #pragma unroll
