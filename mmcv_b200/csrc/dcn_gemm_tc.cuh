@@ -500,6 +500,7 @@ __global__ void __launch_bounds__(kThreadsOf<PL>, 1) dcn_gemm_tc(const __grid_co
           }
         } else if (res_staged) {
           chunk_in<TO, RB>(chunk, (const TO *)g.res, g.ldr, i0, m, j0, n, lane);
+          __syncwarp();   // written along columns, read a row to a lane
         }
       };
       const bool takes = load_in || res_staged;

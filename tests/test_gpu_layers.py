@@ -760,3 +760,20 @@ def test_fused_projections_of_the_attention_layer():
     assert torch.allclose(a(q, **kw), b(q, **kw), atol=2e-5)
     b.train()
     assert torch.isfinite(b(q, **kw)).all()     # dropout active: the identity is added outside
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,cout', [(1237, 250, 388), (2500, 264, 384), (4000, 512, 520), (300, 1024, 256)])
+def test_residual_off_16_bytes_gives_the_bits_of_an_aligned_one(rows, cin, cout, dtype):
+    """The residual's element-by-element form (several staging chunks to an epilogue warp) against the tensor
+    load's, and both against the bounds."""
+    x, w, b, r, _ = linear_case(rows, cin, cout, dtype, None)
+    wide = torch.zeros(rows, cout + 9, dtype=dtype, device='cuda')
+    wide[:, 1:1 + cout] = r
+    for act in (None, 'relu', 'gelu'):
+        leaf = w.detach().requires_grad_(True)   # what the backward pass needs is kept: another epilogue
+        y = ops.fused_linear(x, w, b, r, act)
+        hold({'y': y}, plain.linear(x, w, b, r, act))
+        for _ in range(3):
+            assert torch.equal(ops.fused_linear(x, w, b, wide[:, 1:1 + cout], act), y)
+            assert torch.equal(ops.fused_linear(x, leaf, b, wide[:, 1:1 + cout], act).detach(), y)
