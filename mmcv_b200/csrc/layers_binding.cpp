@@ -308,8 +308,9 @@ struct FeedForwardNode final : torch::autograd::Node {
                nb2 = task_should_compute_output(4), inner = nx || nw1 || nb1;
     // bias1's gradient from the hidden gradient before its rounding, in the epilogue of the product that makes
     // it (13 us for 35642 x 1024); from 768 columns on from the rounded one, beside weight1's (2 us): its error
-    // is then that of two roundings, not one.  fp32 gradients are not rounded.
-    const bool early = nb1 && hidden < 768 && gy.scalar_type() != at::kFloat;
+    // is then that of two roundings, not one.  fp32 gradients are not rounded.  Without an activation there is
+    // no such epilogue.
+    const bool early = nb1 && act != DCN_ACT_NONE && hidden < 768 && gy.scalar_type() != at::kFloat;
     {
       const c10::AutoGradMode off(false);
       Tensor gz;

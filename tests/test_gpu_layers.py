@@ -777,3 +777,27 @@ def test_residual_off_16_bytes_gives_the_bits_of_an_aligned_one(rows, cin, cout,
         for _ in range(3):
             assert torch.equal(ops.fused_linear(x, w, b, wide[:, 1:1 + cout], act), y)
             assert torch.equal(ops.fused_linear(x, leaf, b, wide[:, 1:1 + cout], act).detach(), y)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cin,hidden', [(1, 16, 32), (45, 33, 70), (300, 48, 768), (2049, 64, 1000)])
+def test_feed_forward_without_activation(rows, cin, hidden, dtype):
+    """activation=None: all gradients together, and each alone."""
+    x, r, gy = tensors(1, dtype, (rows, cin), (rows, cin), (rows, cin))
+    w1, w2 = tensors(2, dtype, (hidden, cin), (cin, hidden), scale=(cin + hidden) ** -0.5)
+    b1, b2 = tensors(3, dtype, (hidden,), (cin,), scale=0.1)
+    want = plain.feed_forward(x, w1, b1, w2, b2, r, None, gy)
+    # oracle.layers passes the hidden gradient on unrounded where there is no activation; it is stored in the
+    # tensors' type: rounded here, before the products that read it
+    gz = plain.product(plain.Value(gy), plain.Value(w2).t()).rounded(dtype)
+    want['gx'] = plain.product(gz, plain.Value(w1).t()).rounded(dtype)
+    want['gw1'] = plain.product(gz.t(), plain.Value(x).t()).rounded(dtype)
+    want['gb1'] = plain.column_sum(gz).rounded(dtype)
+    names = ('gx', 'gw1', 'gb1', 'gw2', 'gb2')
+    leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2)]
+    y = ops.feed_forward(*leaves, r, None)
+    hold({'y': y.detach(), **dict(zip(names, torch.autograd.grad(y, leaves, gy)))}, want)
+    for only in range(5):
+        parts = [t.detach().requires_grad_(i == only) for i, t in enumerate((x, w1, b1, w2, b2))]
+        g, = torch.autograd.grad(ops.feed_forward(*parts, r, None), parts[only], gy)
+        hold({'g': g}, {'g': want[names[only]]})
