@@ -101,7 +101,7 @@ def cast_weight(t, dtype):
         return t
     if _frozen is None or torch.is_grad_enabled() and t.requires_grad:
         return t.to(dtype)
-    key = (t.data_ptr(), t.dtype, dtype, tuple(t.shape))
+    key = (t.device, t.data_ptr(), t.dtype, dtype, tuple(t.shape), t.stride(), t.is_neg())
     hit = _frozen.casts.get(key)
     if hit is None:
         hit = _frozen.casts[key] = (t, t.detach().to(dtype))

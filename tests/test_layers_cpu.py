@@ -100,3 +100,15 @@ def test_layer_parameters_carry_the_reference_names():
     assert layer.attentions[0].fused_proj and layer.ffns[0].feedforward_channels == 48
     with pytest.raises(ValueError, match='divisible'):
         ops.DeformableEncoderLayer(30, num_heads=4)
+
+
+def test_kept_casts_tell_layouts_apart():
+    """frozen_weights(): a square weight and its transpose, and two views from one start, are different weights."""
+    import mmcv_b200
+    from mmcv_b200 import _ext
+    w = torch.randn(8, 8)
+    with torch.no_grad(), mmcv_b200.frozen_weights():
+        for t in (w, w.t(), w[:4], w[::2], w.t()[:4], torch._neg_view(w)):
+            for _ in range(2):
+                assert torch.equal(_ext.cast_weight(t, torch.bfloat16), t.to(torch.bfloat16))
+        assert _ext.cast_weight(w.t(), torch.bfloat16) is _ext.cast_weight(w.t(), torch.bfloat16)
