@@ -95,6 +95,18 @@ def frozen_weights():
         _frozen = outer
 
 
+def _may_keep(dev):
+    """Whether what the current stream has just been given to make may be kept for later calls.  Not inside a
+    capture: it is made when the graph is replayed, not before.  Otherwise the stream is waited for, once
+    for each thing kept: later calls may come from other streams."""
+    if dev.type == 'cuda':
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                return False
+            torch.cuda.current_stream().synchronize()
+    return True
+
+
 def cast_weight(t, dtype):
     """t in `dtype`; cached while frozen_weights() is active."""
     if t is None or t.dtype == dtype:
@@ -104,7 +116,9 @@ def cast_weight(t, dtype):
     key = (t.device, t.data_ptr(), t.dtype, dtype, tuple(t.shape), t.stride(), t.is_neg())
     hit = _frozen.casts.get(key)
     if hit is None:
-        hit = _frozen.casts[key] = (t, t.detach().to(dtype))
+        hit = (t, t.detach().to(dtype))
+        if _may_keep(t.device):
+            _frozen.casts[key] = hit
     return hit[1]
 
 
@@ -122,7 +136,9 @@ def _weight_image(lib, p, weight, dev, stream):
             image = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
             _lib.check(lib.dcn_prepare_weights(ctypes.byref(p), _ptr(image), nbytes.value,
                                                stream))
-        hit = _frozen.images[key] = (weight, image)
+        hit = (weight, image)
+        if image is None or _may_keep(dev):
+            _frozen.images[key] = hit
     if hit[1] is not None:
         p.weight_image = _ptr(hit[1])
         p.weight_image_bytes = hit[1].numel()

@@ -801,3 +801,57 @@ def test_feed_forward_without_activation(rows, cin, hidden, dtype):
         parts = [t.detach().requires_grad_(i == only) for i, t in enumerate((x, w1, b1, w2, b2))]
         g, = torch.autograd.grad(ops.feed_forward(*parts, r, None), parts[only], gy)
         hold({'g': g}, {'g': want[names[only]]})
+
+
+def test_kept_casts_and_captures():
+    """frozen_weights(): what a capture would make is not kept (an eager call after it would find it unmade),
+    what eager calls have kept serves a capture, and other streams find it complete."""
+    import mmcv_b200
+    from mmcv_b200 import _ext
+    x, w, b, _, _ = linear_case(300, 2048, 4096, torch.float32, None)
+    with torch.no_grad(), torch.autocast('cuda', dtype=torch.bfloat16):
+        want = ops.fused_linear(x, w, b)
+        with mmcv_b200.frozen_weights():
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = ops.fused_linear(x, w, b)
+            assert not _ext._frozen.casts
+            assert torch.equal(ops.fused_linear(x, w, b), want)
+            assert len(_ext._frozen.casts) == 2
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want)
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                ops.fused_linear(x, w, b)
+            assert len(_ext._frozen.casts) == 2
+        for _ in range(3):
+            with mmcv_b200.frozen_weights():
+                one, two = torch.cuda.Stream(), torch.cuda.Stream()
+                torch.cuda.synchronize()
+                with torch.cuda.stream(one):
+                    torch.cuda._sleep(20_000_000)
+                    ops.fused_linear(x, w, b)
+                with torch.cuda.stream(two):
+                    y = ops.fused_linear(x, w, b)
+                torch.cuda.synchronize()
+                assert torch.equal(y, want)
+
+
+def test_kept_weight_images_and_captures():
+    """The same for the convolution's re-laid-out weights."""
+    import mmcv_b200
+    from mmcv_b200 import _ext
+    torch.manual_seed(5)
+    layer = ops.ModulatedDeformConv2dPack(64, 64, 3, padding=1, deform_groups=2).cuda().bfloat16()
+    x = torch.randn(2, 64, 24, 40, device='cuda', dtype=torch.bfloat16)
+    with torch.no_grad():
+        want = layer(x)
+        with mmcv_b200.frozen_weights():
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = layer(x)
+            assert all(image is None for _, image in _ext._frozen.images.values())
+            assert torch.equal(layer(x), want)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want)
