@@ -12,6 +12,7 @@
 #include <tuple>
 #include <vector>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -20,6 +21,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -187,6 +189,16 @@ void refuse_tangents(const char *op, std::initializer_list<const Tensor *> tenso
                 ": forward-mode differentiation is not supported");
 }
 
+// A tracer records dispatched operations, and there is none here: the results of the example's values would
+// stand in the traced program as constants.
+void refuse_tracing(const char *op) {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(Mode::PROXY).has_value() &&
+                  !Modes::get_mode(Mode::FAKE).has_value(),
+              "dcn_b200: ", op, ": tracing is not supported (the traced program would keep this call's values)");
+}
+
 const Tensor &get(const OptTensor &t) {
   static const Tensor none;
   return t.has_value() ? *t : none;
@@ -260,6 +272,7 @@ OptTensor check_residual(const char *op, const Tensor &input, const OptTensor &r
 
 Tensor fused_linear(const Tensor &input, const Tensor &weight, const OptTensor &bias, const OptTensor &residual,
                     int64_t act) {
+  refuse_tracing("fused_linear");
   check_input("fused_linear", input);
   check_weight("fused_linear", "weight", input, input.size(-1), weight);
   check_bias("fused_linear", "bias", input, bias, weight.size(0));
@@ -341,6 +354,7 @@ struct FeedForwardNode final : torch::autograd::Node {
 Tensor feed_forward(const Tensor &input, const Tensor &w1, const OptTensor &b1, const Tensor &w2, const OptTensor &b2,
                     const OptTensor &residual, int64_t act) {
   const char *op = "feed_forward";
+  refuse_tracing(op);
   check_input(op, input);
   check_weight(op, "weight1", input, input.size(-1), w1);
   check_bias(op, "bias1", input, b1, w1.size(0));
@@ -433,6 +447,7 @@ struct NormNode final : torch::autograd::Node {
 Tensor layer_norm(const Tensor &input, const std::vector<int64_t> &shape, const OptTensor &weight,
                   const OptTensor &bias, double eps) {
   const char *op = "layer_norm";
+  refuse_tracing(op);
   check_input(op, input);
   const int64_t n = (int64_t)shape.size();
   TORCH_CHECK(n > 0 && input.dim() >= n && input.sizes().slice(input.dim() - n) == at::IntArrayRef(shape), "dcn_b200: ",

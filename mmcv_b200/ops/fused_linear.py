@@ -21,8 +21,9 @@ def fused_linear(input, weight, bias=None, residual=None, activation=None):
     None, all of one type (float32, bfloat16 or float16) on one CUDA device; activation None,
     'relu' or 'gelu' (the exact form).  Everything is accumulated in fp32 and rounded once.  Under
     autocast, input, weight and bias are cast as ``torch.nn.functional.linear`` casts them, and a
-    residual of another type is added outside the kernel.  Second derivatives and forward-mode
-    differentiation are refused."""
+    residual of another type is added outside the kernel.  Second derivatives, forward-mode
+    differentiation and tracing (torch.jit.trace, make_fx, torch.export) are refused; torch.compile runs
+    the call as it is, between two graphs."""
     act = _layers.activation_code(activation)
     dt = _layers.autocast_dtype()
     if dt is not None:
@@ -35,7 +36,7 @@ def fused_linear(input, weight, bias=None, residual=None, activation=None):
 def feed_forward(input, weight1, bias1, weight2, bias2, residual=None, activation='relu'):
     """``act(input @ weight1.T + bias1) @ weight2.T + bias2 + residual``: the feed-forward block of a
     transformer layer.  weight1 (hidden, in), weight2 (out, hidden); the biases may be None; types,
-    devices, activations and autocast as for ``fused_linear``.  The hidden activations are kept in
+    devices, activations, autocast and refusals as for ``fused_linear``.  The hidden activations are kept in
     the tensors' type.  The gradient between the two products passes the activation's derivative in
     the epilogue of the product that computes it, and is rounded to that type as well.  Pass the input itself as residual (the usual
     identity) and its two gradients come out of one kernel, already added."""

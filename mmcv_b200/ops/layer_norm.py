@@ -14,8 +14,8 @@ def layer_norm(input, normalized_shape, weight=None, bias=None, eps=1e-5):
     """Layer norm of ``input`` over its last ``len(normalized_shape)`` dimensions, statistics in fp32.
     input float32, bfloat16 or float16 on a CUDA device; weight and bias of shape normalized_shape,
     both of input's type or both float32, or None.  The result has input's type; under autocast it
-    is float32, as ``torch.nn.functional.layer_norm`` has it there.  Second derivatives and
-    forward-mode differentiation are refused."""
+    is float32, as ``torch.nn.functional.layer_norm`` has it there.  Second derivatives,
+    forward-mode differentiation and tracing are refused."""
     if isinstance(normalized_shape, numbers.Integral):
         normalized_shape = (int(normalized_shape),)
     if torch.is_autocast_enabled('cuda'):

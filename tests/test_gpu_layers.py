@@ -855,3 +855,26 @@ def test_kept_weight_images_and_captures():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_compile_runs_the_operators_between_its_graphs(backend):
+    """torch.compile breaks its graph at the operators: new inputs give new results, and gradients."""
+    x, w, b, _, _ = linear_case(40, 24, 24, torch.float32, None)
+
+    def f(t):
+        return ops.layer_norm(torch.relu(ops.fused_linear(t * 2, w, b)) * 3, (24,)) + t
+
+    g = torch.compile(f, backend=backend)
+    for seed in (1, 2):
+        a, gy = tensors(seed, torch.float32, (40, 24), (40, 24))
+        leaf, other = a.detach().requires_grad_(True), a.detach().requires_grad_(True)
+        y, want = g(leaf), f(other)
+        assert torch.equal(y, want)
+        assert torch.equal(torch.autograd.grad(y, leaf, gy)[0], torch.autograd.grad(want, other, gy)[0])
+
+
+def test_tracing_is_refused_on_the_device():
+    x, w, b, _, _ = linear_case(40, 24, 24, torch.float32, None)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='tracing is not supported'):
+        torch.jit.trace(lambda t: torch.relu(ops.fused_linear(t, w, b)) * 2, x)

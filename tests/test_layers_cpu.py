@@ -112,3 +112,34 @@ def test_kept_casts_tell_layouts_apart():
             for _ in range(2):
                 assert torch.equal(_ext.cast_weight(t, torch.bfloat16), t.to(torch.bfloat16))
         assert _ext.cast_weight(w.t(), torch.bfloat16) is _ext.cast_weight(w.t(), torch.bfloat16)
+
+
+def traced_calls():
+    return [lambda t: ops.fused_linear(t, t), lambda t: ops.feed_forward(t, t, None, t, None, t),
+            lambda t: ops.layer_norm(t, (4,))]
+
+
+def test_tracing_is_refused():
+    """A traced program would keep the example's results; the check stands before those on devices."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 4)
+    for f in traced_calls():
+        with torch.no_grad(), pytest.raises(RuntimeError, match='tracing is not supported'):
+            torch.jit.trace(lambda t: torch.relu(f(t)) * 2, x)   # noqa: B023
+        for mode in ('real', 'fake'):
+            with pytest.raises(RuntimeError, match='tracing is not supported'):
+                make_fx(lambda t: f(t) * 2 + t, tracing_mode=mode)(x)   # noqa: B023
+
+
+def test_export_is_refused():
+    class Model(torch.nn.Module):
+        def __init__(self, f):
+            super().__init__()
+            self.f = f
+
+        def forward(self, t):
+            return torch.relu(self.f(t)) * 2
+
+    for f in traced_calls():
+        with pytest.raises(RuntimeError, match='tracing is not supported'):
+            torch.export.export(Model(f), (torch.randn(4, 4),), strict=False)
