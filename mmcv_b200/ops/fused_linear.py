@@ -10,7 +10,6 @@ path: CPU tensors raise ``RuntimeError``.
 import torch.nn as nn
 
 from .. import _layers
-from .modulated_deform_conv import register_layer
 
 
 def fused_linear(input, weight, bias=None, residual=None, activation=None):
@@ -72,7 +71,9 @@ class FusedLinear(nn.Linear):
 class FFN(nn.Module):
     """Feed-forward block with identity: Linear, activation, Dropout, Linear, Dropout, and the
     dropout of the residual branch (mmcv/cnn/bricks/transformer.py, class FFN; parameter names
-    ``layers.0.0.*`` and ``layers.1.*``).  While no dropout is active the whole block is
+    ``layers.0.0.*`` and ``layers.1.*``).  It takes a part of what that layer takes, so it does not stand
+    under its registry name: configurations build the layer they always built.  init_cfg is kept and not
+    acted upon.  While no dropout is active the whole block is
     ``feed_forward``; with an active dropout the two products are ``fused_linear`` around it."""
 
     def __init__(self, embed_dims=256, feedforward_channels=1024, num_fcs=2, act_cfg=None, ffn_drop=0.,
@@ -111,6 +112,3 @@ class FFN(nn.Module):
         h = drop1(fused_linear(x, fc1.weight, fc1.bias, None, self.activation))
         out = self.dropout_layer(drop2(fused_linear(h, fc2.weight, fc2.bias)))
         return out if identity is None else identity + out
-
-
-register_layer('FFN', FFN)

@@ -143,3 +143,26 @@ def test_export_is_refused():
     for f in traced_calls():
         with pytest.raises(RuntimeError, match='tracing is not supported'):
             torch.export.export(Model(f), (torch.randn(4, 4),), strict=False)
+
+
+def test_import_leaves_a_registered_ffn_alone():
+    """Configurations that name 'FFN' build what they built before: a stand-in for the registry package."""
+    import os
+    import subprocess
+    import sys
+    code = ("import sys, types\n"
+            "class Registry(dict):\n"
+            "    def register_module(self, name=None, force=False, module=None):\n"
+            "        assert force or name not in self\n"
+            "        self[name] = module\n"
+            "package, registry = types.ModuleType('mmengine'), types.ModuleType('mmengine.registry')\n"
+            "registry.MODELS = package.MODELS = Registry(FFN='theirs')\n"
+            "package.registry = registry\n"
+            "sys.modules.update({'mmengine': package, 'mmengine.registry': registry})\n"
+            "import mmcv_b200.ops\n"
+            "assert registry.MODELS['FFN'] == 'theirs', registry.MODELS\n"
+            "assert {'DCN', 'DCNv2', 'MultiScaleDeformableAttention'} <= set(registry.MODELS)\n"
+            "print('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and 'done' in r.stdout, r.stdout + r.stderr
