@@ -81,11 +81,18 @@ class FFN(nn.Module):
         super().__init__()
         if num_fcs != 2:
             raise ValueError(f'FFN is built for num_fcs=2, but got {num_fcs}')
-        kind = (act_cfg or dict(type='ReLU')).get('type')
+        act_cfg = act_cfg or dict(type='ReLU')
+        kind = act_cfg.get('type')
         if kind not in ('ReLU', 'GELU'):
             raise ValueError(f"FFN takes act_cfg of type 'ReLU' or 'GELU', but got {kind!r}")
-        if dropout_layer is not None and dropout_layer.get('type') != 'Dropout':
-            raise ValueError(f"FFN takes a dropout_layer of type 'Dropout', but got {dropout_layer!r}")
+        # in place or not is the kernels' own affair; whatever else would change the arithmetic
+        if set(act_cfg) - {'type', 'inplace' if kind == 'ReLU' else 'approximate'} or \
+                act_cfg.get('approximate', 'none') != 'none':
+            raise ValueError(f'FFN has ReLU and the exact GELU without further options, but got {act_cfg!r}')
+        if dropout_layer is not None and (dropout_layer.get('type') != 'Dropout' or
+                                          set(dropout_layer) - {'type', 'drop_prob', 'inplace'}):
+            raise ValueError("FFN takes a dropout_layer of type 'Dropout' with drop_prob, "
+                             f'but got {dropout_layer!r}')
         self.embed_dims = embed_dims
         self.feedforward_channels = feedforward_channels
         self.num_fcs = num_fcs

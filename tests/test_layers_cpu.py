@@ -166,3 +166,14 @@ def test_import_leaves_a_registered_ffn_alone():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and 'done' in r.stdout, r.stdout + r.stderr
+
+
+def test_ffn_options_that_it_does_not_have_are_refused():
+    for kw in (dict(act_cfg=dict(type='GELU', approximate='tanh')), dict(act_cfg=dict(type='ReLU', negative_slope=0.1)),
+               dict(act_cfg=dict(type='GELU', inplace=True)), dict(dropout_layer=dict(type='Dropout', p=0.1))):
+        with pytest.raises(ValueError):
+            ops.FFN(4, 8, **kw)
+    for kw in (dict(act_cfg=dict(type='ReLU', inplace=True)), dict(act_cfg=dict(type='GELU', approximate='none')),
+               dict(act_cfg=dict(type='GELU')), dict(dropout_layer=dict(type='Dropout', drop_prob=0.1, inplace=True)),
+               dict(dropout_layer=dict(type='Dropout')), dict(act_cfg={})):
+        ops.FFN(4, 8, **kw)
