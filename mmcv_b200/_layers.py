@@ -9,6 +9,7 @@ import importlib.util
 import os
 
 import torch
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _ext, _lib
 
@@ -45,3 +46,12 @@ def autocast_dtype():
 
 
 cast_weight = _ext.cast_weight
+
+
+def untouched(module, kind):
+    """Whether a call of `module` is `kind`'s forward on its parameters and nothing besides: the very type (no
+    adapter, no parametrization), no hooks, no forward of its own.  Only then may a layer take its child's
+    parameters instead of calling it."""
+    return (type(module) is kind and 'forward' not in module.__dict__ and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or _has_any_global_hook()))

@@ -74,7 +74,8 @@ class FFN(nn.Module):
     ``layers.0.0.*`` and ``layers.1.*``).  It takes a part of what that layer takes, so it does not stand
     under its registry name: configurations build the layer they always built.  init_cfg is kept and not
     acted upon.  While no dropout is active the whole block is
-    ``feed_forward``; with an active dropout the two products are ``fused_linear`` around it."""
+    ``feed_forward``; with an active dropout the two products are ``fused_linear`` around it.  Children
+    that carry hooks, or were replaced or parametrized, are called as they are."""
 
     def __init__(self, embed_dims=256, feedforward_channels=1024, num_fcs=2, act_cfg=None, ffn_drop=0.,
                  dropout_layer=None, add_identity=True, init_cfg=None):
@@ -106,15 +107,27 @@ class FFN(nn.Module):
         self.dropout_layer = (nn.Dropout(dropout_layer.get('drop_prob', 0.5)) if dropout_layer
                               else nn.Identity())
 
+    def _children_as_built(self):
+        kinds = (nn.Linear, nn.ReLU if self.activation == 'relu' else nn.GELU, nn.Dropout)
+        outer, inner = self.layers, self.layers[0]
+        return (_layers.untouched(outer, nn.Sequential) and len(outer) == 3 and
+                _layers.untouched(inner, nn.Sequential) and len(inner) == 3 and
+                _layers.untouched(inner[0], kinds[0]) and _layers.untouched(inner[1], kinds[1]) and
+                getattr(inner[1], 'approximate', 'none') == 'none' and _layers.untouched(outer[1], kinds[0]))
+
     def forward(self, x, identity=None):
-        fc1, _, drop1 = self.layers[0]
-        fc2, drop2 = self.layers[1], self.layers[2]
         if self.add_identity and identity is None:
             identity = x
         if not self.add_identity:
             identity = None
-        p_out = getattr(self.dropout_layer, 'p', 0.)
-        if not self.training or (drop1.p == 0 and drop2.p == 0 and p_out == 0):
+        if not self._children_as_built():
+            out = self.dropout_layer(self.layers(x))
+            return out if identity is None else identity + out
+        fc1, _, drop1 = self.layers[0]
+        fc2, drop2 = self.layers[1], self.layers[2]
+        drops = (drop1, drop2, self.dropout_layer)
+        if (not self.training or all(getattr(d, 'p', 0.) == 0 for d in drops)) and all(
+                _layers.untouched(d, nn.Dropout) or _layers.untouched(d, nn.Identity) for d in drops):
             return feed_forward(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias, identity, self.activation)
         h = drop1(fused_linear(x, fc1.weight, fc1.bias, None, self.activation))
         out = self.dropout_layer(drop2(fused_linear(h, fc2.weight, fc2.bias)))

@@ -15,6 +15,7 @@ import torch.nn as nn
 from torch.autograd.function import Function, once_differentiable
 
 from .. import _ext as ext_module
+from .. import _layers
 from .fused_linear import fused_linear
 from .modulated_deform_conv import register_layer
 
@@ -68,7 +69,8 @@ class MultiScaleDeformableAttention(nn.Module):
 
     fused_proj (not in the reference): the four projections run on this library's matrix product
     (``fused_linear``), the last one with the identity in its epilogue while no dropout is active.
-    The sums are the same, rounded once where the default rounds twice."""
+    The sums are the same, rounded once where the default rounds twice.  A projection that carries hooks,
+    or was replaced or parametrized, is called as it is."""
 
     def __init__(self, embed_dims: int = 256, num_heads: int = 8, num_levels: int = 4,
                  num_points: int = 4, im2col_step: int = 64, dropout: float = 0.1,
@@ -120,7 +122,9 @@ class MultiScaleDeformableAttention(nn.Module):
         self._is_init = True
 
     def _project(self, linear, x):
-        return fused_linear(x, linear.weight, linear.bias) if self.fused_proj else linear(x)
+        if self.fused_proj and _layers.untouched(linear, nn.Linear):
+            return fused_linear(x, linear.weight, linear.bias)
+        return linear(x)
 
     def forward(self, query, key=None, value=None, identity=None, query_pos=None,
                 key_padding_mask=None, reference_points=None, spatial_shapes=None,
@@ -167,7 +171,8 @@ class MultiScaleDeformableAttention(nn.Module):
         output = MultiScaleDeformableAttnFunction.apply(
             value.contiguous(), spatial_shapes, level_start_index, sampling_locations.contiguous(),
             attention_weights.contiguous(), self.im2col_step)
-        if self.fused_proj and (self.dropout.p == 0 or not self.training):
+        if (self.fused_proj and _layers.untouched(self.output_proj, nn.Linear) and
+                _layers.untouched(self.dropout, nn.Dropout) and (self.dropout.p == 0 or not self.training)):
             if not self.batch_first:
                 identity = identity.permute(1, 0, 2)
             output = fused_linear(output, self.output_proj.weight, self.output_proj.bias, identity)

@@ -878,3 +878,88 @@ def test_tracing_is_refused_on_the_device():
     x, w, b, _, _ = linear_case(40, 24, 24, torch.float32, None)
     with torch.no_grad(), pytest.raises(RuntimeError, match='tracing is not supported'):
         torch.jit.trace(lambda t: torch.relu(ops.fused_linear(t, w, b)) * 2, x)
+
+
+class Adapter(torch.nn.Module):
+    """A low-rank addition around a linear layer whose weight and bias it exposes."""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+        self.down = torch.nn.Linear(base.in_features, 2, bias=False)
+        self.up = torch.nn.Linear(2, base.out_features, bias=False)
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + self.up(self.down(x))
+
+
+def altered_children(parent, name):
+    """(what was done, how to undo it) of each way in which users change a child's call."""
+    child = getattr(parent, name)
+    seen = []
+    handle = child.register_forward_hook(lambda m, a, out: out * 2)
+    yield 'hook', handle.remove
+    handle = child.register_forward_pre_hook(lambda m, a: (a[0] + 1,))
+    yield 'pre-hook', handle.remove
+    child.forward = lambda x: torch.nn.functional.linear(x, child.weight) * 3
+    yield 'forward of its own', lambda: delattr(child, 'forward')
+    torch.nn.utils.parametrizations.weight_norm(child)
+    yield 'parametrization', lambda: torch.nn.utils.parametrize.remove_parametrizations(child, 'weight')
+    setattr(parent, name, Adapter(child).cuda())
+    yield 'adapter', lambda: setattr(parent, name, child)
+    handle = torch.nn.modules.module.register_module_forward_hook(
+        lambda m, a, out: out + 1 if m is child else None)
+    yield 'hook on all modules', handle.remove
+    handle = child.register_full_backward_hook(lambda m, gi, go: seen.append(1))
+    yield 'backward hook', handle.remove
+    assert seen
+
+
+def test_children_of_the_block_are_called_where_they_were_changed():
+    torch.manual_seed(0)
+    x, gy = tensors(0, torch.float32, (2, 50, 64), (2, 50, 64))
+    ffn = ops.FFN(64, 96, act_cfg=dict(type='GELU')).cuda()
+    untouched = ffn(x)
+    assert torch.equal(untouched, ops.feed_forward(x, ffn.layers[0][0].weight, ffn.layers[0][0].bias,
+                                                   ffn.layers[1].weight, ffn.layers[1].bias, x, 'gelu'))
+    for parent, name in ((ffn.layers[0], '0'), (ffn.layers, '1')):
+        for what, undo in altered_children(parent, name):
+            leaf = x.detach().requires_grad_(True)
+            y = ffn(leaf)
+            want = leaf + ffn.layers(leaf)
+            assert torch.equal(y, want), (name, what)
+            assert torch.isfinite(torch.autograd.grad(y, leaf, gy)[0]).all()
+            undo()
+        # the weight went through a norm and back: as good as untouched
+        assert torch.allclose(ffn(x), untouched, atol=2e-5)
+    for module in (ffn.layers, ffn.layers[0], ffn.layers[0][1], ffn.layers[2], ffn.dropout_layer):
+        handle = module.register_forward_hook(lambda m, a, out: out * 2)
+        assert torch.allclose(ffn(x), x + ffn.dropout_layer(ffn.layers(x)), atol=1e-4)
+        assert not torch.allclose(ffn(x), untouched, atol=1e-2)
+        handle.remove()
+    ffn.layers[0][1] = torch.nn.SiLU()
+    assert torch.equal(ffn(x), x + ffn.layers(x))
+
+
+def test_projections_of_the_attention_layer_are_called_where_they_were_changed():
+    torch.manual_seed(1)
+    layer = ops.MultiScaleDeformableAttention(64, 4, 2, 3, dropout=0., batch_first=True, fused_proj=True).cuda()
+    q, = tensors(0, torch.float32, (2, 36, 64))
+    kw = dict(reference_points=torch.rand(2, 36, 2, 2, device='cuda'), spatial_shapes=torch.tensor([[6, 5], [3, 2]]).cuda(),
+              level_start_index=torch.tensor([0, 30]).cuda())
+    for name in ('value_proj', 'sampling_offsets', 'attention_weights', 'output_proj'):
+        for what, undo in altered_children(layer, name):
+            leaf = q.detach().requires_grad_(True)
+            y = layer(leaf, **kw)
+            y.sum().backward()
+            layer.fused_proj = False
+            want = layer(q, **kw)
+            layer.fused_proj = True
+            assert torch.allclose(y, want, atol=1e-4), (name, what)
+            undo()
+    handle = layer.dropout.register_forward_hook(lambda m, a, out: out * 0)
+    assert torch.equal(layer(q, **kw), q)
+    handle.remove()
