@@ -9,6 +9,7 @@ import importlib.util
 import os
 
 import torch
+import torch.nn as nn
 from torch.nn.modules.module import _has_any_global_hook
 
 from . import _ext, _lib
@@ -55,3 +56,9 @@ def untouched(module, kind):
     return (type(module) is kind and 'forward' not in module.__dict__ and not (
         module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
         or _has_any_global_hook()))
+
+
+def passes_on(dropout):
+    """Whether `dropout` hands its input on: by its own mode, which need not be its parent's."""
+    return untouched(dropout, nn.Identity) or untouched(dropout, nn.Dropout) and (
+        dropout.p == 0 or not dropout.training)

@@ -125,9 +125,7 @@ class FFN(nn.Module):
             return out if identity is None else identity + out
         fc1, _, drop1 = self.layers[0]
         fc2, drop2 = self.layers[1], self.layers[2]
-        drops = (drop1, drop2, self.dropout_layer)
-        if (not self.training or all(getattr(d, 'p', 0.) == 0 for d in drops)) and all(
-                _layers.untouched(d, nn.Dropout) or _layers.untouched(d, nn.Identity) for d in drops):
+        if all(_layers.passes_on(d) for d in (drop1, drop2, self.dropout_layer)):
             return feed_forward(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias, identity, self.activation)
         h = drop1(fused_linear(x, fc1.weight, fc1.bias, None, self.activation))
         out = self.dropout_layer(drop2(fused_linear(h, fc2.weight, fc2.bias)))

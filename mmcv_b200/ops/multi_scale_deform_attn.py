@@ -171,8 +171,7 @@ class MultiScaleDeformableAttention(nn.Module):
         output = MultiScaleDeformableAttnFunction.apply(
             value.contiguous(), spatial_shapes, level_start_index, sampling_locations.contiguous(),
             attention_weights.contiguous(), self.im2col_step)
-        if (self.fused_proj and _layers.untouched(self.output_proj, nn.Linear) and
-                _layers.untouched(self.dropout, nn.Dropout) and (self.dropout.p == 0 or not self.training)):
+        if self.fused_proj and _layers.untouched(self.output_proj, nn.Linear) and _layers.passes_on(self.dropout):
             if not self.batch_first:
                 identity = identity.permute(1, 0, 2)
             output = fused_linear(output, self.output_proj.weight, self.output_proj.bias, identity)

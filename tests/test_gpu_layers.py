@@ -963,3 +963,27 @@ def test_projections_of_the_attention_layer_are_called_where_they_were_changed()
     handle = layer.dropout.register_forward_hook(lambda m, a, out: out * 0)
     assert torch.equal(layer(q, **kw), q)
     handle.remove()
+
+
+def test_dropouts_go_by_their_own_mode():
+    """Dropouts switched on in a model that evaluates (sampling its uncertainty), or off in one that trains."""
+    torch.manual_seed(0)
+    x, = tensors(0, torch.float32, (2, 36, 64))
+    kw = dict(reference_points=torch.rand(2, 36, 2, 2, device='cuda'), spatial_shapes=torch.tensor([[6, 5], [3, 2]]).cuda(),
+              level_start_index=torch.tensor([0, 30]).cuda())
+    ffn = ops.FFN(64, 96, ffn_drop=0.5, dropout_layer=dict(type='Dropout', drop_prob=0.5)).cuda()
+    att = ops.MultiScaleDeformableAttention(64, 4, 2, 3, dropout=0.5, batch_first=True, fused_proj=True).cuda()
+    for layer, call in ((ffn, lambda: ffn(x)), (att, lambda: att(x, **kw))):
+        drops = [m for m in layer.modules() if isinstance(m, torch.nn.Dropout)]
+        layer.eval()
+        quiet = call()
+        assert torch.equal(call(), quiet)
+        for drop in drops:
+            drop.train()
+            assert not torch.equal(call(), call())
+            drop.eval()
+        layer.train()
+        assert not torch.equal(call(), call())
+        for drop in drops:
+            drop.eval()
+        assert torch.equal(call(), quiet)
