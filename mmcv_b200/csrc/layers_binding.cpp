@@ -320,10 +320,13 @@ struct FeedForwardNode final : torch::autograd::Node {
                nb1 = task_should_compute_output(2), nw2 = task_should_compute_output(3),
                nb2 = task_should_compute_output(4), inner = nx || nw1 || nb1;
     // bias1's gradient from the hidden gradient before its rounding, in the epilogue of the product that makes
-    // it (13 us for 35642 x 1024); from 768 columns on from the rounded one, beside weight1's (2 us): its error
-    // is then that of two roundings, not one.  fp32 gradients are not rounded.  Without an activation there is
-    // no such epilogue.
-    const bool early = nb1 && act != DCN_ACT_NONE && hidden < 768 && gy.scalar_type() != at::kFloat;
+    // it, up to 2^22 hidden values; beyond, where that takes 8 to 13 % of the step, from the rounded one, beside
+    // weight1's: two roundings, not one.  us of a bf16 training step with relu, before / after the rounding: 300 x 256 x 1024
+    // 47.5 / 47.5, 1200 x 256 x 1024 61.8 / 59.8, 4000 x 256 x 1024 68.0 / 65.9, 8000 x 256 x 1024 85.6 / 79.0,
+    // 35642 x 256 x 512 123.7 / 108.5, 35642 x 256 x 1024 187 / 165.  fp32 gradients are not rounded; without an
+    // activation there is no such epilogue.
+    const bool early = nb1 && act != DCN_ACT_NONE && gy.scalar_type() != at::kFloat &&
+                       gy.numel() / gy.size(-1) * hidden <= 1 << 22;
     {
       const c10::AutoGradMode off(false);
       Tensor gz;

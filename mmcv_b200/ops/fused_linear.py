@@ -37,8 +37,9 @@ def feed_forward(input, weight1, bias1, weight2, bias2, residual=None, activatio
     transformer layer.  weight1 (hidden, in), weight2 (out, hidden); the biases may be None; types,
     devices, activations, autocast and refusals as for ``fused_linear``.  The hidden activations are kept in
     the tensors' type.  The gradient between the two products passes the activation's derivative in
-    the epilogue of the product that computes it, and is rounded to that type as well.  Pass the input itself as residual (the usual
-    identity) and its two gradients come out of one kernel, already added."""
+    the epilogue of the product that computes it, and is rounded to that type as well (bias1's
+    gradient is summed before that rounding up to 2^22 hidden values, after it beyond).  Pass the input
+    itself as residual (the usual identity) and its two gradients come out of one kernel, already added."""
     act = _layers.activation_code(activation)
     dt = _layers.autocast_dtype()
     if dt is not None:

@@ -987,3 +987,22 @@ def test_dropouts_go_by_their_own_mode():
         for drop in drops:
             drop.eval()
         assert torch.equal(call(), quiet)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rows,cin,hidden', [(1, 16, 1024), (70, 40, 1000), (300, 48, 2048), (2048, 32, 2048), (2049, 32, 2048),
+                                             (9001, 24, 520)])
+def test_feed_forward_bias_gradient_by_the_number_of_hidden_values(rows, cin, hidden, dtype):
+    """Summed before the hidden gradient's rounding up to 2^22 hidden values, whatever the width; after it
+    beyond."""
+    x, gy = tensors(1, dtype, (rows, cin), (rows, cin))
+    w1, w2 = tensors(2, dtype, (hidden, cin), (cin, hidden), scale=(cin + hidden) ** -0.5)
+    b1, b2 = tensors(3, dtype, (hidden,), (cin,), scale=0.1)
+    z = plain.add(plain.product(plain.Value(x), plain.Value(w1)), b1.double())
+    for act in ('relu', 'gelu'):
+        gz = plain.through(plain.product(plain.Value(gy), plain.Value(w2).t()), z, act, kept=torch.float16)
+        if rows * hidden > 2 ** 22:
+            gz = gz.rounded(dtype)
+        leaf = b1.detach().requires_grad_(True)
+        g, = torch.autograd.grad(ops.feed_forward(x, w1, leaf, w2, b2, None, act), leaf, gy)
+        hold({'gb1': g}, {'gb1': plain.column_sum(gz).rounded(dtype)})
