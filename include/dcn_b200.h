@@ -369,7 +369,8 @@ int dcn_msda_backward(const void *value, const int64_t *spatial_shapes, const in
  *   RELU  uint32 words [rows][(cout + 31) / 32]; bit j % 32 of word j / 32 is set where the
  *         pre-activation is not <= 0;
  *   GELU  the derivative Phi(z) + z phi(z), [rows][(cout + 7) / 8 * 8], 16-byte aligned: fp32 for fp32
- *         tensors, for 16-bit ones uint16 codes (derivative * 2^15 + 2^13 rounded, 65535: NaN);
+ *         tensors, for 16-bit ones uint16 codes: below 37376 the derivative in steps of 2^-15, from
+ *         37376 on a negative one, -2^-30 2^((code - 37376) / 1024) with the fraction linear; 65535: NaN;
  *   NONE  not written.
  *
  * dcn_linear_backward, from gy = dL/dy [rows, cout] (row stride ldgy) and gz = gy * act'(z):

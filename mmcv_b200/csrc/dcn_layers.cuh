@@ -187,20 +187,32 @@ __device__ __forceinline__ float gelu_slope(float z) {
 }
 
 // What is kept of gelu for the backward pass: the derivative.  fp32 tensors keep it as it is.  For 16-bit ones
-// it is a fixed-point number of 16 bits, 2^-15 a step from -0.25 (it lies in -0.13 .. 1.13; 0 and 1 are exact):
-// within 1.6e-5, an eighth of half a step of fp16 at 1, for one instruction each way instead of the
-// derivative's twenty in the backward pass.  65535 stands for NaN.
-//
-// 1.5 * 2^23 + q has q in the low bits of its pattern; a NaN comes out of the multiply-add as 0x7fffffff.
+// it is a code of 16 bits, for a few instructions each way instead of the derivative's twenty in the backward
+// pass:
+//   0 .. 36995      the derivative in steps of 2^-15 (it is at most 1.1290; 0 and 1 are exact): within 2^-16, a
+//                   sixteenth of half a step of fp16 at 1
+//   37376 .. 65057  negative ones (at least -0.1290) as a float of ten mantissa bits from -2^-30 on: within 2^-11
+//                   of the derivative, down to where z is -6.6.  In the steps of 2^-15 it would be 3 % off at z = -4
+//                   and zero from -5 on, and such a unit would no longer learn.
+//   65535           NaN
+// Between 0 and -2^-30 it is 0.
+constexpr uint32_t kNegativeCode = 0x9200u;   // -2^-30
+// the code: the low 16 bits.  1.5 * 2^23 + q has q in the low bits of its pattern; a NaN comes out of the
+// multiply-add as 0x7fffffff.  0xB0800000, the pattern of -2^-30, shifted by 13 ends in 0x8400.
 __device__ __forceinline__ uint32_t slope_code(float slope) {
-  return __float_as_uint(fmaf(slope, 32768.f, 12582912.f + 8192.f));   // the code: the low 16 bits
+  const uint32_t fixed = __float_as_uint(fmaf(slope, 32768.f, 12582912.f));
+  const uint32_t floating = (__float_as_uint(slope) + (((kNegativeCode - 0x8400u) << 13) + 0x1000u)) >> 13;
+  return slope <= -9.31322574615478515625e-10f ? floating : fixed;
 }
 __device__ __forceinline__ uint32_t slope_codes(float lo, float hi) {
   return __byte_perm(slope_code(lo), slope_code(hi), 0x5410);
 }
+// pattern: 0x4B400000, which is 1.5 * 2^23, with the code in its low 16 bits
 __device__ __forceinline__ float slope_of(uint32_t pattern) {
-  const float v = fmaf(__uint_as_float(pattern), 1.f / 32768.f, -384.25f);   // exact
-  return v > 1.5f ? __uint_as_float(0x7fffffffu) : v;
+  const float fixed = fmaf(__uint_as_float(pattern), 1.f / 32768.f, -384.f);   // exact
+  const float floating = __uint_as_float((pattern << 13) + (0xB0800000u - (kNegativeCode << 13)));
+  const float v = pattern >= (0x4B400000u | kNegativeCode) ? floating : fixed;
+  return v < -0.15f ? __uint_as_float(0x7fffffffu) : v;
 }
 __device__ __forceinline__ float slope_of_low(uint32_t codes) { return slope_of(__byte_perm(codes, 0x4B400000u, 0x7610)); }
 __device__ __forceinline__ float slope_of_high(uint32_t codes) { return slope_of(__byte_perm(codes, 0x4B400000u, 0x7632)); }

@@ -1006,3 +1006,58 @@ def test_feed_forward_bias_gradient_by_the_number_of_hidden_values(rows, cin, hi
         leaf = b1.detach().requires_grad_(True)
         g, = torch.autograd.grad(ops.feed_forward(x, w1, leaf, w2, b2, None, act), leaf, gy)
         hold({'gb1': g}, {'gb1': plain.column_sum(gz).rounded(dtype)})
+
+
+def kept_slope_bound(z, dtype):
+    """How far gelu's derivative at z (16-bit tensors, |z| <= 6) may be off as the backward pass has it.  Computed:
+    |z| Phi(-|z|) within 0.0073 of half a step of fp16 (2^-11 of it, at least 2^-25), the density from an
+    exponent of up to 26 with two roundings of 2^-24, and one addition.  Kept: 2^-16 if positive, else 2^-11 of it
+    and 2^-30."""
+    a = z.abs().clamp(min=1e-2)
+    tail = 0.5 * torch.special.erfc(a / 2 ** 0.5)
+    weighted = a * torch.exp(-a * a / 2) / (2 * torch.pi) ** 0.5
+    slope = plain.activation(z, 'gelu')[1]
+    computed = 0.0073 * torch.maximum(2.0 ** -11 * tail, 2.0 ** -25 / a) + 4e-6 * weighted + 2.0 ** -23 * (slope.abs() + tail + weighted)
+    kept = torch.where(slope >= -computed, 2.0 ** -16, 2.0 ** -11 * slope.abs() + 2.0 ** -30)
+    return slope, computed + kept
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rows,cols', [(8, 8), (8, 9), (600, 8), (600, 9), (600, 264), (5000, 72)])
+def test_kept_derivative_of_gelu_keeps_its_digits(rows, cols, dtype):
+    """One element per row with a weight of one: gx is the derivative, rounded once.  Relative precision on the
+    negative side as well, where the derivative falls to 4e-8 (gy lifts it out of fp16's subnormals), through
+    every kernel that keeps or reads it."""
+    z = torch.linspace(-6, 6, rows) if rows > 8 else torch.tensor([-6, -5.5, -5, -4.5, -4, -2, 0.5, 3])
+    x = torch.zeros(rows, cols)
+    x[:, 0] = z
+    x = x.to(dtype).cuda()
+    eye = torch.eye(cols, dtype=dtype, device='cuda')
+    gy = torch.full((rows, cols), 16384.0, dtype=dtype, device='cuda')
+    res = torch.zeros(rows, cols, dtype=dtype, device='cuda')
+    zd = x[:, 0].double()
+    slope, off = kept_slope_bound(zd, dtype)
+    bound = off + plain.half_step(dtype) * (slope.abs() + off) + plain.floor_of(dtype) / 16384
+    for f in (lambda t: ops.fused_linear(t, eye, activation='gelu'), lambda t: ops.fused_linear(t, eye, None, res, 'gelu'),
+              lambda t: ops.feed_forward(t, eye, None, eye, None, None, 'gelu')):
+        leaf = x.detach().requires_grad_(True)
+        gx, = torch.autograd.grad(f(leaf), leaf, gy)
+        over = ((gx[:, 0].double() / 16384 - slope).abs() / bound).max().item()
+        assert over <= 1.0, over
+        assert (gx[:, 0][zd < -1] < 0).all()
+
+
+def test_kept_derivative_of_gelu_beyond_its_range():
+    """Far on the negative side the derivative is 0, far on the positive one 1, and a NaN stays one."""
+    inf = float('inf')
+    z = torch.tensor([-7.0, -20.0, -1e4, -inf, 7.0, 20.0, 1e4, inf, float('nan')])
+    for dtype in (torch.bfloat16, torch.float16):
+        for rows in (9, 300):
+            x = torch.zeros(rows, 8)
+            x[:9, 0] = z
+            x = x.to(dtype).cuda().requires_grad_(True)
+            w = torch.zeros(8, 8, dtype=dtype, device='cuda')
+            w[:, 0] = 1
+            y = ops.fused_linear(x, w, activation='gelu')
+            gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+            assert gx[:8, 0].tolist() == [0, 0, 0, 0, 8, 8, 8, 8] and torch.isnan(gx[8, 0])
