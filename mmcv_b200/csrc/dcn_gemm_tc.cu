@@ -66,16 +66,29 @@ __global__ void __launch_bounds__(256) dcn_column_reduce(const float *__restrict
   if (threadIdx.x < 8 && c < cols) out[c] = ElemOf<T>::from(v);
 }
 
-// x = x1 + x2 + x3, 8 bits each (truncated, so that nothing overflows); an infinity or NaN stays in x1
-__device__ __forceinline__ void split3(float x, uint32_t (&b)[3]) {
-  b[0] = __float_as_uint(x) & 0xffff0000u;
-  const float r1 = x - __uint_as_float(b[0]);
-  const bool finite = (b[0] & 0x7f800000u) != 0x7f800000u;
-  b[1] = finite ? __float_as_uint(r1) & 0xffff0000u : 0u;
-  const float r2 = r1 - __uint_as_float(b[1]);
-  b[2] = finite ? __float_as_uint(r2) & 0xffff0000u : 0u;
-  // a NaN whose payload lies in the low bits must not turn into an infinity
-  if (x != x) b[0] |= 0x00400000u;
+// Two values as x = x1 + x2 + x3 of 8 bits each, exact, rounded to nearest one after another: |x2| <= 2^-8 |x|,
+// |x3| <= 2^-17 |x|, of either sign.  Truncated planes are twice as large and all of x's sign, so that what the
+// product leaves out would add up (7.8 times 2^-24 of |x||y| at worst).  w: a plane's pair, the second value on top.
+// A finite x that would round to infinity is truncated; an infinity or NaN stays in x1, the others are 0.
+// (A product within 2^-7 of fp32's largest value may come out infinite: both leading planes rounded up.)
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&w)[3]) {
+  float rx = x, ry = y;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(ry), "f"(rx));
+    uint32_t bx = w[k] << 16, by = w[k] & 0xffff0000u;
+    if (k == 0) {
+      const bool infx = (bx & 0x7fffffffu) == 0x7f800000u, infy = (by & 0x7fffffffu) == 0x7f800000u;
+      if (infx) bx = __float_as_uint(x) & 0xffff0000u;
+      if (infy) by = __float_as_uint(y) & 0xffff0000u;
+      w[0] = (bx >> 16) | by;
+      rx = (bx & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(bx);
+      ry = (by & 0x7f800000u) == 0x7f800000u ? 0.f : y - __uint_as_float(by);
+    } else {
+      rx -= __uint_as_float(bx);
+      ry -= __uint_as_float(by);
+    }
+  }
 }
 
 constexpr int kStageResident = 3;   // blocks that share an SM: two rows a thread in flight take 80 registers
@@ -144,11 +157,10 @@ __global__ void __launch_bounds__(256, kStageResident) dcn_gemm_stage(const __gr
       uint32_t w[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t lo[3], hi[3];
-        split3(v[2 * i], lo);
-        split3(v[2 * i + 1], hi);
+        uint32_t pair[3];
+        split3(v[2 * i], v[2 * i + 1], pair);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) w[k][i] = (lo[k] >> 16) | hi[k];
+        for (int k = 0; k < 3; ++k) w[k][i] = pair[k];
       }
 #pragma unroll
       for (int k = 0; k < 3; ++k)

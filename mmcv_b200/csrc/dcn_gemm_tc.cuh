@@ -29,7 +29,7 @@
 // 16-bit tensors: one plane (PL = 1).  fp32 tensors: every operand is the exact sum of three bf16
 // planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_stage writes them), and the product is
 //   x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1);
-// what is left out is below 2^-24 of |x||y|.  A tensor core truncates where it adds to its
+// what is left out, x2 y3 + x3 y2 + x3 y3, is at most 2^-24 + 2^-34 of |x||y|, of either sign.  A tensor core truncates where it adds to its
 // accumulator, so long fp32 sums would drift by 2^-24 a step: the leading product and the five small
 // ones have accumulators of their own, and every 256 values of k the epilogue warps take both out
 // into registers, where the additions round to nearest.

@@ -1061,3 +1061,48 @@ def test_kept_derivative_of_gelu_beyond_its_range():
             y = ops.fused_linear(x, w, activation='gelu')
             gx, = torch.autograd.grad(y, x, torch.ones_like(y))
             assert gx[:8, 0].tolist() == [0, 0, 0, 0, 8, 8, 8, 8] and torch.isnan(gx[8, 0])
+
+
+def test_fp32_products_keep_fp32_accuracy_element_by_element():
+    """Sums of one product each, on the tensor cores.  Three planes of 8 bits rounded to nearest leave out at
+    most 2^-24 + 2^-34 of the product; adding the small products to the leading one (exact: 16 bits) rounds by
+    2^-24, the small ones' own sum by five truncations of 2^-23 at 2^-7 of it: 2.5 * 2^-24 in all, and the error has no
+    sign."""
+    rows, cin, cout = 2048, 64, 1024
+    gen = torch.Generator().manual_seed(0)
+
+    def values(n):
+        v = (1 + torch.rand(n, generator=gen)) * torch.where(torch.rand(n, generator=gen) < 0.5, -1.0, 1.0)
+        v[:4] = torch.tensor([0x3f80ffff, 0x3f807fff, 0x3f808001, 0x3fffffff], dtype=torch.int32).view(torch.float32)
+        return v.cuda()
+
+    def check(got, p, q):
+        want = p.double()[:, None] * q.double()[None, :]
+        rel = got.double() / want - 1
+        assert rel.abs().max().item() <= 2.5 * 2.0 ** -24, rel.abs().max().item() * 2 ** 24
+        assert abs(rel.mean().item()) <= 0.1 * 2.0 ** -24, rel.mean().item() * 2 ** 24
+
+    x, w, gy = (torch.zeros(s, device='cuda') for s in ((rows, cin), (cout, cin), (rows, cout)))
+    p, q = values(rows), values(cout)
+    x[:, 3], w[:, 3] = p, q
+    check(ops.fused_linear(x, w), p, q)
+    x = torch.randn(rows, cin, device='cuda').requires_grad_(True)
+    w = torch.zeros(cout, cin, device='cuda')
+    k = values(cin)
+    w[5], gy[:, 5] = k, p
+    check(torch.autograd.grad(ops.fused_linear(x, w), x, gy)[0], p, k)
+    x, gy, w = torch.zeros(rows, cin, device='cuda'), torch.zeros(rows, cout, device='cuda'), w.requires_grad_(True)
+    x[7], gy[7] = k, q
+    check(torch.autograd.grad(ops.fused_linear(x, w), w, gy)[0], q, k)
+
+
+def test_fp32_largest_values():
+    """The largest and the lowest finite value, and a little below, stay what they are."""
+    big = torch.finfo(torch.float32).max
+    x = torch.zeros(2048, 64, device='cuda')
+    x[:, 0] = torch.tensor([big, -big, big / 2 * 1.999, 3.396e38, 3.397e38, 3.39e38, -3.4e38, 1e38]).repeat(256).cuda()
+    w = torch.zeros(1024, 64, device='cuda')
+    w[:, 0] = 1
+    y = ops.fused_linear(x, w)
+    assert torch.isfinite(y).all()
+    assert (y.double() / x[:, :1].double() - 1).abs().max().item() <= 2.5 * 2.0 ** -24
