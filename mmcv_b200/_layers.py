@@ -2,11 +2,12 @@
 (``dcn_linear_*``, ``dcn_layer_norm_*``; mmcv_b200/csrc/layers_binding.cpp): argument checks, row
 strides, workspaces, streams and autograd nodes.  ``mmcv_b200.ops`` documents the operators.
 
-There is no fallback: if the module is missing, importing this one raises.
+There is no fallback: if the module is missing, the first call of such an operator raises.
 """
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 import torch
 import torch.nn as nn
@@ -29,9 +30,20 @@ def _load():
     return module
 
 
-native = _load()
-native.set_check_status(_ext._check_status)
-_ext._status_listeners.append(native.set_check_status)
+_loading = threading.Lock()
+
+
+def __getattr__(name):
+    # `native` at its first use: the convolutions and the sampler need the C library only
+    if name != 'native':
+        raise AttributeError(f'module {__name__!r} has no attribute {name!r}')
+    with _loading:
+        if name not in globals():
+            module = _load()
+            module.set_check_status(_ext._check_status)
+            _ext._status_listeners.append(module.set_check_status)
+            globals()[name] = module
+    return globals()[name]
 
 
 def activation_code(name):

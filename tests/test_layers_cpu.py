@@ -177,3 +177,38 @@ def test_ffn_options_that_it_does_not_have_are_refused():
                dict(act_cfg=dict(type='GELU')), dict(dropout_layer=dict(type='Dropout', drop_prob=0.1, inplace=True)),
                dict(dropout_layer=dict(type='Dropout')), dict(act_cfg={})):
         ops.FFN(4, 8, **kw)
+
+
+def run_python(code):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and 'done' in r.stdout, r.stdout + r.stderr
+
+
+def test_only_the_layer_operators_need_the_tensor_front():
+    """Without it the package imports, other layers are built, and these operators say what is missing."""
+    run_python("import os, torch\n"
+               "real = os.path.exists\n"
+               "os.path.exists = lambda p: '_layers_native' not in str(p) and real(p)\n"
+               "from mmcv_b200 import ops\n"
+               "ops.ModulatedDeformConv2dPack(8, 8, 3), ops.MultiScaleDeformableAttention(32, 4), ops.DeformableEncoderLayer(32, 4)\n"
+               "for f in (lambda: ops.fused_linear(torch.ones(2, 2), torch.ones(2, 2)), lambda: ops.layer_norm(torch.ones(2, 2), 2)):\n"
+               "    try:\n"
+               "        f()\n"
+               "        raise SystemExit('no error')\n"
+               "    except ImportError as e:\n"
+               "        assert 'build_ext' in str(e)\n"
+               "print('done')\n")
+
+
+def test_status_flag_reaches_a_tensor_front_loaded_later():
+    run_python("from mmcv_b200 import _ext, _layers\n"
+               "_ext.set_check_status(True)\n"
+               "assert 'native' not in vars(_layers) and not _ext._status_listeners\n"
+               "_layers.native\n"
+               "assert 'native' in vars(_layers) and len(_ext._status_listeners) == 1\n"
+               "_ext.set_check_status(False)\n"
+               "print('done')\n")
