@@ -1,4 +1,4 @@
-"""Loads ``_layers_native.so``, the C++ tensor front of the transformer-layer entries of the library
+"""Loads ``lib/_layers_native.*.so``, the C++ tensor front of the transformer-layer entries of the library
 (``dcn_linear_*``, ``dcn_layer_norm_*``; mmcv_b200/csrc/layers_binding.cpp): argument checks, row
 strides, workspaces, streams and autograd nodes.  ``mmcv_b200.ops`` documents the operators.
 
@@ -13,10 +13,10 @@ import torch
 import torch.nn as nn
 from torch.nn.modules.module import _has_any_global_hook
 
-from . import _ext, _lib
+from . import _ext, _lib, build_ext
 
 ACTIVATIONS = {None: _lib.ACT_NONE, 'relu': _lib.ACT_RELU, 'gelu': _lib.ACT_GELU}
-NATIVE_PATH = os.path.join(os.path.dirname(_lib.LIB_PATH), '_layers_native.so')
+NATIVE_PATH = build_ext.binding_path()   # of this Python and torch
 
 
 def _load():

@@ -1,5 +1,5 @@
 """Compile the CUDA sources into ``mmcv_b200/lib/libdcn_b200.so`` (sm_100a only) and the tensor front
-of the transformer-layer operators into ``mmcv_b200/lib/_layers_native.so`` (host code, linked against
+of the transformer-layer operators into ``mmcv_b200/lib/_layers_native.<python>-<torch>.so`` (host code, linked against
 torch and that library).
 
 ``python -m mmcv_b200.build_ext [--force] [--verbose]``.  nvcc cross-compiles
@@ -23,7 +23,6 @@ EXTRA_FLAGS = os.environ.get('DCN_B200_NVCC_FLAGS', '').split()   # e.g. -DDCN_T
 
 
 BINDING_SRC = os.path.join(CSRC, 'layers_binding.cpp')
-BINDING = os.path.join(LIB_DIR, '_layers_native.so')
 CXX = os.environ.get('DCN_B200_CXX', 'g++')   # the compiler nvcc uses too: one C++ runtime in the process
 
 
@@ -42,13 +41,21 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
+def binding_path():
+    """The tensor front is linked against one torch and one Python: both are in its name, so that neither
+    another torch's file is taken for this one's nor a build for this one left out."""
+    import torch
+    version = torch.__version__.replace('+', '_')
+    return os.path.join(LIB_DIR, f'_layers_native.{sys.implementation.cache_tag}-torch{version}.so')
+
+
 def build_binding(force=False):
-    """layers_binding.cpp -> _layers_native.so; it calls the C ABI, so only the header and its own source
+    """layers_binding.cpp -> binding_path(); it calls the C ABI, so only the header and its own source
     make it stale."""
     deps = [BINDING_SRC, os.path.join(ROOT, 'include', 'dcn_b200.h')]
-    if not force and os.path.exists(BINDING) and all(
-            os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
-        return BINDING
+    out = binding_path()
+    if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
+        return out
     import sysconfig
     import torch
     from torch.utils import cpp_extension
@@ -59,12 +66,12 @@ def build_binding(force=False):
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}']
     for i in include:
         cmd += ['-isystem', i]
-    cmd += [BINDING_SRC, '-o', BINDING, '-L', LIB_DIR, '-l:libdcn_b200.so', '-L', torch_lib, '-lc10', '-lc10_cuda',
+    cmd += [BINDING_SRC, '-o', out, '-L', LIB_DIR, '-l:libdcn_b200.so', '-L', torch_lib, '-lc10', '-lc10_cuda',
             '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f'{CXX} failed on {BINDING_SRC}:\n{r.stdout}{r.stderr}')
-    return BINDING
+    return out
 
 
 def _compile(src, obj, verbose):

@@ -212,3 +212,19 @@ def test_status_flag_reaches_a_tensor_front_loaded_later():
                "assert 'native' in vars(_layers) and len(_ext._status_listeners) == 1\n"
                "_ext.set_check_status(False)\n"
                "print('done')\n")
+
+
+def test_the_tensor_front_is_this_torch_s():
+    """Another torch (or Python) has a file of its own: it is neither loaded nor counted as built."""
+    import sys
+    from mmcv_b200 import _layers, build_ext
+    assert _layers.NATIVE_PATH == build_ext.binding_path()
+    assert torch.__version__.replace('+', '_') in _layers.NATIVE_PATH and sys.implementation.cache_tag in _layers.NATIVE_PATH
+    run_python("import torch\n"
+               "torch.__version__ = '0.0.1+other'\n"
+               "from mmcv_b200 import _layers\n"
+               "try:\n"
+               "    _layers.native\n"
+               "except ImportError as e:\n"
+               "    assert '0.0.1_other' in str(e) and 'build_ext' in str(e)\n"
+               "    print('done')\n")
