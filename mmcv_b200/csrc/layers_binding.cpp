@@ -189,6 +189,14 @@ void refuse_tangents(const char *op, std::initializer_list<const Tensor *> tenso
                 ": forward-mode differentiation is not supported");
 }
 
+// A view that negates lazily has the opposite sign in memory.
+bool negated(std::initializer_list<const Tensor *> tensors) {
+  for (const Tensor *t : tensors)
+    if (t->defined() && t->is_neg()) return true;
+  return false;
+}
+Tensor resolved(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A tracer records dispatched operations, and there is none here: the results of the example's values would
 // stand in the traced program as constants.
 void refuse_tracing(const char *op) {
@@ -234,7 +242,7 @@ struct LinearNode final : torch::autograd::Node {
       LinearGrads g;
       {
         const c10::AutoGradMode off(false);
-        g = linear_backward(gys[0], x.unpack(), w.unpack(), cin, shape, saved.unpack(), act, want, Tensor(),
+        g = linear_backward(resolved(gys[0]), x.unpack(), w.unpack(), cin, shape, saved.unpack(), act, want, Tensor(),
                             DCN_ACT_NONE, Tensor());
       }
       out = {g.x, g.w, g.b, Tensor()};
@@ -276,6 +284,8 @@ Tensor fused_linear(const Tensor &input, const Tensor &weight, const OptTensor &
   check_input("fused_linear", input);
   check_weight("fused_linear", "weight", input, input.size(-1), weight);
   check_bias("fused_linear", "bias", input, bias, weight.size(0));
+  if (negated({&input, &weight, &get(bias), &get(residual)}))
+    return fused_linear(resolved(input), resolved(weight), resolved(get(bias)), resolved(get(residual)), act);
   const OptTensor res = check_residual("fused_linear", input, residual, weight.size(0));
   refuse_tangents("fused_linear", {&input, &weight, &get(bias), &get(res)});
   const bool grad = at::GradMode::is_enabled(), nx = grad && needs(input), nw = grad && needs(weight),
@@ -314,7 +324,7 @@ struct FeedForwardNode final : torch::autograd::Node {
   variable_list apply(variable_list &&gys) override {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(6);
-    const Tensor &gy = gys[0];
+    const Tensor gy = resolved(gys[0]);
     if (!gy.defined()) return out;
     const bool nx = task_should_compute_output(0), nw1 = task_should_compute_output(1),
                nb1 = task_should_compute_output(2), nw2 = task_should_compute_output(3),
@@ -363,6 +373,11 @@ Tensor feed_forward(const Tensor &input, const Tensor &w1, const OptTensor &b1, 
   check_bias(op, "bias1", input, b1, w1.size(0));
   check_weight(op, "weight2", input, w1.size(0), w2);
   check_bias(op, "bias2", input, b2, w2.size(0));
+  if (negated({&input, &w1, &get(b1), &w2, &get(b2), &get(residual)})) {
+    const Tensor x = resolved(input);
+    return feed_forward(x, resolved(w1), resolved(get(b1)), resolved(w2), resolved(get(b2)),
+                        has(residual) && residual->is_same(input) ? x : resolved(get(residual)), act);
+  }
   const bool identity = has(residual) && residual->is_same(input) && w2.size(0) == input.size(-1);
   const OptTensor res = identity ? OptTensor() : check_residual(op, input, residual, w2.size(0));
   refuse_tangents(op, {&input, &w1, &get(b1), &w2, &get(b2), &get(res)});
@@ -433,7 +448,7 @@ struct NormNode final : torch::autograd::Node {
       if (task_should_compute_output(0)) out[0] = make(in.sizes(), in.scalar_type(), in);
       if (task_should_compute_output(1)) out[1] = make(shape, type, in);
       if (task_should_compute_output(2)) out[2] = make(shape, type, in);
-      const Rows gr(gys[0], cols), xr(in, cols);
+      const Rows gr(resolved(gys[0]), cols), xr(in, cols);
       size_t bytes = 0;
       if (out[1].defined() || out[2].defined()) check(dcn_layer_norm_workspace_bytes(xr.rows, cols, &bytes));
       const Tensor ws = workspace(in, bytes);
@@ -470,6 +485,8 @@ Tensor layer_norm(const Tensor &input, const std::vector<int64_t> &shape, const 
   }
   TORCH_CHECK(!has(weight) || !has(bias) || weight->scalar_type() == bias->scalar_type(), "dcn_b200: ", op,
               ": weight and bias have different dtypes");
+  if (negated({&input, &get(weight), &get(bias)}))
+    return layer_norm(resolved(input), shape, resolved(get(weight)), resolved(get(bias)), eps);
   const OptTensor w = has(weight) ? OptTensor(weight->contiguous()) : OptTensor();
   const OptTensor b = has(bias) ? OptTensor(bias->contiguous()) : OptTensor();
   refuse_tangents(op, {&input, &get(w), &get(b)});

@@ -1106,3 +1106,31 @@ def test_fp32_largest_values():
     y = ops.fused_linear(x, w)
     assert torch.isfinite(y).all()
     assert (y.double() / x[:, :1].double() - 1).abs().max().item() <= 2.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_lazily_negated_views_have_their_sign(dtype):
+    """Inputs, parameters, residuals and gradients whose memory holds the opposite sign."""
+    lazy = torch._neg_view
+    x, gy, w1, b1, w2, b2, g, b = block_inputs(dtype)
+    half = lazy(x)
+    assert half.is_neg() and torch.equal(half, -x)
+    cases = [(lambda n, t, w, c, r: ops.fused_linear(n(t), n(w), n(c), n(r), 'gelu'), (x, w1, b1, gy.new_ones(70, 96))),
+             (lambda n, t, w, c, r: ops.feed_forward(n(t), n(w), n(c), n(r), None, None, 'gelu'), (x, w1, b1, w2)),
+             (lambda n, t, w, c, r: ops.feed_forward(t, n(w), n(c), n(r), None, t), (lazy(x), w1, b1, w2)),
+             (lambda n, t, w, c, r: ops.layer_norm(n(t), (64,), n(w), n(c)) + r, (x, g, b, x)),
+             (lambda n, t, w, c, r: ops.fused_linear(n(t), n(w), n(c)) + r, (x[:, :1], w1[:, :1], b1, gy.new_ones(70, 96)))]
+    for f, given in cases:
+        out = []
+        for n, flip in ((lambda t: -t, lambda t: -t), (lazy, lazy)):
+            leaves = [t.detach().clone().requires_grad_(True) if not t.is_neg() else t.detach().requires_grad_(True)
+                      for t in given]
+            y = f(n, *leaves)
+            dy = tensors(8, dtype, y.shape)[0]
+            out.append([y.detach(), *torch.autograd.grad(y, leaves, flip(dy))])
+        assert all(torch.equal(p, q) for p, q in zip(*out))
+    w = torch.randn(1, 64, device='cuda')       # a gradient of one column that autograd itself negates lazily
+    leaf = torch.randn(70, 64, device='cuda', requires_grad=True)
+    y = ops.fused_linear(leaf, w)
+    torch.complex(y * 0, y).conj().imag.sum().backward()
+    assert torch.equal(leaf.grad, -w.expand(70, 64))
