@@ -58,7 +58,16 @@ def autocast_dtype():
     return torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else None
 
 
-cast_weight = _ext.cast_weight
+_CAST = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def autocast(t, dtype):
+    """t as an active autocast hands it on: fp64 and whole numbers stay, and are refused, as without it."""
+    return t.to(dtype) if t is not None and t.dtype in _CAST else t
+
+
+def autocast_weight(t, dtype):
+    return _ext.cast_weight(t, dtype) if t is not None and t.dtype in _CAST else t
 
 
 def untouched(module, kind):

@@ -26,7 +26,8 @@ def fused_linear(input, weight, bias=None, residual=None, activation=None):
     act = _layers.activation_code(activation)
     dt = _layers.autocast_dtype()
     if dt is not None:
-        input, weight, bias = input.to(dt), _layers.cast_weight(weight, dt), _layers.cast_weight(bias, dt)
+        input = _layers.autocast(input, dt)
+        weight, bias = _layers.autocast_weight(weight, dt), _layers.autocast_weight(bias, dt)
         if residual is not None and residual.dtype != dt:
             return fused_linear(input, weight, bias, None, activation) + residual
     return _layers.native.fused_linear(input, weight, bias, residual, act)
@@ -44,8 +45,8 @@ def feed_forward(input, weight1, bias1, weight2, bias2, residual=None, activatio
     dt = _layers.autocast_dtype()
     if dt is not None:
         same = residual is input
-        input = input.to(dt)
-        weight1, bias1, weight2, bias2 = (_layers.cast_weight(t, dt) for t in (weight1, bias1, weight2, bias2))
+        input = _layers.autocast(input, dt)
+        weight1, bias1, weight2, bias2 = (_layers.autocast_weight(t, dt) for t in (weight1, bias1, weight2, bias2))
         if residual is not None and residual.dtype != dt:
             return feed_forward(input, weight1, bias1, weight2, bias2, None, activation) + residual
         if same:

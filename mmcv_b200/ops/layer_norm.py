@@ -19,9 +19,7 @@ def layer_norm(input, normalized_shape, weight=None, bias=None, eps=1e-5):
     if isinstance(normalized_shape, numbers.Integral):
         normalized_shape = (int(normalized_shape),)
     if torch.is_autocast_enabled('cuda'):
-        input = input.float()
-        weight = None if weight is None else weight.float()
-        bias = None if bias is None else bias.float()
+        input, weight, bias = (_layers.autocast(t, torch.float32) for t in (input, weight, bias))
     return _layers.native.layer_norm(input, normalized_shape, weight, bias, eps)
 
 

@@ -1134,3 +1134,20 @@ def test_lazily_negated_views_have_their_sign(dtype):
     y = ops.fused_linear(leaf, w)
     torch.complex(y * 0, y).conj().imag.sum().backward()
     assert torch.equal(leaf.grad, -w.expand(70, 64))
+
+
+def test_autocast_leaves_other_types_to_their_refusal():
+    """autocast does not touch fp64 or whole numbers; the operators refuse them there as elsewhere."""
+    x, w, b, r, _ = linear_case(20, 24, 24, torch.float32, None)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        for t in (x.double(), x.int(), x.bool()):
+            for f in (lambda: ops.fused_linear(t, w), lambda: ops.fused_linear(x, t), lambda: ops.fused_linear(x, w, t[0]),
+                      lambda: ops.feed_forward(t, w, b, w, b), lambda: ops.feed_forward(x, w, b, t, b),
+                      lambda: ops.layer_norm(t, (24,)), lambda: ops.layer_norm(x, (24,), t[0])):
+                with pytest.raises(RuntimeError, match='dtype'):
+                    f()
+        assert ops.fused_linear(x.half(), w, b).dtype == torch.bfloat16
+        # a residual of another type is added outside, whatever it is
+        y = ops.fused_linear(x, w, b, r.double())
+        assert y.dtype == torch.float64
+        assert torch.equal(y, ops.fused_linear(x, w, b) + r.double())
