@@ -23,16 +23,16 @@
 // loops of four steps only (35642 x 256 x 1024 bf16 with relu: 42 us with eight warps, 28 with sixteen).
 // Every wait is bounded.
 //
-// Measured: 8192 x 4096 x 4096 bf16 171 us, 1.61 PFLOP/s, the tensor pipe 88 % busy; 35642 x 256 x 1024 28 us
+// Measured: 8192 x 4096 x 4096 bf16 171 us, 1.61 PFLOP/s, the tensor pipe 87 % busy; 35642 x 256 x 1024 28 us
 // (its bytes 14 us at the copy rate), bound by the epilogue's chain.
 //
 // 16-bit tensors: one plane (PL = 1).  fp32 tensors: every operand is the exact sum of three bf16
 // planes x = x1 + x2 + x3 of 8 bits each (dcn_gemm_stage writes them), and the product is
 //   x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1);
-// what is left out, x2 y3 + x3 y2 + x3 y3, is at most 2^-24 + 2^-34 of |x||y|, of either sign.  A tensor core truncates where it adds to its
-// accumulator, so long fp32 sums would drift by 2^-24 a step: the leading product and the five small
-// ones have accumulators of their own, and every 256 values of k the epilogue warps take both out
-// into registers, where the additions round to nearest.
+// what is left out, x2 y3 + x3 y2 + x3 y3, is at most 2^-24 + 2^-34 of |x||y|, of either sign.
+// A tensor core truncates where it adds to its accumulator, so long fp32 sums would drift by 2^-24 a step:
+// the leading product and the five small ones have accumulators of their own, and every 256 values of k the
+// epilogue warps take both out into registers, where the additions round to nearest.
 //
 // The weight gradient's sum over the rows is cut into `splits` ranges when its tiles alone do not
 // fill the SMs; the fp32 parts are added in order by dcn_gemm_reduce.  With 16-bit tensors its bias gradient

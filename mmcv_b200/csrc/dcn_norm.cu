@@ -11,7 +11,7 @@
 // Both passes read each tensor once: a row (up to 8192 columns) lives in the registers of a group of G
 // threads, 4 to 256, E elements to a thread, loaded 16 bytes at a time (one element at a time where sizes or
 // alignment forbid it).  Bound: memory for fp32 (35642 x 256 forward 11.7 us, its bytes 11.1 at the copy rate),
-// instructions and the latency of short rows for 16 bits (bf16 8.8 us, bytes 5.6).
+// instructions and the latency of short rows for 16 bits (bf16 8.6 us, bytes 5.6; 64 % of the issue slots).
 // The backward pass keeps gw and gb in registers over all rows that a group takes, adds the groups of
 // a block in order, writes one partial row per block, and a second kernel adds those in order: the
 // result does not depend on when blocks run (35642 x 256 bf16: 17.6 us with both kernels, 11.8 for gx alone,
@@ -490,7 +490,8 @@ cudaError_t run_backward(const NormArgs &a, bool params, int *parts, cudaStream_
 // Elements to a thread and threads to a row.
 //
 // Forward: two loads of 16 bytes while that keeps a row within a warp (35642 x 64 bf16: 3.9 us against 11.3 us
-// with a warp to each row; 35642 x 256 bf16: 9.5 us, with one load 11.5, with four 10.6), 32 elements beyond
+// with a warp to each row; 35642 x 256 bf16, before the arithmetic went two elements at a time: 9.5 us, with one
+// load 11.5, with four 10.6), 32 elements beyond
 // (20000 x 768 bf16 16.8 us, with two loads 20.3; 5000 x 1536 10.0 us, with one load 13.8).  Keeping the
 // parameters in registers over several rows, with the next row's loads ahead, was slower everywhere
 // (35642 x 256 fp32 25 us against 11.6).  One element at a time: a warp's lanes side by side, for the sake of

@@ -73,7 +73,8 @@ def apply(z, act):
 
 
 def through(g, z, act, kept=None):
-    """g * act'(z); `kept`: the type to which z was rounded before its derivative was taken."""
+    """g * act'(z); `kept`: what the forward pass keeps for the derivative is bounded by z's rounding to that
+    type."""
     _, d, _, curve = activation(z.v, act)
     ez = z.e if kept is None else z.rounded(kept).e
     if act == 'relu':
