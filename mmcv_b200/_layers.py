@@ -70,16 +70,22 @@ def autocast_weight(t, dtype):
     return _ext.cast_weight(t, dtype) if t is not None and t.dtype in _CAST else t
 
 
-def untouched(module, kind):
-    """Whether a call of `module` is `kind`'s forward on its parameters and nothing besides: the very type (no
-    adapter, no parametrization), no hooks, no forward of its own.  Only then may a layer take its child's
-    parameters instead of calling it."""
-    return (type(module) is kind and 'forward' not in module.__dict__ and not (
-        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
-        or _has_any_global_hook()))
+def untouched(*pairs):
+    """Whether, for each (module, kind), a call of the module is `kind`'s forward on its parameters and nothing
+    besides: the very type (no adapter, no parametrization), no hooks, no forward of its own.  Only then may a
+    layer take its child's parameters instead of calling it."""
+    if _has_any_global_hook():
+        return False
+    for module, kind in pairs:
+        if type(module) is not kind or 'forward' in module.__dict__ or module._forward_hooks or \
+                module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+            return False
+    return True
 
 
-def passes_on(dropout):
-    """Whether `dropout` hands its input on: by its own mode, which need not be its parent's."""
-    return untouched(dropout, nn.Identity) or untouched(dropout, nn.Dropout) and (
-        dropout.p == 0 or not dropout.training)
+def passes_on(*dropouts):
+    """Whether dropouts hand their input on: by their own mode, which need not be their parent's."""
+    for drop in dropouts:
+        if type(drop) is nn.Dropout and drop.p and drop.training:
+            return False
+    return untouched(*((drop, nn.Identity if type(drop) is nn.Identity else nn.Dropout) for drop in dropouts))

@@ -109,25 +109,31 @@ class FFN(nn.Module):
         self.dropout_layer = (nn.Dropout(dropout_layer.get('drop_prob', 0.5)) if dropout_layer
                               else nn.Identity())
 
-    def _children_as_built(self):
-        kinds = (nn.Linear, nn.ReLU if self.activation == 'relu' else nn.GELU, nn.Dropout)
-        outer, inner = self.layers, self.layers[0]
-        return (_layers.untouched(outer, nn.Sequential) and len(outer) == 3 and
-                _layers.untouched(inner, nn.Sequential) and len(inner) == 3 and
-                _layers.untouched(inner[0], kinds[0]) and _layers.untouched(inner[1], kinds[1]) and
-                getattr(inner[1], 'approximate', 'none') == 'none' and _layers.untouched(outer[1], kinds[0]))
+    def _as_built(self):
+        """(fc1, dropout, fc2, dropout) while the children are those of the constructor, else None."""
+        kind = nn.ReLU if self.activation == 'relu' else nn.GELU
+        if type(self.layers) is not nn.Sequential or len(self.layers._modules) != 3:
+            return None
+        inner, fc2, drop2 = self.layers._modules.values()
+        if type(inner) is not nn.Sequential or len(inner._modules) != 3:
+            return None
+        fc1, act, drop1 = inner._modules.values()
+        if not _layers.untouched((self.layers, nn.Sequential), (inner, nn.Sequential), (fc1, nn.Linear), (act, kind),
+                                 (fc2, nn.Linear)) or kind is nn.GELU and act.approximate != 'none':
+            return None
+        return fc1, drop1, fc2, drop2
 
     def forward(self, x, identity=None):
         if self.add_identity and identity is None:
             identity = x
         if not self.add_identity:
             identity = None
-        if not self._children_as_built():
+        parts = self._as_built()
+        if parts is None:
             out = self.dropout_layer(self.layers(x))
             return out if identity is None else identity + out
-        fc1, _, drop1 = self.layers[0]
-        fc2, drop2 = self.layers[1], self.layers[2]
-        if all(_layers.passes_on(d) for d in (drop1, drop2, self.dropout_layer)):
+        fc1, drop1, fc2, drop2 = parts
+        if _layers.passes_on(drop1, drop2, self.dropout_layer):
             return feed_forward(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias, identity, self.activation)
         h = drop1(fused_linear(x, fc1.weight, fc1.bias, None, self.activation))
         out = self.dropout_layer(drop2(fused_linear(h, fc2.weight, fc2.bias)))

@@ -122,7 +122,7 @@ class MultiScaleDeformableAttention(nn.Module):
         self._is_init = True
 
     def _project(self, linear, x):
-        if self.fused_proj and _layers.untouched(linear, nn.Linear):
+        if self.fused_proj and _layers.untouched((linear, nn.Linear)):
             return fused_linear(x, linear.weight, linear.bias)
         return linear(x)
 
@@ -171,7 +171,7 @@ class MultiScaleDeformableAttention(nn.Module):
         output = MultiScaleDeformableAttnFunction.apply(
             value.contiguous(), spatial_shapes, level_start_index, sampling_locations.contiguous(),
             attention_weights.contiguous(), self.im2col_step)
-        if self.fused_proj and _layers.untouched(self.output_proj, nn.Linear) and _layers.passes_on(self.dropout):
+        if self.fused_proj and _layers.untouched((self.output_proj, nn.Linear)) and _layers.passes_on(self.dropout):
             if not self.batch_first:
                 identity = identity.permute(1, 0, 2)
             output = fused_linear(output, self.output_proj.weight, self.output_proj.bias, identity)

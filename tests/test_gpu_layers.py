@@ -943,6 +943,22 @@ def test_children_of_the_block_are_called_where_they_were_changed():
         handle.remove()
     ffn.layers[0][1] = torch.nn.SiLU()
     assert torch.equal(ffn(x), x + ffn.layers(x))
+    ffn.layers[0] = torch.nn.Linear(64, 96).cuda()
+    assert torch.equal(ffn(x), x + ffn.layers(x))
+    ffn.layers = torch.nn.Identity()
+    assert torch.equal(ffn(x), x + x)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_feed_forward_of_no_rows(dtype):
+    _, _, w1, b1, w2, b2, _, _ = block_inputs(dtype)
+    x = w1.new_empty(3, 0, 64)
+    for act in (None, 'relu', 'gelu'):
+        for same in (False, True):
+            leaves = [t.detach().requires_grad_(True) for t in (x, w1, b1, w2, b2)]
+            y = ops.feed_forward(*leaves, leaves[0] if same else None, act)
+            grads = torch.autograd.grad(y, leaves, torch.empty_like(y))
+            assert y.shape == grads[0].shape == (3, 0, 64) and not any(g.any() for g in grads[1:])
 
 
 def test_projections_of_the_attention_layer_are_called_where_they_were_changed():
